@@ -1,0 +1,422 @@
+// mws_conv.hip -- the short causal convolution over tokens with its activation: forward, backward, one token.
+//
+//   s_t = b + sum_j w_j x_{t-K+1+j}, y_t = s_t sigmoid(s_t); ds_t = dy_t silu'(s_t)
+//   dx_p = sum_j w_j ds_{p+K-1-j}, dw_j = sum_t ds_t x_{t-K+1+j}, db = sum_t ds_t
+//
+// where x of a token before the row's first comes from the state, and of one before the episode's first is zero.
+//
+// Bound by memory.  A lane keeps V neighbouring channels (one 16-byte access a token), a wave walks over a tile of tokens with the
+// last K of them in registers, so that every value is read once but for K - 1 tokens at a tile's edge.  The episodes' beginnings
+// of a tile are one 64-bit mask in scalar registers.
+#include "mws_common.hpp"
+
+namespace mws {
+
+struct ConvArgs {
+    const void *x, *weight, *bias, *state, *dy, *dlast;
+    const uint8_t *reset;
+    const int32_t *lengths;
+    void *y, *last, *dx, *dstate;
+    float *part;                 // [blocks over tiles][K + 1][width]
+    int64_t batch, length, tiles;
+    int64_t x_batch, x_time, dy_batch, dy_time, reset_batch, reset_time;
+    int width, tile;             // tokens of one wave's walk
+    bool wide;
+};
+
+constexpr int kMostTile = 32;    // a tile with the tokens around it that matter to it fits one 64-bit mask
+
+__device__ __forceinline__ int64_t row_length(const int32_t *lengths, int64_t b, int64_t length) {
+    if (lengths == nullptr) return length;
+    int64_t n = lengths[b];
+    return n < 0 ? 0 : n > length ? length : n;
+}
+
+// bit i: an episode begins at token from + i (i < count, tokens within [0, end))
+__device__ __forceinline__ uint64_t reset_mask(const uint8_t *reset, int64_t at, int64_t stride, int64_t from, int count, int64_t end) {
+    if (reset == nullptr) return 0;
+    int lane = threadIdx.x % kWave;
+    int64_t t = from + lane;
+    return __ballot(lane < count && t >= 0 && t < end && reset[at + t * stride] != 0);
+}
+
+template <class T, int V> struct Chan {
+    float v[V];
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < V; i++) v[i] = 0;
+    }
+    __device__ __forceinline__ void set(const Vec<T, V> &r) {
+#pragma unroll
+        for (int i = 0; i < V; i++) v[i] = up<T>(r.v[i]);
+    }
+    __device__ __forceinline__ Vec<T, V> rounded() const {
+        Vec<T, V> r;
+#pragma unroll
+        for (int i = 0; i < V; i++) r.v[i] = down<T>(v[i]);
+        return r;
+    }
+};
+
+template <class T, int V, int K> __device__ __forceinline__ void taps(const ConvArgs &a, int e, Chan<T, V> (&w)[K], Chan<T, V> &b) {
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        bool on = e + i < a.width;
+#pragma unroll
+        for (int j = 0; j < K; j++) w[j].v[i] = on ? param<T>(a.weight, (int64_t)(e + i) * K + j, a.wide) : 0.0f;
+        b.v[i] = on && a.bias != nullptr ? param<T>(a.bias, e + i, a.wide) : 0.0f;
+    }
+}
+
+// the input at token p of row b (p >= -(K - 1); below zero: the state)
+template <class T, int V, int K> __device__ __forceinline__ Vec<T, V> input(const ConvArgs &a, int64_t b, int64_t p, int e, int n) {
+    using raw = typename T::raw;
+    if (p >= 0) return load_some<T, V>((const raw *)a.x + b * a.x_batch + p * a.x_time + e, n);
+    if (a.state != nullptr) return load_some<T, V>((const raw *)a.state + (b * (K - 1) + p + K - 1) * a.width + e, n);
+    Vec<T, V> r;
+#pragma unroll
+    for (int i = 0; i < V; i++) r.v[i] = 0;
+    return r;
+}
+
+template <class T, int V, int K> __global__ __launch_bounds__(256) void conv_forward(ConvArgs a) {
+    using raw = typename T::raw;
+    int lane = threadIdx.x % kWave, e = (blockIdx.y * kWave + lane) * V, n = a.width - e;
+    int64_t item = (int64_t)blockIdx.x * (blockDim.x / kWave) + uniform(threadIdx.x / kWave);
+    if (item >= a.batch * a.tiles) return;
+    int64_t b = item / a.tiles, t0 = (item % a.tiles) * a.tile, t1 = t0 + a.tile < a.length ? t0 + a.tile : a.length;
+    int64_t end = row_length(a.lengths, b, a.length), stop = t1 < end ? t1 : end;
+    if (n <= 0) e = 0;
+    Chan<T, V> w[K], bias, x[K];
+    taps<T, V, K>(a, e, w, bias);
+    raw *y = (raw *)a.y + (b * a.length) * a.width + e;
+    // bit i: token t0 - (K - 1) + i
+    uint64_t begins = reset_mask(a.reset, b * a.reset_batch, a.reset_time, t0 - (K - 1), a.tile + K - 1, end);
+    if (t0 < stop) {
+        x[0].zero();
+#pragma unroll
+        for (int j = 1; j < K; j++) {
+            x[j].set(input<T, V, K>(a, b, t0 - K + j, e, n));
+            if (begins >> (j - 1) & 1)
+#pragma unroll
+                for (int i = 0; i < j; i++) x[i].zero();
+        }
+        begins >>= K - 1;
+        for (int64_t t = t0; t < stop; t += 4) {
+            Vec<T, V> in[4];
+#pragma unroll
+            for (int q = 0; q < 4; q++) in[q] = input<T, V, K>(a, b, t + q < stop ? t + q : stop - 1, e, n);
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                if (t + q >= stop) break;
+#pragma unroll
+                for (int j = 0; j + 1 < K; j++) x[j] = x[j + 1];
+                if (begins >> q & 1)
+#pragma unroll
+                    for (int j = 0; j + 1 < K; j++) x[j].zero();
+                x[K - 1].set(in[q]);
+                Chan<T, V> s = bias;
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+#pragma unroll
+                    for (int j = 0; j < K; j++) s.v[i] += w[j].v[i] * x[j].v[i];
+                    s.v[i] *= sigmoid_(s.v[i]);
+                }
+                if (n > 0) store_some<T, V>(y + (t + q) * a.width, s.rounded(), n);
+            }
+            begins >>= 4;
+        }
+    }
+    Vec<T, V> none;
+#pragma unroll
+    for (int i = 0; i < V; i++) none.v[i] = 0;
+    for (int64_t t = t0 > end ? t0 : end; t < t1; t++)
+        if (n > 0) store_some<T, V>(y + t * a.width, none, n);
+    // the state after the last token: the inputs of its episode among the last K - 1, by the tile that holds this token
+    if (a.last != nullptr && t0 == (end > 0 ? (end - 1) / a.tile : 0) * a.tile) {
+        uint64_t tail = reset_mask(a.reset, b * a.reset_batch, a.reset_time, end - (K - 1), K - 1, end);
+#pragma unroll
+        for (int j = 0; j + 1 < K; j++) {
+            bool seen = (tail >> (j + 1)) == 0;          // none begins after token end - (K - 1) + j
+            Vec<T, V> r = seen ? input<T, V, K>(a, b, end - (K - 1) + j, e, n) : none;
+            if (n > 0) store_some<T, V>((raw *)a.last + (b * (K - 1) + j) * a.width + e, r, n);
+        }
+    }
+}
+
+// A wave walks from its tile's first token to K - 1 tokens past it: it takes dw and db of its own tokens, and dx of them, whose last
+// terms come from the tokens past the tile.  The state's K - 1 inputs count as tokens before the first.
+template <class T, int V, int K> __global__ __launch_bounds__(256) void conv_backward(ConvArgs a) {
+    using raw = typename T::raw;
+    int lane = threadIdx.x % kWave, e = (blockIdx.y * kWave + lane) * V, n = a.width - e, wave = uniform(threadIdx.x / kWave), waves = blockDim.x / kWave;
+    if (n <= 0) e = 0;
+    Chan<T, V> w[K], bias, dw[K], db;
+    taps<T, V, K>(a, e, w, bias);
+#pragma unroll
+    for (int j = 0; j < K; j++) dw[j].zero();
+    db.zero();
+    for (int64_t item = (int64_t)blockIdx.x * waves + wave; item < a.batch * a.tiles; item += (int64_t)gridDim.x * waves) {
+        int64_t b = item / a.tiles, t0 = (item % a.tiles) * a.tile, t1 = t0 + a.tile < a.length ? t0 + a.tile : a.length;
+        int64_t end = row_length(a.lengths, b, a.length), stop = t1 + K - 1 < end ? t1 + K - 1 : end, own = t1 < end ? t1 : end;
+        uint64_t begins = reset_mask(a.reset, b * a.reset_batch, a.reset_time, t0 - (K - 1), a.tile + 2 * (K - 1), end);
+        uint64_t tail = reset_mask(a.reset, b * a.reset_batch, a.reset_time, end - (K - 1), K - 1, end);
+        Chan<T, V> x[K], pend[K];
+        x[0].zero();
+#pragma unroll
+        for (int j = 0; j < K; j++) pend[j].zero();
+        int age = K;                                     // tokens since the episode's first
+        raw *dx = (raw *)a.dx + b * a.length * a.width + e, *dstate = (raw *)a.dstate + b * (K - 1) * a.width + e;
+        // dx of token p, whose terms are complete: those of the tokens, and of the state that the row leaves
+        auto emit = [&](int64_t p, Chan<T, V> v) {
+            if (p >= t1 || (p < t0 && t0 > 0)) return;
+            int64_t j = p - (end - (K - 1));
+            if (a.dlast != nullptr && j >= 0 && j < K - 1 && (tail >> (j + 1)) == 0) {
+                Chan<T, V> d;
+                d.set(load_some<T, V>((const raw *)a.dlast + (b * (K - 1) + j) * a.width + e, n));
+#pragma unroll
+                for (int i = 0; i < V; i++) v.v[i] += d.v[i];
+            }
+            if (n <= 0) return;
+            if (p >= 0) {
+                if (a.dx != nullptr) store_some<T, V>(dx + p * a.width, v.rounded(), n);
+            } else if (a.dstate != nullptr) store_some<T, V>(dstate + (p + K - 1) * a.width, v.rounded(), n);
+        };
+        int64_t t = t0;
+        if (t0 < end) {
+#pragma unroll
+            for (int j = 1; j < K; j++) {
+                x[j].set(input<T, V, K>(a, b, t0 - K + j, e, n));
+                if (begins >> (j - 1) & 1) {
+                    age = K - 1 - j;
+#pragma unroll
+                    for (int i = 0; i < j; i++) x[i].zero();
+                }
+            }
+            begins >>= K - 1;
+            const raw *dyp = (const raw *)a.dy + b * a.dy_batch + e;
+            while (t < stop) {
+                Vec<T, V> in[4], out[4];
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    int64_t p = t + q < stop ? t + q : stop - 1;
+                    in[q] = input<T, V, K>(a, b, p, e, n);
+                    out[q] = load_some<T, V>(dyp + p * a.dy_time, n);
+                }
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    if (t >= stop) break;
+#pragma unroll
+                    for (int j = 0; j + 1 < K; j++) x[j] = x[j + 1];
+                    age = age < K ? age + 1 : K;
+                    if (begins & 1) {
+                        age = 0;
+#pragma unroll
+                        for (int j = 0; j + 1 < K; j++) x[j].zero();
+                    }
+                    begins >>= 1;
+                    x[K - 1].set(in[q]);
+                    Chan<T, V> s = bias, d;
+                    d.set(out[q]);
+#pragma unroll
+                    for (int i = 0; i < V; i++) {
+#pragma unroll
+                        for (int j = 0; j < K; j++) s.v[i] += w[j].v[i] * x[j].v[i];
+                        float sig = sigmoid_(s.v[i]);
+                        d.v[i] *= sig * (1.0f + s.v[i] * (1.0f - sig));
+                    }
+#pragma unroll
+                    for (int j = 0; j < K; j++)
+                        if (K - 1 - j <= age)
+#pragma unroll
+                            for (int i = 0; i < V; i++) pend[j].v[i] += w[j].v[i] * d.v[i];
+                    if (t < own) {
+#pragma unroll
+                        for (int i = 0; i < V; i++) {
+                            db.v[i] += d.v[i];
+#pragma unroll
+                            for (int j = 0; j < K; j++) dw[j].v[i] += d.v[i] * x[j].v[i];
+                        }
+                    }
+                    emit(t - (K - 1), pend[0]);
+#pragma unroll
+                    for (int j = 0; j + 1 < K; j++) pend[j] = pend[j + 1];
+                    pend[K - 1].zero();
+                    t++;
+                }
+            }
+        }
+        // tokens t - (K - 1) .. t - 1 wait for no further term (t: the row's end, K - 1 past the tile, or its first token where the row ended before)
+        if (t0 < end || t0 == 0)
+#pragma unroll
+            for (int j = 0; j + 1 < K; j++)
+                if (t - (K - 1) + j < end) emit(t - (K - 1) + j, pend[j]);
+        Chan<T, V> none;
+        none.zero();
+        if (a.dx != nullptr && n > 0)
+            for (int64_t p = t0 > end ? t0 : end; p < t1; p++) store_some<T, V>(dx + p * a.width, none.rounded(), n);
+    }
+    if (a.part == nullptr) return;
+    __shared__ float meet[4][kWave];
+    float *part = a.part + (int64_t)blockIdx.x * (K + 1) * a.width;
+#pragma unroll
+    for (int j = 0; j <= K; j++)
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            __syncthreads();
+            meet[wave][lane] = j < K ? dw[j < K ? j : 0].v[i] : db.v[i];
+            __syncthreads();
+            if (wave == 0 && i < n) {
+                float s = 0;
+                for (int k = 0; k < waves; k++) s += meet[k][lane];
+                part[(int64_t)j * a.width + e + i] = s;
+            }
+        }
+}
+
+// one token: the window is the state and x; every value of the state is read and written once
+template <class T, int V, int K> __global__ __launch_bounds__(256) void conv_step(ConvArgs a, int64_t groups) {
+    using raw = typename T::raw;
+    int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (at >= a.batch * groups) return;
+    int64_t b = at / groups;
+    int e = (int)(at % groups) * V, n = a.width - e;
+    Chan<T, V> w[K], s;
+    taps<T, V, K>(a, e, w, s);
+    bool first = a.reset != nullptr && a.reset[b * a.reset_batch] != 0;
+    Vec<T, V> in[K];
+#pragma unroll
+    for (int j = 0; j < K; j++) {
+        in[j] = input<T, V, K>(a, b, j - (K - 1), e, n);
+        if (first && j + 1 < K)
+#pragma unroll
+            for (int i = 0; i < V; i++) in[j].v[i] = 0;
+    }
+#pragma unroll
+    for (int j = 0; j < K; j++)
+#pragma unroll
+        for (int i = 0; i < V; i++) s.v[i] += w[j].v[i] * up<T>(in[j].v[i]);
+#pragma unroll
+    for (int i = 0; i < V; i++) s.v[i] *= sigmoid_(s.v[i]);
+    store_some<T, V>((raw *)a.y + b * a.width + e, s.rounded(), n);
+#pragma unroll
+    for (int j = 0; j + 1 < K; j++) store_some<T, V>((raw *)a.last + (b * (K - 1) + j) * a.width + e, in[j + 1], n);
+}
+
+struct ConvOut {
+    void *dweight, *dbias;
+    int width, taps, type;
+    bool wide;
+    __device__ void operator()(int64_t col, float v) const {
+        int j = (int)(col / width), e = (int)(col % width);
+        void *to = j < taps ? dweight : dbias;
+        int64_t at = j < taps ? (int64_t)e * taps + j : e;
+        if (to == nullptr) return;
+        if (wide || type == MWS_F32) ((float *)to)[at] = v;
+        else if (type == MWS_BF16) ((uint16_t *)to)[at] = down<BF16>(v);
+        else ((uint16_t *)to)[at] = down<F16>(v);
+    }
+};
+
+// A tile of 32 tokens re-reads K - 1 of its neighbour's; where that leaves less than four waves to a SIMD, tiles get shorter.
+static int conv_v(const mws_conv_args *a) { return a->type == MWS_F32 ? 4 : 8; }
+static int conv_tile(const mws_conv_args *a) {
+    int64_t across = a->batch * ceil_div(a->width, kWave * conv_v(a));
+    int tile = kMostTile;
+    while (tile > 8 && across * ceil_div(a->length, tile) < 4 * kSimds) tile /= 2;
+    return tile;
+}
+static int64_t conv_tiles(const mws_conv_args *a) { return a->length > 0 ? ceil_div(a->length, conv_tile(a)) : 1; }
+// backward: each block's partial sums are K + 1 values a channel; two blocks to a compute unit, over the channels' groups
+static int64_t conv_blocks(const mws_conv_args *a) {
+    int64_t need = ceil_div(a->batch * conv_tiles(a), 4), groups = ceil_div(a->width, kWave * conv_v(a));
+    int64_t most = groups < 16 ? 1024 / groups : 64;
+    return need < most ? need : most;
+}
+
+static int32_t conv_check(const mws_conv_args *a, const char *what, bool backward, bool step) {
+    if (a == nullptr) return fail("%s: no arguments", what);
+    if (a->type < MWS_F32 || a->type > MWS_F16) return fail("%s: type %d is none of MWS_F32, MWS_BF16, MWS_F16", what, a->type);
+    if (a->param_type != MWS_F32 && a->param_type != a->type) return fail("%s: parameters are float or of the activations' type", what);
+    if (a->taps < MWS_CONV_MIN_TAPS || a->taps > MWS_CONV_MAX_TAPS) return fail("%s: %d taps are not within %d .. %d", what, a->taps, MWS_CONV_MIN_TAPS, MWS_CONV_MAX_TAPS);
+    if (a->width < 1 || a->width > (1 << 24)) return fail("%s: width %d", what, a->width);
+    if (a->batch < 0 || a->length < 0 || a->batch > (1 << 30) || a->length > (1 << 30) || a->batch * (a->length + 1) > ((int64_t)1 << 33)) return fail("%s: %lld rows of %lld tokens", what, (long long)a->batch, (long long)a->length);
+    if (a->weight == nullptr) return fail("%s: weight is NULL", what);
+    if (step && a->length != 1) return fail("%s: one token at a time", what);
+    if (a->batch == 0) return 0;
+    if (a->length > 0 && a->x == nullptr) return fail("%s: x is NULL", what);
+    if (!backward && a->length > 0 && a->y == nullptr) return fail("%s: y is NULL", what);
+    if (backward && a->length > 0 && a->dy == nullptr) return fail("%s: dy is NULL", what);
+    if (step && (a->state == nullptr || a->last == nullptr)) return fail("%s: the state is NULL", what);
+    return 0;
+}
+
+static ConvArgs conv_device(const mws_conv_args *a) {
+    ConvArgs d = {};
+    d.x = a->x, d.weight = a->weight, d.bias = a->bias, d.state = a->state, d.dy = a->dy, d.dlast = a->dlast;
+    d.reset = a->reset, d.lengths = a->lengths, d.y = a->y, d.last = a->last, d.dx = a->dx, d.dstate = a->dstate;
+    d.batch = a->batch, d.length = a->length, d.tile = conv_tile(a);
+    d.tiles = conv_tiles(a);
+    d.x_batch = a->x_batch, d.x_time = a->x_time, d.dy_batch = a->dy_batch, d.dy_time = a->dy_time;
+    d.reset_batch = a->reset_batch, d.reset_time = a->reset_time;
+    d.width = a->width, d.wide = a->param_type == MWS_F32;
+    return d;
+}
+
+enum { kForward, kBackward, kStep };
+template <class T, int V, int K> static void conv_go(const mws_conv_args *a, const ConvArgs &d, int what, hipStream_t stream) {
+    unsigned groups = (unsigned)ceil_div(a->width, kWave * V);
+    if (what == kForward) hipLaunchKernelGGL((conv_forward<T, V, K>), dim3((unsigned)ceil_div(d.batch * d.tiles, 4), groups), dim3(256), 0, stream, d);
+    else if (what == kBackward) hipLaunchKernelGGL((conv_backward<T, V, K>), dim3((unsigned)conv_blocks(a), groups), dim3(256), 0, stream, d);
+    else {
+        int64_t each = ceil_div(a->width, V);
+        hipLaunchKernelGGL((conv_step<T, V, K>), dim3((unsigned)ceil_div(d.batch * each, 256)), dim3(256), 0, stream, d, each);
+    }
+}
+template <class T, int V> static void conv_taps(const mws_conv_args *a, const ConvArgs &d, int what, hipStream_t stream) {
+    if (a->taps == 2) conv_go<T, V, 2>(a, d, what, stream);
+    else if (a->taps == 3) conv_go<T, V, 3>(a, d, what, stream);
+    else conv_go<T, V, 4>(a, d, what, stream);
+}
+static void conv_run(const mws_conv_args *a, const ConvArgs &d, int what, hipStream_t stream) {
+    if (a->type == MWS_F32) conv_taps<F32, 4>(a, d, what, stream);
+    else if (a->type == MWS_BF16) conv_taps<BF16, 8>(a, d, what, stream);
+    else conv_taps<F16, 8>(a, d, what, stream);
+}
+}  // namespace mws
+
+using namespace mws;
+
+extern "C" int32_t mws_conv_forward(const mws_conv_args *a, void *stream) {
+    if (int32_t e = conv_check(a, "mws_conv_forward", false, false)) return e;
+    if (a->batch == 0) return 0;
+    conv_run(a, conv_device(a), kForward, (hipStream_t)stream);
+    return launched("mws_conv_forward");
+}
+
+extern "C" int64_t mws_conv_workspace(const mws_conv_args *a) {
+    if (int32_t e = conv_check(a, "mws_conv_workspace", true, false)) return e;
+    return a->dweight != nullptr || a->dbias != nullptr ? conv_blocks(a) * (a->taps + 1) * a->width * (int64_t)sizeof(float) : 0;
+}
+
+extern "C" int32_t mws_conv_backward(const mws_conv_args *a, void *stream) {
+    if (int32_t e = conv_check(a, "mws_conv_backward", true, false)) return e;
+    int64_t need = mws_conv_workspace(a);
+    if (a->workspace_bytes < need || (need > 0 && a->workspace == nullptr)) return fail("mws_conv_backward: the workspace needs %lld bytes", (long long)need);
+    ConvArgs d = conv_device(a);
+    bool params = a->dweight != nullptr || a->dbias != nullptr;
+    d.part = params ? (float *)a->workspace : nullptr;
+    int64_t blocks = conv_blocks(a);
+    if (blocks > 0) conv_run(a, d, kBackward, (hipStream_t)stream);
+    if (params) {
+        ConvOut out = {a->dweight, a->dbias, a->width, a->taps, a->type, a->param_type == MWS_F32};
+        launch_sum_parts((const float *)a->workspace, (int)blocks, (int64_t)(a->taps + 1) * a->width, out, (hipStream_t)stream);
+    }
+    return launched("mws_conv_backward");
+}
+
+extern "C" int32_t mws_conv_step(const mws_conv_args *a, void *stream) {
+    if (int32_t e = conv_check(a, "mws_conv_step", false, true)) return e;
+    if (a->batch == 0) return 0;
+    conv_run(a, conv_device(a), kStep, (hipStream_t)stream);
+    return launched("mws_conv_step");
+}

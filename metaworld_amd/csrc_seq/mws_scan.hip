@@ -1,0 +1,729 @@
+// mws_scan.hip -- the selective state space scan: forward, backward, one token.
+//
+//   d_t = softplus(dt_t + dt_bias), a_t = exp(d_t A), h_t = a_t h_{t-1} + d_t u_t B_t, o_t = C_t . h_t + D u_t, y_t = o_t silu(z_t)
+//   do = dy silu(z), g_t = do_t C_t + a_{t+1} g_{t+1}
+//   dC_t = sum over channels of do h_t, dB_t = sum over channels of g d u, du = D do + d (g . B), dz = dy o silu'(z)
+//   dd_t = u (g . B) + g . (A a_t h_{t-1}), ddt = dd sigmoid(dt + dt_bias), dA = sum over tokens of g d a_t h_{t-1}
+//
+// where an episode begins, a_t counts as zero.
+//
+// A lane is a channel with all its states in registers, so that a token's B and C are the same for the whole wave: they come in
+// scalar registers, from a small copy in float, [token][B | C][states], that `spread` makes first (128 bytes a token next to the
+// channels' 8 bytes each).  A wave walks along the time axis; u, dt, z and y are read and written in order of channels.
+// Bound by the vector unit: per value and state one exp and four multiplications or additions forward.
+//
+// Where batch x channels leave the card empty, the time axis is cut into segments of whole chunks: scan_segment takes each
+// segment's end state from zero and its sum of d (the product of its a is exp(A sum d)), scan_join runs over the segments, and the
+// scan itself starts every segment from its joined state.  The same holds for g, from the end.
+#include "mws_common.hpp"
+
+namespace mws {
+
+// Tokens between two states kept for the backward pass; segments are whole chunks.  And a block's channels at most: the backward
+// pass keeps the states inside a chunk in shared memory, 64 KB for a block at most.
+constexpr int chunk_of(int ns) { return ns >= 32 ? 16 : 32; }
+constexpr int sub_of(int ns) { return ns >= 32 ? 4 : 8; }
+constexpr int lanes_of(int ns) { return ns >= 32 ? 128 : 256; }
+
+struct ScanArgs {
+    const void *u, *dt, *z, *dy;
+    const float *A, *D, *dt_bias, *state, *dlast;
+    const uint8_t *reset;
+    const int32_t *lengths;
+    void *y, *du, *ddt, *dz;
+    float *last, *kept, *dstate;
+    const float *bc;             // [batch][length][2][NS]
+    float *seg, *sum;            // [batch][segments][NS][width] states, [batch][segments][width] sums of d (negative: cut by an episode's beginning)
+    float *part_bc;              // [blocks over channels][batch][length][2 NS]
+    float *part;                 // [groups][NS + 2][width]: dA, dD, ddt_bias
+    int64_t batch, length, chunks;
+    int64_t u_batch, u_time, dt_batch, dt_time, z_batch, z_time, dy_batch, dy_time, reset_batch, reset_time;
+    int width, states, across, segments, span, groups;            // across: blocks over the channels; span: tokens of a segment
+};
+
+__device__ __forceinline__ int64_t row_length(const int32_t *lengths, int64_t b, int64_t length) {
+    if (lengths == nullptr) return length;
+    int64_t n = lengths[b];
+    return n < 0 ? 0 : n > length ? length : n;
+}
+
+// log(1 + e^x): with w = 1 + e rounded, log(w) e / (w - 1) undoes the rounding of w; beyond 20 it is x to 32 bits
+__device__ __forceinline__ float softplus_(float x) {
+    float e = exp_(x), w = 1.0f + e, d = w - 1.0f;
+    float l = __builtin_amdgcn_logf(w) * kLn2;
+    float r = d == 0.0f ? e : l * (e * rcp_(d));
+    return x > 20.0f ? x : r;
+}
+
+// bit i: an episode begins at token t0 + i of the chunk
+template <int CHUNK> __device__ __forceinline__ uint32_t chunk_mask(const ScanArgs &a, int64_t b, int64_t t0, int64_t end) {
+    if (a.reset == nullptr) return 0;
+    int lane = threadIdx.x % kWave;
+    int64_t t = t0 + lane;
+    return (uint32_t)__ballot(lane < CHUNK && t < end && a.reset[b * a.reset_batch + t * a.reset_time] != 0);
+}
+
+// ---- B and C in float, padded with zeros to NS states ----
+template <class T> __global__ __launch_bounds__(256) void spread(const void *B, const void *C, float *bc, int64_t length, int64_t B_batch, int64_t B_time, int64_t C_batch,
+                                                                  int64_t C_time, int states, int ns, int64_t count) {
+    int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (at >= count) return;
+    int n = (int)(at % ns);
+    int64_t rest = at / ns, token = rest >> 1, b = token / length, t = token % length;
+    const typename T::raw *from = (const typename T::raw *)(rest & 1 ? C : B) + (rest & 1 ? b * C_batch + t * C_time : b * B_batch + t * B_time);
+    bc[at] = n < states ? up<T>(from[n]) : 0.0f;
+}
+
+// one token's B and C: the address is the same for the wave and nothing of this kernel writes there, which the constant address
+// space says, so that they are scalar loads
+using Fixed = const __attribute__((address_space(4))) float;
+__device__ __forceinline__ Fixed *fixed(const float *p) { return (Fixed *)(uintptr_t)p; }
+template <int NS> struct Pair {
+    float B[NS], C[NS];
+    __device__ __forceinline__ void read(Fixed *p) {
+#pragma unroll
+        for (int n = 0; n < NS; n++) B[n] = p[n], C[n] = p[NS + n];
+    }
+};
+
+template <int NS> __device__ __forceinline__ void rates(const ScanArgs &a, uint32_t e, float (&A2)[NS]) {       // A / ln 2, for exp2
+#pragma unroll
+    for (int n = 0; n < NS; n++) A2[n] = n < a.states ? a.A[(int64_t)e * a.states + n] * kLog2e : 0.0f;
+}
+template <int NS> __device__ __forceinline__ void first_state(const float *state, const ScanArgs &a, int64_t b, uint32_t e, float (&h)[NS]) {
+#pragma unroll
+    for (int n = 0; n < NS; n++) h[n] = state != nullptr && n < a.states ? state[(b * a.width + e) * a.states + n] : 0.0f;
+}
+template <int NS> __device__ __forceinline__ void last_state(float *to, const ScanArgs &a, int64_t b, uint32_t e, const float (&h)[NS]) {
+#pragma unroll
+    for (int n = 0; n < NS; n++)
+        if (n < a.states) to[(b * a.width + e) * a.states + n] = h[n];
+}
+template <int NS> __device__ __forceinline__ void get_row(const float *p, int64_t row, const ScanArgs &a, uint32_t e, float (&h)[NS]) {
+#pragma unroll
+    for (int n = 0; n < NS; n++) h[n] = (p + (row * NS + n) * a.width)[e];
+}
+template <int NS> __device__ __forceinline__ void put_row(float *p, int64_t row, const ScanArgs &a, uint32_t e, const float (&h)[NS]) {
+#pragma unroll
+    for (int n = 0; n < NS; n++) (p + (row * NS + n) * a.width)[e] = h[n];
+}
+
+struct Place {          // what a block of the grid works on
+    int64_t b, t0, t1, end;
+    uint32_t e;
+    int at, seg;
+    bool on;
+    __device__ __forceinline__ Place(const ScanArgs &a, int64_t item, int part) {
+        at = part * (int)blockDim.x + (int)threadIdx.x;
+        on = at < a.width;
+        e = on ? at : a.width - 1;
+        b = item / a.segments, seg = (int)(item % a.segments);
+        end = row_length(a.lengths, b, a.length);
+        t0 = (int64_t)seg * a.span, t1 = t0 + a.span < a.length ? t0 + a.span : a.length;
+    }
+};
+
+template <class T, int NS> __global__ __launch_bounds__(256) void scan_forward(ScanArgs a) {
+    using raw = typename T::raw;
+    constexpr int G = 4, kChunk = chunk_of(NS);
+    Place p(a, blockIdx.x / a.across, blockIdx.x % a.across);
+    int64_t stop = p.t1 < p.end ? p.t1 : p.end;
+    raw *y = (raw *)a.y + p.b * a.length * a.width;
+    bool whole_end = p.end <= p.t1 && (p.end > p.t0 || p.seg == 0);      // the row ends in this segment
+    if (p.t0 < stop || whole_end) {
+        float h[NS], A2[NS];
+        rates<NS>(a, p.e, A2);
+        if (p.seg == 0) first_state<NS>(a.state, a, p.b, p.e, h);
+        else get_row<NS>(a.seg, p.b * a.segments + p.seg, a, p.e, h);
+        float D = a.D != nullptr ? a.D[p.e] : 0.0f, bias = a.dt_bias != nullptr ? a.dt_bias[p.e] : 0.0f;
+        const raw *u = (const raw *)a.u + p.b * a.u_batch, *dt = (const raw *)a.dt + p.b * a.dt_batch;
+        const raw *z = a.z != nullptr ? (const raw *)a.z + p.b * a.z_batch : nullptr;
+        Fixed *bc = fixed(a.bc + p.b * a.length * 2 * NS);
+        for (int64_t c0 = p.t0; c0 < stop; c0 += kChunk) {
+            uint32_t begins = chunk_mask<kChunk>(a, p.b, c0, p.end);
+            if (a.kept != nullptr && p.on) put_row<NS>(a.kept, p.b * a.chunks + c0 / kChunk, a, p.e, h);
+            int64_t c1 = c0 + kChunk < stop ? c0 + kChunk : stop;
+            for (int64_t t = c0; t < c1; t += G) {
+                raw ru[G], rd[G], rz[G];
+#pragma unroll
+                for (int q = 0; q < G; q++) {
+                    int64_t at = t + q < c1 ? t + q : c1 - 1;
+                    ru[q] = (u + at * a.u_time)[p.e], rd[q] = (dt + at * a.dt_time)[p.e];
+                    if (z != nullptr) rz[q] = (z + at * a.z_time)[p.e];
+                }
+#pragma unroll
+                for (int q = 0; q < G; q++) {
+                    if (t + q >= c1) break;
+                    Pair<NS> m;
+                    m.read(bc + (t + q) * 2 * NS);
+                    float uf = up<T>(ru[q]), d = softplus_(up<T>(rd[q]) + bias), du = d * uf, o = D * uf, o2 = 0;
+                    if (begins >> q & 1)
+#pragma unroll
+                        for (int n = 0; n < NS; n++) h[n] = 0;
+#pragma unroll
+                    for (int n = 0; n < NS; n++) {
+                        h[n] = __builtin_fmaf(exp2_(d * A2[n]), h[n], du * m.B[n]);
+                        if (n & 1) o2 = __builtin_fmaf(m.C[n], h[n], o2);
+                        else o = __builtin_fmaf(m.C[n], h[n], o);
+                    }
+                    o += o2;
+                    if (z != nullptr) {
+                        float zf = up<T>(rz[q]);
+                        o *= zf * sigmoid_(zf);
+                    }
+                    if (p.on) (y + (t + q) * a.width)[p.e] = down<T>(o);
+                }
+                begins >>= G;
+            }
+        }
+        if (a.last != nullptr && whole_end && p.on) last_state<NS>(a.last, a, p.b, p.e, h);
+    }
+    if (p.on)
+        for (int64_t t = p.t0 > p.end ? p.t0 : p.end; t < p.t1; t++) (y + t * a.width)[p.e] = down<T>(0.0f);
+}
+
+// a segment's end state from zero, and its sum of d
+template <class T, int NS> __global__ __launch_bounds__(256) void scan_segment(ScanArgs a) {
+    using raw = typename T::raw;
+    constexpr int G = 4, kChunk = chunk_of(NS);
+    Place p(a, blockIdx.x / a.across, blockIdx.x % a.across);
+    int64_t stop = p.t1 < p.end ? p.t1 : p.end;
+    float h[NS], A2[NS], sum = 0;
+    rates<NS>(a, p.e, A2);
+#pragma unroll
+    for (int n = 0; n < NS; n++) h[n] = 0;
+    bool cut = false;
+    float bias = a.dt_bias != nullptr ? a.dt_bias[p.e] : 0.0f;
+    const raw *u = (const raw *)a.u + p.b * a.u_batch, *dt = (const raw *)a.dt + p.b * a.dt_batch;
+    Fixed *bc = fixed(a.bc + p.b * a.length * 2 * NS);
+    for (int64_t c0 = p.t0; c0 < stop; c0 += kChunk) {
+        uint32_t begins = chunk_mask<kChunk>(a, p.b, c0, p.end);
+        cut = cut || begins != 0;
+        int64_t c1 = c0 + kChunk < stop ? c0 + kChunk : stop;
+        for (int64_t t = c0; t < c1; t += G) {
+            raw ru[G], rd[G];
+#pragma unroll
+            for (int q = 0; q < G; q++) {
+                int64_t at = t + q < c1 ? t + q : c1 - 1;
+                ru[q] = (u + at * a.u_time)[p.e], rd[q] = (dt + at * a.dt_time)[p.e];
+            }
+#pragma unroll
+            for (int q = 0; q < G; q++) {
+                if (t + q >= c1) break;
+                Pair<NS> m;
+                m.read(bc + (t + q) * 2 * NS);
+                float d = softplus_(up<T>(rd[q]) + bias), du = d * up<T>(ru[q]);
+                sum += d;
+                if (begins >> q & 1)
+#pragma unroll
+                    for (int n = 0; n < NS; n++) h[n] = 0;
+#pragma unroll
+                for (int n = 0; n < NS; n++) h[n] = __builtin_fmaf(exp2_(d * A2[n]), h[n], du * m.B[n]);
+            }
+            begins >>= G;
+        }
+    }
+    if (p.on) {
+        int64_t row = p.b * a.segments + p.seg;
+        put_row<NS>(a.seg, row, a, p.e, h);
+        a.sum[row * a.width + p.e] = cut ? -1.0f : sum;
+    }
+}
+
+// what g leaves before a segment's first token, from zero after its last
+template <class T, int NS> __global__ __launch_bounds__(256) void scan_segment_back(ScanArgs a) {
+    using raw = typename T::raw;
+    constexpr int kChunk = chunk_of(NS);
+    Place p(a, blockIdx.x / a.across, blockIdx.x % a.across);
+    int64_t stop = p.t1 < p.end ? p.t1 : p.end;
+    float g[NS], A2[NS], sum = 0;
+    rates<NS>(a, p.e, A2);
+#pragma unroll
+    for (int n = 0; n < NS; n++) g[n] = 0;
+    bool cut = false;
+    float bias = a.dt_bias != nullptr ? a.dt_bias[p.e] : 0.0f;
+    const raw *dt = (const raw *)a.dt + p.b * a.dt_batch, *dy = (const raw *)a.dy + p.b * a.dy_batch;
+    const raw *z = a.z != nullptr ? (const raw *)a.z + p.b * a.z_batch : nullptr;
+    Fixed *bc = fixed(a.bc + p.b * a.length * 2 * NS);
+    if (p.t0 < stop)
+        for (int64_t c0 = p.t0 + (stop - 1 - p.t0) / kChunk * kChunk; c0 >= p.t0; c0 -= kChunk) {
+            uint32_t begins = chunk_mask<kChunk>(a, p.b, c0, p.end);
+            cut = cut || begins != 0;
+            int64_t c1 = c0 + kChunk < stop ? c0 + kChunk : stop;
+            for (int64_t t = c1 - 1; t >= c0; t--) {
+                Pair<NS> m;
+                m.read(bc + t * 2 * NS);
+                float d = softplus_(up<T>((dt + t * a.dt_time)[p.e]) + bias), o = up<T>((dy + t * a.dy_time)[p.e]);
+                if (z != nullptr) {
+                    float zf = up<T>((z + t * a.z_time)[p.e]);
+                    o *= zf * sigmoid_(zf);
+                }
+                sum += d;
+#pragma unroll
+                for (int n = 0; n < NS; n++) g[n] = exp2_(d * A2[n]) * __builtin_fmaf(o, m.C[n], g[n]);
+                if (begins >> (int)(t - c0) & 1)
+#pragma unroll
+                    for (int n = 0; n < NS; n++) g[n] = 0;
+            }
+        }
+    if (p.on) {
+        int64_t row = p.b * a.segments + p.seg;
+        put_row<NS>(a.seg, row, a, p.e, g);
+        a.sum[row * a.width + p.e] = cut ? -1.0f : sum;
+    }
+}
+
+// every segment's incoming state, in the place of what it left from zero: forward the state before its first token, backward g
+// after its last (from the segment that the row ends in; those behind it are not read)
+__global__ __launch_bounds__(256) void scan_join(ScanArgs a, int ns, bool backward) {
+    int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (at >= a.batch * ns * a.width) return;
+    int e = (int)(at % a.width), n = (int)(at / a.width % ns);
+    int64_t b = at / a.width / ns, end = row_length(a.lengths, b, a.length);
+    int last = (int)(end > 0 ? (end - 1) / a.span : 0);
+    bool real = n < a.states;
+    float A2 = real ? a.A[(int64_t)e * a.states + n] * kLog2e : 0.0f;
+    const float *from = backward ? a.dlast : a.state;
+    float h = from != nullptr && real ? from[(b * a.width + e) * a.states + n] : 0.0f;
+    for (int k = 0; k <= last; k++) {
+        int s = backward ? last - k : k;
+        int64_t row = b * a.segments + s;
+        float *mine = a.seg + (row * ns + n) * a.width + e;
+        float left = *mine, sum = a.sum[row * a.width + e];
+        *mine = h;
+        h = sum < 0.0f || h == 0.0f ? left : __builtin_fmaf(exp2_(sum * A2), h, left);
+    }
+    if (backward && a.dstate != nullptr && real) a.dstate[(b * a.width + e) * a.states + n] = h;
+}
+
+// ---- sums of M values over the 64 lanes of a wave: every step adds one half of the lanes to the other and halves the values that
+// a lane carries, so that M values take about 2 M instructions.  Lane l gets the sum of value l / (64 / M). ----
+__device__ __forceinline__ void swap32(float &x, float &y) {
+    auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y), false, false);
+    unsigned r0 = r[0], r1 = r[1];       // (a bit cast of an element itself takes the vector's first)
+    x = __builtin_bit_cast(float, r0), y = __builtin_bit_cast(float, r1);
+}
+__device__ __forceinline__ void swap16(float &x, float &y) {
+    auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y), false, false);
+    unsigned r0 = r[0], r1 = r[1];       // (a bit cast of an element itself takes the vector's first)
+    x = __builtin_bit_cast(float, r0), y = __builtin_bit_cast(float, r1);
+}
+template <int CTRL> __device__ __forceinline__ float dpp(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+constexpr int kRor8 = 0x128, kHalfMirror = 0x141, kQuad2 = 0x4E, kQuad1 = 0xB1;    // the lane 8 on in its row; 7 - lane in its half row; lane ^ 2; lane ^ 1
+template <int CTRL, int COUNT> __device__ __forceinline__ void fold(float *v, bool high) {      // COUNT values to COUNT / 2, or one value over both halves
+    if constexpr (COUNT == 1) v[0] += dpp<CTRL>(v[0]);
+    else {
+#pragma unroll
+        for (int k = 0; k < COUNT / 2; k++) {
+            float keep = high ? v[k + COUNT / 2] : v[k], give = high ? v[k] : v[k + COUNT / 2];
+            v[k] = keep + dpp<CTRL>(give);
+        }
+    }
+}
+__device__ __forceinline__ float first_sum(float x, float y) {      // the first step: value k and value k + M / 2
+    swap32(x, y);
+    return x + y;
+}
+template <int M> __device__ __forceinline__ float wave_sums(float (&v)[M / 2]) {
+    static_assert(M >= 8 && M <= 64 && (M & (M - 1)) == 0, "a power of two");
+    int lane = threadIdx.x % kWave;
+#pragma unroll
+    for (int k = 0; k < M / 4; k++) {
+        swap16(v[k], v[k + M / 4]);
+        v[k] += v[k + M / 4];
+    }
+    fold<kRor8, M / 4>(v, lane & 8);
+    fold<kHalfMirror, (M / 8 > 1 ? M / 8 : 1)>(v, lane & 4);
+    fold<kQuad2, (M / 16 > 1 ? M / 16 : 1)>(v, lane & 2);
+    fold<kQuad1, (M / 32 > 1 ? M / 32 : 1)>(v, lane & 1);
+    return v[0];
+}
+
+// The backward pass walks over a segment's chunks from the last.  In a chunk it goes forward once from the kept state and leaves the
+// state before every SUB-th token in shared memory; then, from the last SUB tokens, forward again with what each token keeps of the
+// state before it, a_t h_{t-1}, in registers (SUB x NS = 128 of them), and backward over them.  dB and dC are summed over the wave's
+// channels token by token (wave_sums), over the block's waves once a chunk, over blocks by scan_bc_out.
+template <class T, int NS> __global__ __launch_bounds__(256, 2) void scan_backward(ScanArgs a) {
+    using raw = typename T::raw;
+    constexpr int kChunk = chunk_of(NS), SUB = sub_of(NS), kSubs = kChunk / SUB, M = 2 * NS;
+    extern __shared__ float pool[];
+    int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), waves = blockDim.x / kWave;
+    float *states = pool + (size_t)wave * (kSubs - 1) * NS * kWave + lane;       // [subs - 1][NS][64] of this wave
+    float *sums = pool + (size_t)waves * (kSubs - 1) * NS * kWave;               // [waves][chunk][M]
+    int part = blockIdx.x % a.across, group = blockIdx.x / a.across;
+    float dA[NS], dD = 0, dbias = 0, A2[NS];
+    {
+        int at = part * (int)blockDim.x + (int)threadIdx.x;
+        rates<NS>(a, at < a.width ? at : a.width - 1, A2);
+    }
+#pragma unroll
+    for (int n = 0; n < NS; n++) dA[n] = 0;
+    for (int64_t item = group; item < a.batch * a.segments; item += a.groups) {
+        Place p(a, item, part);
+        int64_t stop = p.t1 < p.end ? p.t1 : p.end;
+        bool whole_end = p.end <= p.t1 && (p.end > p.t0 || p.seg == 0);
+        raw *du = (raw *)a.du + p.b * a.length * a.width, *ddt = (raw *)a.ddt + p.b * a.length * a.width;
+        raw *dz = a.z != nullptr ? (raw *)a.dz + p.b * a.length * a.width : nullptr;
+        float g[NS];
+        if (p.t0 < stop || whole_end) {
+            if (a.segments > 1) get_row<NS>(a.seg, p.b * a.segments + p.seg, a, p.e, g);
+            else first_state<NS>(a.dlast, a, p.b, p.e, g);
+            if (!p.on)
+#pragma unroll
+                for (int n = 0; n < NS; n++) g[n] = 0;
+            float D = a.D != nullptr ? a.D[p.e] : 0.0f, bias = a.dt_bias != nullptr ? a.dt_bias[p.e] : 0.0f;
+            const raw *u = (const raw *)a.u + p.b * a.u_batch, *dt = (const raw *)a.dt + p.b * a.dt_batch, *dy = (const raw *)a.dy + p.b * a.dy_batch;
+            const raw *z = a.z != nullptr ? (const raw *)a.z + p.b * a.z_batch : nullptr;
+            Fixed *bc = fixed(a.bc + p.b * a.length * 2 * NS);
+            if (p.t0 < stop)
+                for (int64_t c0 = p.t0 + (stop - 1 - p.t0) / kChunk * kChunk; c0 >= p.t0; c0 -= kChunk) {
+                    uint32_t begins = chunk_mask<kChunk>(a, p.b, c0, p.end);
+                    int count = (int)(c0 + kChunk < stop ? kChunk : stop - c0), subs = (count + SUB - 1) / SUB;
+                    float h[NS];
+                    get_row<NS>(a.kept, p.b * a.chunks + c0 / kChunk, a, p.e, h);
+                    for (int s = 0; s + 1 < subs; s++) {
+#pragma unroll
+                        for (int q = 0; q < SUB; q++) {
+                            int64_t t = c0 + s * SUB + q;
+                            float d = softplus_(up<T>((dt + t * a.dt_time)[p.e]) + bias), x = d * up<T>((u + t * a.u_time)[p.e]);
+                            if (begins >> (s * SUB + q) & 1)
+#pragma unroll
+                                for (int n = 0; n < NS; n++) h[n] = 0;
+                            Fixed *m = bc + t * 2 * NS;
+#pragma unroll
+                            for (int n = 0; n < NS; n++) h[n] = __builtin_fmaf(exp2_(d * A2[n]), h[n], x * m[n]);
+                        }
+#pragma unroll
+                        for (int n = 0; n < NS; n++) states[(s * NS + n) * kWave] = h[n];
+                    }
+                    for (int s = subs - 1; s >= 0; s--) {
+                        if (s > 0)
+#pragma unroll
+                            for (int n = 0; n < NS; n++) h[n] = states[((s - 1) * NS + n) * kWave];
+                        else get_row<NS>(a.kept, p.b * a.chunks + c0 / kChunk, a, p.e, h);
+                        float keep[SUB][NS], d[SUB], uf[SUB], raws[SUB];
+                        int here = count - s * SUB < SUB ? count - s * SUB : SUB;
+#pragma unroll
+                        for (int q = 0; q < SUB; q++) {
+                            if (q < here) {
+                                int64_t t = c0 + s * SUB + q;
+                                raws[q] = up<T>((dt + t * a.dt_time)[p.e]) + bias;
+                                uf[q] = up<T>((u + t * a.u_time)[p.e]);
+                                d[q] = softplus_(raws[q]);
+                                float x = d[q] * uf[q];
+                                bool first = begins >> (s * SUB + q) & 1;
+                                Fixed *m = bc + t * 2 * NS;
+#pragma unroll
+                                for (int n = 0; n < NS; n++) {
+                                    keep[q][n] = first ? 0.0f : exp2_(d[q] * A2[n]) * h[n];
+                                    h[n] = __builtin_fmaf(x, m[n], keep[q][n]);
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int q = SUB - 1; q >= 0; q--) {
+                            if (q < here) {
+                                int64_t t = c0 + s * SUB + q;
+                                Pair<NS> m;
+                                m.read(bc + t * 2 * NS);
+                                float out = p.on ? up<T>((dy + t * a.dy_time)[p.e]) : 0.0f, zf = 0, gate = 1, sig = 0;
+                                if (z != nullptr) {
+                                    zf = up<T>((z + t * a.z_time)[p.e]);
+                                    sig = sigmoid_(zf);
+                                    gate = zf * sig;
+                                }
+                                float o = out * gate, x = d[q] * uf[q], gB = 0, gk = 0, y = D * uf[q], v[NS];
+#pragma unroll
+                                for (int n = 0; n < NS; n++) {
+                                    float hn = __builtin_fmaf(x, m.B[n], keep[q][n]);
+                                    y = __builtin_fmaf(m.C[n], hn, y);
+                                    g[n] = __builtin_fmaf(o, m.C[n], g[n]);
+                                    v[n] = first_sum(g[n] * x, o * hn);
+                                    gB = __builtin_fmaf(g[n], m.B[n], gB);
+                                    float k = g[n] * keep[q][n];
+                                    gk = __builtin_fmaf(k, A2[n], gk);
+                                    dA[n] = __builtin_fmaf(k, d[q], dA[n]);
+                                    g[n] *= exp2_(d[q] * A2[n]);
+                                }
+                                if (begins >> (s * SUB + q) & 1)
+#pragma unroll
+                                    for (int n = 0; n < NS; n++) g[n] = 0;
+                                float dd = __builtin_fmaf(uf[q], gB, gk * kLn2), draw = dd * sigmoid_(raws[q]);
+                                dD = __builtin_fmaf(o, uf[q], dD);
+                                dbias += draw;
+                                if (p.on) {
+                                    (du + t * a.width)[p.e] = down<T>(__builtin_fmaf(D, o, d[q] * gB));
+                                    (ddt + t * a.width)[p.e] = down<T>(draw);
+                                    if (z != nullptr) (dz + t * a.width)[p.e] = down<T>(out * y * sig * (1.0f + zf * (1.0f - sig)));
+                                }
+                                float total = wave_sums<M>(v);
+                                if (lane % (kWave / M) == 0) sums[(wave * kChunk + s * SUB + q) * M + lane / (kWave / M)] = total;
+                            }
+                        }
+                    }
+                    __syncthreads();
+                    for (int k = threadIdx.x; k < count * M; k += blockDim.x) {
+                        float v = 0;
+                        for (int w = 0; w < waves; w++) v += sums[w * kChunk * M + k];
+                        a.part_bc[((int64_t)part * a.batch * a.length + p.b * a.length + c0) * M + k] = v;
+                    }
+                    __syncthreads();
+                }
+            if (p.on && p.seg == 0 && a.segments == 1 && a.dstate != nullptr) last_state<NS>(a.dstate, a, p.b, p.e, g);
+        }
+        if (p.on)
+            for (int64_t t = p.t0 > p.end ? p.t0 : p.end; t < p.t1; t++) {
+                (du + t * a.width)[p.e] = (ddt + t * a.width)[p.e] = down<T>(0.0f);
+                if (dz != nullptr) (dz + t * a.width)[p.e] = down<T>(0.0f);
+            }
+    }
+    int at = part * (int)blockDim.x + (int)threadIdx.x;
+    if (at < a.width) {
+        float *to = a.part + (int64_t)group * (NS + 2) * a.width + at;
+#pragma unroll
+        for (int n = 0; n < NS; n++) to[(int64_t)n * a.width] = dA[n];
+        to[(int64_t)NS * a.width] = dD;
+        to[(int64_t)(NS + 1) * a.width] = dbias;
+    }
+}
+
+template <class T> __global__ __launch_bounds__(256) void scan_bc_out(const float *part, const int32_t *lengths, void *dB, void *dC, int64_t batch, int64_t length, int parts, int states,
+                                                                       int ns) {
+    int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, all = batch * length * 2 * ns;
+    if (at >= all) return;
+    int n = (int)(at % ns);
+    if (n >= states) return;
+    int64_t rest = at / ns, token = rest >> 1;
+    float v = 0;
+    if (lengths == nullptr || token % length < row_length(lengths, token / length, length))
+        for (int k = 0; k < parts; k++) v += part[k * all + at];
+    ((typename T::raw *)(rest & 1 ? dC : dB))[token * states + n] = down<T>(v);
+}
+
+struct ScanOut {
+    float *dA, *dD, *dbias;
+    int width, states, ns;
+    __device__ void operator()(int64_t col, float v) const {
+        int n = (int)(col / width), e = (int)(col % width);
+        if (n < states) {
+            if (dA != nullptr) dA[(int64_t)e * states + n] = v;
+        } else if (n == ns) {
+            if (dD != nullptr) dD[e] = v;
+        } else if (n == ns + 1 && dbias != nullptr) dbias[e] = v;
+    }
+};
+
+// ---- one token ----
+// Q lanes share a channel, four states each: the state goes through registers in 16-byte pieces, in order of memory.  Bound by memory:
+// 8 bytes a state.  Q = 0: a lane takes a channel's states one by one, for numbers of states that four lanes cannot share evenly.
+template <class T, int Q> __global__ __launch_bounds__(256) void scan_step(ScanArgs a, const void *B, const void *C, int64_t B_batch, int64_t C_batch) {
+    using raw = typename T::raw;
+    constexpr int kLanesOf = Q > 0 ? Q : 1;
+    int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, row = at / kLanesOf;
+    if (row >= a.batch * a.width) return;            // whole groups of Q lanes leave together
+    int q = (int)(at % kLanesOf), e = (int)(row % a.width);
+    int64_t b = row / a.width;
+    float uf = up<T>(((const raw *)a.u)[b * a.u_batch + e]);
+    float d = softplus_(up<T>(((const raw *)a.dt)[b * a.dt_batch + e]) + (a.dt_bias != nullptr ? a.dt_bias[e] : 0.0f)), x = d * uf, o = 0;
+    bool first = a.reset != nullptr && a.reset[b * a.reset_batch] != 0;
+    const raw *Bp = (const raw *)B + b * B_batch, *Cp = (const raw *)C + b * C_batch;
+    const float *from = a.state + row * a.states, *A = a.A + (int64_t)e * a.states;
+    float *to = a.last + row * a.states;
+    if constexpr (Q > 0) {
+        Vec<F32, 4> h = load<F32, 4>(from + q * 4), r = load<F32, 4>(A + q * 4);
+        Vec<T, 4> Bv = load<T, 4>(Bp + q * 4), Cv = load<T, 4>(Cp + q * 4);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float keep = first ? 0.0f : exp2_(d * (r.v[i] * kLog2e)) * h.v[i];
+            h.v[i] = __builtin_fmaf(x, up<T>(Bv.v[i]), keep);
+            o = __builtin_fmaf(up<T>(Cv.v[i]), h.v[i], o);
+        }
+        store<F32, 4>(to + q * 4, h);
+        o = lane_sum<Q>(o);
+    } else {
+        for (int n = 0; n < a.states; n++) {
+            float keep = first ? 0.0f : exp2_(d * (A[n] * kLog2e)) * from[n];
+            float h = __builtin_fmaf(x, up<T>(Bp[n]), keep);
+            o = __builtin_fmaf(up<T>(Cp[n]), h, o);
+            to[n] = h;
+        }
+    }
+    if (q == 0) {
+        if (a.D != nullptr) o = __builtin_fmaf(a.D[e], uf, o);
+        if (a.z != nullptr) {
+            float zf = up<T>(((const raw *)a.z)[b * a.z_batch + e]);
+            o *= zf * sigmoid_(zf);
+        }
+        ((raw *)a.y)[row] = down<T>(o);
+    }
+}
+
+// ---- host ----
+static int scan_ns(const mws_scan_args *a) { return a->states <= 4 ? 4 : a->states <= 8 ? 8 : a->states <= 16 ? 16 : 32; }
+
+struct ScanPlan {
+    int ns, lanes, across, segments, span, groups;
+    int64_t chunks;
+    int64_t bc, seg, sum, part_bc, part, bytes;      // offsets into the workspace, in floats
+};
+
+// Segments: the time axis is cut where the waves over batch and channels leave the SIMDs without two waves each; cutting doubles
+// the work (each segment is walked twice), so that it is worth it from four segments on.
+static ScanPlan scan_plan(const mws_scan_args *a, bool backward) {
+    ScanPlan p = {};
+    p.ns = scan_ns(a);
+    int waves = (int)ceil_div(a->width, kWave);
+    p.lanes = (waves < lanes_of(p.ns) / kWave ? waves : lanes_of(p.ns) / kWave) * kWave;
+    p.across = (int)ceil_div(a->width, p.lanes);
+    p.chunks = ceil_div(a->length, chunk_of(p.ns));
+    int64_t blocks = a->batch * p.across, wanted = ceil_div(2 * kSimds, blocks > 0 ? blocks * (p.lanes / kWave) : 1);
+    int64_t segments = wanted < p.chunks ? wanted : p.chunks;
+    if (segments < 4) segments = 1;
+    int64_t chunks = p.chunks > 0 ? p.chunks : 1, each = ceil_div(chunks, segments);
+    p.segments = (int)ceil_div(chunks, each);
+    p.span = (int)(each * chunk_of(p.ns));
+    int64_t items = a->batch * p.segments, most = 2048 / p.across > 0 ? 2048 / p.across : 1;
+    p.groups = (int)(items < most ? items : most);
+    int64_t at = 0, tokens = a->batch * a->length;
+    auto take = [&at](int64_t n) {
+        int64_t from = at;
+        at += (n + 63) / 64 * 64;
+        return from;
+    };
+    p.bc = take(tokens * 2 * p.ns);
+    p.seg = take(p.segments > 1 ? a->batch * p.segments * p.ns * a->width : 0);
+    p.sum = take(p.segments > 1 ? a->batch * p.segments * a->width : 0);
+    p.part_bc = take(backward ? p.across * tokens * 2 * p.ns : 0);
+    p.part = take(backward ? (int64_t)p.groups * (p.ns + 2) * a->width : 0);
+    p.bytes = at * (int64_t)sizeof(float);
+    return p;
+}
+
+static int32_t scan_check(const mws_scan_args *a, const char *what, bool backward, bool step, bool pointers) {
+    if (a == nullptr) return fail("%s: no arguments", what);
+    if (a->type < MWS_F32 || a->type > MWS_F16) return fail("%s: type %d is none of MWS_F32, MWS_BF16, MWS_F16", what, a->type);
+    if (a->states < 1 || a->states > MWS_SCAN_MAX_STATES) return fail("%s: %d states are not within 1 .. %d", what, a->states, MWS_SCAN_MAX_STATES);
+    if (a->width < 1 || a->width > (1 << 24)) return fail("%s: width %d", what, a->width);
+    if (a->batch < 0 || a->length < 0 || a->batch > (1 << 30) || a->length > (1 << 30) || a->batch * (a->length + 1) > ((int64_t)1 << 33)) return fail("%s: %lld rows of %lld tokens", what, (long long)a->batch, (long long)a->length);
+    if (step && a->length != 1) return fail("%s: one token at a time", what);
+    if (!pointers) return 0;
+    if (a->A == nullptr) return fail("%s: A is NULL", what);
+    if (a->batch == 0) return 0;
+    if (a->length > 0 && (a->u == nullptr || a->dt == nullptr || a->B == nullptr || a->C == nullptr)) return fail("%s: u, dt, B or C is NULL", what);
+    if (!backward && a->length > 0 && a->y == nullptr) return fail("%s: y is NULL", what);
+    if (backward && a->length > 0 && (a->dy == nullptr || a->kept == nullptr || a->du == nullptr || a->ddt == nullptr || a->dB == nullptr || a->dC == nullptr)) return fail("%s: dy, kept, du, ddt, dB or dC is NULL", what);
+    if (backward && a->length > 0 && a->z != nullptr && a->dz == nullptr) return fail("%s: dz is NULL", what);
+    if (step && (a->state == nullptr || a->last == nullptr)) return fail("%s: the state is NULL", what);
+    return 0;
+}
+
+static ScanArgs scan_device(const mws_scan_args *a, const ScanPlan &p) {
+    ScanArgs d = {};
+    float *w = (float *)a->workspace;
+    d.u = a->u, d.dt = a->dt, d.z = a->z, d.dy = a->dy, d.A = a->A, d.D = a->D, d.dt_bias = a->dt_bias, d.state = a->state, d.dlast = a->dlast;
+    d.reset = a->reset, d.lengths = a->lengths, d.y = a->y, d.du = a->du, d.ddt = a->ddt, d.dz = a->dz;
+    d.last = a->last, d.kept = a->kept, d.dstate = a->dstate;
+    if (w != nullptr) d.bc = w + p.bc, d.seg = w + p.seg, d.sum = w + p.sum, d.part_bc = w + p.part_bc, d.part = w + p.part;
+    d.batch = a->batch, d.length = a->length, d.chunks = p.chunks;
+    d.u_batch = a->u_batch, d.u_time = a->u_time, d.dt_batch = a->dt_batch, d.dt_time = a->dt_time, d.z_batch = a->z_batch, d.z_time = a->z_time;
+    d.dy_batch = a->dy_batch, d.dy_time = a->dy_time, d.reset_batch = a->reset_batch, d.reset_time = a->reset_time;
+    d.width = a->width, d.states = a->states, d.across = p.across, d.segments = p.segments, d.span = p.span, d.groups = p.groups;
+    return d;
+}
+
+template <class T> static void spread_go(const mws_scan_args *a, const ScanPlan &p, const ScanArgs &d, hipStream_t stream) {
+    int64_t count = a->batch * a->length * 2 * p.ns;
+    if (count > 0)
+        hipLaunchKernelGGL((spread<T>), dim3((unsigned)ceil_div(count, 256)), dim3(256), 0, stream, a->B, a->C, const_cast<float *>(d.bc), a->length, a->B_batch, a->B_time, a->C_batch,
+                           a->C_time, a->states, p.ns, count);
+}
+static void join_go(const ScanArgs &d, int ns, bool backward, hipStream_t stream) {
+    hipLaunchKernelGGL(scan_join, dim3((unsigned)ceil_div(d.batch * ns * d.width, 256)), dim3(256), 0, stream, d, ns, backward);
+}
+
+template <class T, int NS> static void forward_go(const ScanPlan &p, const ScanArgs &d, hipStream_t stream) {
+    dim3 grid((unsigned)(d.batch * p.segments * p.across)), block(p.lanes);
+    if (p.segments > 1) {
+        hipLaunchKernelGGL((scan_segment<T, NS>), grid, block, 0, stream, d);
+        join_go(d, NS, false, stream);
+    }
+    hipLaunchKernelGGL((scan_forward<T, NS>), grid, block, 0, stream, d);
+}
+template <class T, int NS> static void backward_go(const mws_scan_args *a, const ScanPlan &p, const ScanArgs &d, hipStream_t stream) {
+    constexpr int kChunk = chunk_of(NS), SUB = sub_of(NS);
+    dim3 block(p.lanes);
+    if (p.segments > 1) {
+        hipLaunchKernelGGL((scan_segment_back<T, NS>), dim3((unsigned)(d.batch * p.segments * p.across)), block, 0, stream, d);
+        join_go(d, NS, true, stream);
+    }
+    size_t lds = (size_t)(p.lanes / kWave) * ((kChunk / SUB - 1) * NS * kWave + kChunk * 2 * NS) * sizeof(float);
+    if (d.batch > 0) hipLaunchKernelGGL((scan_backward<T, NS>), dim3((unsigned)(p.groups * p.across)), block, lds, stream, d);
+    int64_t count = d.batch * d.length * 2 * NS;
+    if (count > 0)
+        hipLaunchKernelGGL((scan_bc_out<T>), dim3((unsigned)ceil_div(count, 256)), dim3(256), 0, stream, d.part_bc, a->lengths, a->dB, a->dC, d.batch, d.length, p.across, a->states, NS);
+    ScanOut out = {a->dA, a->dD, a->ddt_bias, a->width, a->states, NS};
+    launch_sum_parts(d.part, p.groups, (int64_t)(NS + 2) * a->width, out, stream);
+}
+template <class T> static void scan_go(const mws_scan_args *a, const ScanPlan &p, const ScanArgs &d, bool backward, hipStream_t stream) {
+    spread_go<T>(a, p, d, stream);
+#define MWS_GO(NS) (backward ? backward_go<T, NS>(a, p, d, stream) : forward_go<T, NS>(p, d, stream))
+    if (p.ns == 4) MWS_GO(4);
+    else if (p.ns == 8) MWS_GO(8);
+    else if (p.ns == 16) MWS_GO(16);
+    else MWS_GO(32);
+#undef MWS_GO
+}
+static void scan_run(const mws_scan_args *a, const ScanPlan &p, const ScanArgs &d, bool backward, hipStream_t stream) {
+    if (a->type == MWS_F32) scan_go<F32>(a, p, d, backward, stream);
+    else if (a->type == MWS_BF16) scan_go<BF16>(a, p, d, backward, stream);
+    else scan_go<F16>(a, p, d, backward, stream);
+}
+template <class T> static void step_go(const mws_scan_args *a, const ScanArgs &d, hipStream_t stream) {
+    int q = a->states == 4 ? 1 : a->states == 8 ? 2 : a->states == 16 ? 4 : a->states == 32 ? 8 : 0;
+    dim3 grid((unsigned)ceil_div(d.batch * d.width * (q > 0 ? q : 1), 256));
+#define MWS_GO(Q) hipLaunchKernelGGL((scan_step<T, Q>), grid, dim3(256), 0, stream, d, a->B, a->C, a->B_batch, a->C_batch)
+    if (q == 1) MWS_GO(1);
+    else if (q == 2) MWS_GO(2);
+    else if (q == 4) MWS_GO(4);
+    else if (q == 8) MWS_GO(8);
+    else MWS_GO(0);
+#undef MWS_GO
+}
+}  // namespace mws
+
+using namespace mws;
+
+extern "C" int64_t mws_scan_kept(const mws_scan_args *a) {
+    if (int32_t e = scan_check(a, "mws_scan_kept", false, false, false)) return e;
+    return a->batch * ceil_div(a->length, chunk_of(scan_ns(a))) * scan_ns(a) * a->width;
+}
+
+extern "C" int64_t mws_scan_workspace(const mws_scan_args *a, int32_t backward) {
+    if (int32_t e = scan_check(a, "mws_scan_workspace", false, false, false)) return e;
+    return scan_plan(a, backward != 0).bytes;
+}
+
+static int32_t scan_call(const mws_scan_args *a, const char *what, bool backward, void *stream) {
+    if (int32_t e = scan_check(a, what, backward, false, true)) return e;
+    ScanPlan p = scan_plan(a, backward);
+    if (a->workspace_bytes < p.bytes || (p.bytes > 0 && a->workspace == nullptr)) return fail("%s: the workspace needs %lld bytes", what, (long long)p.bytes);
+    if (!backward && a->batch == 0) return 0;
+    if (a->batch * p.segments * p.across > 0x7fffffff) return fail("%s: too many rows", what);
+    scan_run(a, p, scan_device(a, p), backward, (hipStream_t)stream);
+    return launched(what);
+}
+extern "C" int32_t mws_scan_forward(const mws_scan_args *a, void *stream) { return scan_call(a, "mws_scan_forward", false, stream); }
+extern "C" int32_t mws_scan_backward(const mws_scan_args *a, void *stream) { return scan_call(a, "mws_scan_backward", true, stream); }
+
+extern "C" int32_t mws_scan_step(const mws_scan_args *a, void *stream) {
+    if (int32_t e = scan_check(a, "mws_scan_step", false, true, true)) return e;
+    if (a->batch == 0) return 0;
+    ScanPlan none = {};
+    ScanArgs d = scan_device(a, none);
+    if (a->type == MWS_F32) step_go<F32>(a, d, (hipStream_t)stream);
+    else if (a->type == MWS_BF16) step_go<BF16>(a, d, (hipStream_t)stream);
+    else step_go<F16>(a, d, (hipStream_t)stream);
+    return launched("mws_scan_step");
+}

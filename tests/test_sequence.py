@@ -1,0 +1,711 @@
+"""The operators of a policy with memory (metaworld_amd.sequence) against plain implementations in 64 bits, written from the formulas:
+values, gradients (the formulas' and central differences), states, empty and padded rows, strides, streams, graphs; and their refusals.
+
+Tolerances.  An output of type t is rounded once, by at most half a step: eps(t) / 2 relative.  Before that everything is float32: an
+operation is off by at most 2^-24 relative to its operands' magnitude (the hardware's exp2, log2 and reciprocal by twice that), so that
+an output with n operations on its longest path is off by at most n 2^-24 times its MAGNITUDE, the same sum with every term's absolute
+value, which the plain implementations compute as well.  n is counted beside each test.
+"""
+import numpy as np
+import pytest
+import torch
+
+from metaworld_amd import sequence
+
+gpu = pytest.mark.gpu
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+U = 2.0 ** -24
+
+
+def check(what, got, want, mag, n):
+    kind = got.dtype
+    g, w, m = got.detach().double().cpu(), want.double(), mag.double()
+    assert g.shape == w.shape, (what, g.shape, w.shape)
+    # values below a type's smallest normal number are rounded to its fixed step there
+    tol = torch.finfo(kind).eps / 2 * (w.abs() + n * U * m) + n * U * m + torch.finfo(kind).tiny * torch.finfo(kind).eps
+    bad = (g - w).abs() > tol
+    assert not bad.any() and torch.isfinite(g).all(), f"{what}: {int(bad.sum())} of {bad.numel()} values off, by up to {float(((g - w).abs() / tol).max()):.3g} of the tolerance"
+
+
+def rand(gen, *shape, scale=1.0, kind=torch.float64):
+    """values of type `kind`, as their own type's numbers in 64 bits"""
+    return (torch.randn(shape, generator=gen, dtype=torch.float64) * scale).to(kind).double()
+
+
+def seeded(*numbers):
+    return torch.Generator().manual_seed(sum(n * p for n, p in zip(numbers, (1, 31, 1009, 40009))))
+
+
+def on(t, kind=None, grad=False):
+    if t is None:
+        return None
+    t = t.to("cuda") if kind is None else t.to("cuda", kind)
+    return t.requires_grad_() if grad else t
+
+
+# ---- layer norm ----
+def plain_norm(x, w, b, eps, dy, mag=False):
+    """y, dx, dw, db; with `mag` the sums of absolute values that the same formulas add"""
+    mean = x.mean(-1, keepdim=True)
+    r = ((x - mean).square().mean(-1, keepdim=True) + eps).rsqrt()
+    if not mag:
+        n = (x - mean) * r
+        g = dy * w
+        return n * w + b, r * (g - g.mean(-1, keepdim=True) - n * (g * n).mean(-1, keepdim=True)), (dy * n).sum(0), dy.sum(0)
+    n = (x.abs() + x.abs().mean(-1, keepdim=True)) * r
+    n = n + n * (n * n).mean(-1, keepdim=True)            # an error of r is one of the squares' sum
+    g = (dy * w).abs()
+    return n * w.abs() + b.abs(), r * (g + g.mean(-1, keepdim=True) + n * (g * n).mean(-1, keepdim=True)), (dy.abs() * n).sum(0), dy.abs().sum(0)
+
+
+@gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows,width", [(1, 1), (3, 7), (50, 32), (33, 100), (70, 128), (5, 257), (130, 395), (9, 512), (4, 700), (6, 1024), (3, 1500), (5, 3000), (2, 5001), (3, 8192), (2, 16384),
+                                        (3000, 64)])
+def test_layer_norm(kind, rows, width):
+    gen = seeded(rows, width)
+    x, dy = rand(gen, rows, width, kind=kind) , rand(gen, rows, width, kind=kind)
+    x = (x * 1.5 + 0.5).to(kind).double()
+    for par in {torch.float32, kind}:
+        w, b = (1 + rand(gen, width, scale=0.2)).to(par).double(), rand(gen, width, kind=par)
+        gx, gw, gb = on(x, kind, True), on(w, par, True), on(b, par, True)
+        y = sequence.layer_norm(gx, gw, gb)
+        dx, dw, db = torch.autograd.grad(y, (gx, gw, gb), on(dy, kind))
+        assert y.dtype == dx.dtype == kind and dw.dtype == db.dtype == par
+        eps = float(np.float32(1e-5))
+        # two sums over the row (a tree: width / 64 + 16 additions), a square root, a division and a handful of products; the parameters' sums add `rows` terms
+        n = 4 * (width // 64 + 32)
+        for what, got, want, mag in zip(("y", "dx", "dw", "db"), (y, dx, dw, db), plain_norm(x, w, b, eps, dy), plain_norm(x, w, b, eps, dy, True)):
+            check(f"{what} {par}", got, want, mag, n + (rows if what[1:] in "wb" else 0))
+        # without recording the same values, without parameters the same formula
+        with torch.no_grad():
+            assert torch.equal(y, sequence.layer_norm(gx, gw, gb))
+            bare = sequence.layer_norm(gx)
+        one, none = torch.ones(width, dtype=torch.float64), torch.zeros(width, dtype=torch.float64)
+        check("bare", bare, plain_norm(x, one, none, eps, dy)[0], plain_norm(x, one, none, eps, dy, True)[0], n)
+
+
+@gpu
+def test_layer_norm_shapes_strides_and_broadcast_inputs():
+    gen = seeded(5)
+    big = on(rand(gen, 6, 4, 90), torch.float32)
+    with torch.no_grad():
+        want = sequence.layer_norm(big[:, :, :45].contiguous())
+        assert torch.equal(want, sequence.layer_norm(big[:, :, :45]))                                     # rows apart
+        assert torch.equal(want.transpose(0, 1), sequence.layer_norm(big[:, :, :45].transpose(0, 1)))
+        assert torch.equal(want[2, 1], sequence.layer_norm(big[2, 1, :45]))                               # one dimension
+        odd = big.transpose(1, 2).contiguous().transpose(1, 2)[:, :, :45]                                 # the last dimension not contiguous
+        assert torch.equal(want, sequence.layer_norm(odd))
+        assert sequence.layer_norm(big[:0]).shape == (0, 4, 90)
+    # one row seen many times: its gradient is the sum over them
+    row = big[0, 0].clone().requires_grad_()
+    y = sequence.layer_norm(row.expand(7, 90))
+    dy = torch.randn_like(y)
+    got, = torch.autograd.grad(y, row, dy)
+    again = big[0, 0].clone().requires_grad_()
+    want, = torch.autograd.grad(sequence.layer_norm(again), again, dy.sum(0))
+    assert torch.allclose(got, want, rtol=1e-4, atol=1e-5)
+    # no row at all: the parameters' gradients are zeros
+    w = torch.ones(90, device="cuda", requires_grad=True)
+    assert torch.equal(torch.autograd.grad(sequence.layer_norm(big[:0].reshape(0, 90), w).sum(), w)[0], torch.zeros_like(w))
+    # rows that are constant: no variance, y is the bias
+    flat = torch.full((3, 90), 2.5, device="cuda")
+    assert torch.equal(sequence.layer_norm(flat), torch.zeros_like(flat))
+
+
+# ---- tokens of both operators over time ----
+def flags(gen, batch, time, kind):
+    """reset and lengths: rows of all lengths with the empty and the full one among them, episodes that begin at first, last and any tokens"""
+    if kind == "plain":
+        return None, None
+    reset = torch.rand((batch, time), generator=gen) < 0.15
+    reset[0, 0] = True
+    reset[-1, -1] = True
+    if kind == "reset":
+        return reset, None
+    lengths = torch.randint(0, time + 1, (batch,), generator=gen, dtype=torch.int32)
+    lengths[0] = 0 if batch > 1 else time
+    lengths[-1] = time
+    return reset, lengths
+
+
+def fill_unused(t, lengths, value=float("nan")):
+    """the inputs that no length counts, so that they show wherever they are used"""
+    if lengths is not None:
+        for b, n in enumerate(lengths.tolist()):
+            t[b, n:] = value
+    return t
+
+
+# ---- convolution ----
+def plain_conv(x, w, b, state, reset, lengths, dy, dlast, mag=False):
+    """token by token: y, last, dx, dw, db, dstate"""
+    batch, time, width = x.shape
+    taps = w.shape[1]
+    if mag:
+        x, w, b, state, dy, dlast = (t.abs() for t in (x, w, b, state, dy, dlast))
+    y, dx, dw, db, dstate = torch.zeros_like(x), torch.zeros_like(x), torch.zeros_like(w), torch.zeros_like(b), torch.zeros_like(state)
+    last = torch.zeros_like(state)
+    for r in range(batch):
+        end = time if lengths is None else int(lengths[r])
+        values, grads, began = list(state[r]) + list(x[r, :end]), [torch.zeros(width, dtype=torch.float64) for _ in range(taps - 1 + end)], -taps
+        seen = []
+        for t in range(end):
+            if reset is not None and reset[r, t]:
+                began = t
+            seen.append([j for j in range(taps) if t - taps + 1 + j >= began])
+            pre = b + sum(w[:, j] * values[t + j] for j in seen[t])
+            sig = torch.sigmoid(pre) if not mag else torch.ones_like(pre)
+            y[r, t] = pre * sig * (1 if not mag else 2)           # |silu'| <= 1.1
+            d = dy[r, t] * (sig * (1 + pre * (1 - sig)) if not mag else 1.1 + pre)        # an error of pre moves silu' by half of it at most
+            db += d
+            for j in seen[t]:
+                dw[:, j] += d * values[t + j]
+                grads[t + j] += d * w[:, j]
+        for j in range(taps - 1):
+            if end - taps + 1 + j >= began:
+                last[r, j] = values[end + j]
+                grads[end + j] += dlast[r, j]
+        for j in range(taps - 1):
+            dstate[r, j] = grads[j]
+        for t in range(end):
+            dx[r, t] = grads[taps - 1 + t]
+    return y, last, dx, dw, db, dstate
+
+
+CONV_NAMES = ("y", "last", "dx", "dw", "db", "dstate")
+
+
+@gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("marks", ["plain", "reset", "padded"])
+@pytest.mark.parametrize("batch,time,width,taps", [(1, 1, 1, 2), (3, 2, 5, 4), (2, 9, 130, 3), (4, 33, 64, 4), (2, 40, 517, 4), (5, 70, 9, 2), (70, 5, 33, 4)])
+def test_causal_conv(kind, marks, batch, time, width, taps):
+    gen = seeded(batch, time, width, taps)
+    reset, lengths = flags(gen, batch, time, marks)
+    x, dy = rand(gen, batch, time, width, kind=kind), rand(gen, batch, time, width, kind=kind)
+    state, dlast = rand(gen, batch, taps - 1, width, kind=kind), rand(gen, batch, taps - 1, width, kind=kind)
+    # taps + 1 additions, the activation (exp, two products, an addition, a reciprocal: 8), its slope, taps more for dx; the parameters' sums add all tokens
+    n = 2 * taps + 24
+    for par in {torch.float32, kind}:
+        w, b = rand(gen, width, taps, scale=0.5, kind=par), rand(gen, width, scale=0.3, kind=par)
+        want, mag = (plain_conv(x, w, b, state, reset, lengths, dy, dlast, m) for m in (False, True))
+        leaves = on(fill_unused(x.clone(), lengths), kind, True), on(w, par, True), on(b, par, True), on(state, kind, True)
+        y, last = sequence.causal_conv(*leaves[:3], state=leaves[3], reset=on(reset), lengths=on(lengths))
+        grads = torch.autograd.grad((y, last), leaves, (on(fill_unused(dy.clone(), lengths), kind), on(dlast, kind)))
+        for what, got, v, m in zip(CONV_NAMES, (y, last, *grads), want, mag):
+            check(f"{what} {par}", got, v, m, n + (batch * time if what in ("dw", "db") else 0))
+        with torch.no_grad():
+            again = sequence.causal_conv(*leaves[:3], state=leaves[3], reset=on(reset), lengths=on(lengths))
+        assert torch.equal(again[0], y) and torch.equal(again[1], last)
+
+
+@gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("taps", [2, 3, 4])
+def test_causal_conv_step_by_step_is_the_whole(kind, taps):
+    gen = seeded(11, taps)
+    batch, time, width = 37, 12, 83
+    reset = torch.rand((batch, time), generator=gen) < 0.2
+    x, w, b, state = rand(gen, batch, time, width, kind=kind), rand(gen, width, taps), rand(gen, width), rand(gen, batch, taps - 1, width, kind=kind)
+    gx, gw, gb, gr, held = on(x, kind), on(w, torch.float32), on(b, torch.float32), on(reset), on(state, kind)
+    with torch.no_grad():
+        y, last = sequence.causal_conv(gx, gw, gb, state=held, reset=gr)
+        before = held._version
+        steps = [sequence.causal_conv_step(gx[:, t], gw, gb, state=held, reset=gr[:, t]) for t in range(time)]
+    assert torch.equal(last, held) and held._version == before + time
+    # the same products, added in another order
+    zero = torch.zeros(batch, time, width)
+    _, mag = (plain_conv(x, w.float().double(), b.float().double(), state, reset, None, zero.double(), torch.zeros_like(state), m) for m in (False, True))
+    check("steps", torch.stack(steps, 1), y.double().cpu(), mag[0], 2 * (2 * taps + 24) + (0 if kind == torch.float32 else torch.finfo(kind).eps / 2 / U))
+
+
+# ---- scan ----
+def plain_scan(u, dt, A, B, C, D, z, bias, state, reset, lengths, dy, dlast, mag=False):
+    """token by token: y, last, du, ddt, dA, dB, dC, dD, dz, dbias, dstate"""
+    f = torch.abs if mag else (lambda t: t)
+    u, B, C, D, state, dy, dlast = (f(t) for t in (u, B, C, D, state, dy, dlast))
+    batch, time, width = u.shape
+    y = torch.zeros_like(u)
+    out = {k: torch.zeros_like(t) for k, t in (("u", u), ("dt", dt), ("A", A), ("B", B), ("C", C), ("D", D), ("z", z), ("bias", bias), ("state", state))}
+    last = torch.zeros_like(state)
+    for r in range(batch):
+        end = time if lengths is None else int(lengths[r])
+        h, tape = state[r], []
+        for t in range(end):
+            raw = dt[r, t] + bias
+            d = torch.nn.functional.softplus(raw, threshold=40)
+            a = torch.exp(d[:, None] * A) * (0.0 if reset is not None and reset[r, t] else 1.0)
+            kept = a * h
+            h = kept + (d * u[r, t])[:, None] * B[r, t]
+            o = (h * C[r, t]).sum(1) + D * u[r, t]
+            sig = torch.sigmoid(z[r, t])
+            y[r, t] = o * f(z[r, t] * sig)
+            tape.append((raw, d, a, kept, h, o, sig))
+        last[r] = h
+        g = dlast[r]
+        for t in reversed(range(end)):
+            raw, d, a, kept, h, o, sig = tape[t]
+            do = dy[r, t] * f(z[r, t] * sig)
+            out["z"][r, t] = dy[r, t] * o * f(sig * (1 + z[r, t] * (1 - sig))) if not mag else dy[r, t] * o * (1.1 + z[r, t].abs())
+            out["C"][r, t] = (do[:, None] * h).sum(0)
+            out["D"] += do * u[r, t]
+            g = g + do[:, None] * C[r, t]
+            out["B"][r, t] = (g * (d * u[r, t])[:, None]).sum(0)
+            gB = (g * B[r, t]).sum(1)
+            out["u"][r, t] = D * do + d * gB
+            draw = (u[r, t] * gB + (g * kept * f(A)).sum(1)) * torch.sigmoid(raw)
+            out["dt"][r, t] = draw
+            out["bias"] += draw
+            out["A"] += g * kept * d[:, None]
+            g = a * g
+        out["state"][r] = g
+    return y, last, *out.values()
+
+
+SCAN_NAMES = ("y", "last", "du", "ddt", "dA", "dB", "dC", "dD", "dz", "dbias", "dstate")
+
+
+def scan_inputs(gen, batch, time, width, states, kind):
+    u, dt, z = (rand(gen, batch, time, width, scale=s, kind=kind) for s in (0.7, 0.7, 1.0))
+    B, C = rand(gen, batch, time, states, kind=kind), rand(gen, batch, time, states, kind=kind)
+    A = (-torch.rand((width, states), generator=gen, dtype=torch.float64) * 4 - 0.05).float().double()
+    D, bias = rand(gen, width, kind=torch.float32), (rand(gen, width, scale=0.8) - 2).float().double()
+    return u, dt, A, B, C, D, z, bias, rand(gen, batch, width, states, kind=torch.float32)
+
+
+def scan_operations(ins, time, tokens):
+    """n: a token's factor exp(d A) is off by the 8 roundings of softplus and the product, times |d A|, and 2 of exp2; with its product and sum
+    4 + 8 |d A| a token, there and back over the whole row; then sums over states, channels (waves and blocks: 32) and tokens, and the gates"""
+    u, dt, A, bias = ins[0], ins[1], ins[2], ins[7]
+    d = torch.nn.functional.softplus(dt + bias, threshold=40)
+    return 2 * time * (4 + 8 * float(d.max()) * float(A.abs().max())) + tokens + 128
+
+
+@gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("marks", ["plain", "reset", "padded"])
+@pytest.mark.parametrize("batch,time,width,states", [(1, 1, 1, 1), (2, 3, 65, 5), (3, 33, 70, 16), (2, 65, 300, 16), (2, 40, 130, 32), (3, 9, 64, 8), (1, 200, 20, 4), (2, 150, 33, 12)])
+def test_selective_scan(kind, marks, batch, time, width, states):
+    gen = seeded(batch, time, width, states)
+    reset, lengths = flags(gen, batch, time, marks)
+    ins = scan_inputs(gen, batch, time, width, states, kind)
+    dy, dlast = rand(gen, batch, time, width, kind=kind), rand(gen, batch, width, states, kind=torch.float32)
+    want, mag = (plain_scan(*ins, reset, lengths, dy, dlast, m) for m in (False, True))
+    n = scan_operations(ins, time, batch * time)
+    given = [fill_unused(t.clone(), lengths) if k in (0, 1, 3, 4, 6) else t for k, t in enumerate(ins)]
+    leaves = [on(t, kind if k in (0, 1, 3, 4, 6) else torch.float32, True) for k, t in enumerate(given)]
+    y, last = sequence.selective_scan(*leaves[:8], state=leaves[8], reset=on(reset), lengths=on(lengths))
+    grads = torch.autograd.grad((y, last), leaves, (on(fill_unused(dy.clone(), lengths), kind), on(dlast, torch.float32)))
+    for what, got, v, m in zip(SCAN_NAMES, (y, last, *grads), want, mag):
+        check(what, got, v, m, n)
+    with torch.no_grad():
+        again = sequence.selective_scan(*leaves[:8], state=leaves[8], reset=on(reset), lengths=on(lengths))
+    assert torch.equal(again[0], y) and torch.equal(again[1], last)
+
+
+@gpu
+@pytest.mark.parametrize("states", [1, 4, 7, 8, 16, 32])
+@pytest.mark.parametrize("kind", TYPES)
+def test_selective_scan_step_by_step_is_the_whole(kind, states):
+    gen = seeded(23, states)
+    batch, time, width = 19, 10, 43
+    reset = torch.rand((batch, time), generator=gen) < 0.2
+    ins = scan_inputs(gen, batch, time, width, states, kind)
+    u, dt, A, B, C, D, z, bias, held = (on(t, kind if k in (0, 1, 3, 4, 6) else torch.float32) for k, t in enumerate(ins))
+    gr = on(reset)
+    zero = torch.zeros(batch, time, width, dtype=torch.float64), torch.zeros(batch, width, states, dtype=torch.float64)
+    want, mag = (plain_scan(*ins, reset, None, *zero, m) for m in (False, True))
+    before = held._version
+    with torch.no_grad():
+        steps = [sequence.selective_scan_step(u[:, t], dt[:, t], A, B[:, t], C[:, t], D, z[:, t], bias, state=held, reset=gr[:, t]) for t in range(time)]
+    assert held._version == before + time
+    n = scan_operations(ins, time, 1)
+    check("steps", torch.stack(steps, 1), want[0], mag[0], n)
+    check("state", held, want[1], mag[1], n)
+
+
+@gpu
+def test_scan_without_the_optional_inputs():
+    gen = seeded(3)
+    batch, time, width, states = 2, 37, 50, 16
+    u, dt, A, B, C, D, z, bias, state = scan_inputs(gen, batch, time, width, states, torch.float32)
+    dy = rand(gen, batch, time, width)
+    none = torch.zeros_like
+    leaves = [on(t, torch.float32, True) for t in (u, dt, A, B, C)]
+    y, last = sequence.selective_scan(*leaves)
+    grads = torch.autograd.grad(y, leaves, on(dy, torch.float32))
+    # silu(z) = 1 at z = z1: scale D and C by it afterwards; simplest is z large, where silu(z) = z to 64 bits
+    big = torch.full_like(z, 64.0)
+    args = (u, dt, A, B, C / 64, none(D), big, none(bias), none(state), None, None, dy, none(state))
+    want, mag = plain_scan(*args), plain_scan(*args, True)
+    n = scan_operations((u, dt, A, None, None, None, None, none(bias)), time, batch * time)
+    for k, got in zip((0, 1, 2, 3, 4, 5), (y, last, *grads[:4])):
+        check(SCAN_NAMES[k], got, want[k], mag[k], n)
+    check("dC", grads[4], want[6] / 64, mag[6] / 64, n)
+    # the last state's gradient alone
+    got = torch.autograd.grad(sequence.selective_scan(*leaves)[1], leaves[0], torch.ones(batch, width, states, device="cuda"))[0]
+    args = (u, dt, A, B, C, none(D), z, none(bias), none(state), None, None, none(dy), torch.ones_like(state))
+    check("du of the state", got, plain_scan(*args)[2], plain_scan(*args, True)[2], n)
+
+
+@gpu
+@pytest.mark.parametrize("batch,time,width,states", [(1, 700, 70, 16), (2, 2000, 33, 4), (1, 500, 20, 32)])
+def test_scan_of_long_rows_in_segments(batch, time, width, states):
+    """few channels and many tokens: the time axis is cut, with and without an episode's beginning in a segment and rows that end in one"""
+    gen = seeded(batch, time, width, states)
+    ins = scan_inputs(gen, batch, time, width, states, torch.float32)
+    dy, dlast = rand(gen, batch, time, width, kind=torch.float32), rand(gen, batch, width, states, kind=torch.float32)
+    few = torch.zeros(batch, time, dtype=torch.bool)
+    few[0, time // 3] = few[-1, time - 70] = True
+    ends = torch.full((batch,), time - 190, dtype=torch.int32)
+    for reset, lengths in ((None, None), (few, None), (few, ends)):
+        want, mag = (plain_scan(*ins, reset, lengths, dy, dlast, m) for m in (False, True))
+        leaves = [on(t, torch.float32, True) for t in ins]
+        y, last = sequence.selective_scan(*leaves[:8], state=leaves[8], reset=on(reset), lengths=on(lengths))
+        grads = torch.autograd.grad((y, last), leaves, (on(dy, torch.float32), on(dlast, torch.float32)))
+        for what, got, v, m in zip(SCAN_NAMES, (y, last, *grads), want, mag):
+            check(what, got, v, m, scan_operations(ins, time, batch * time))
+
+
+@gpu
+@pytest.mark.parametrize("which", ["norm", "conv", "scan"])
+def test_gradients_against_differences(which):
+    """central differences of the plain 64-bit values along a random direction: off by h^2 of third derivatives (h = 1e-4), and the kernels' gradient by
+    their float32 roundings: 1e-3 of the direction's own scale holds both by far and would show any wrong term"""
+    gen = seeded(41)
+    if which == "norm":
+        ins = [rand(gen, 6, 40, kind=torch.float32), rand(gen, 40, kind=torch.float32), rand(gen, 40, kind=torch.float32)]
+        dy = rand(gen, 6, 40, kind=torch.float32)
+        value = lambda a: (plain_norm(*a, 1e-5, dy)[0] * dy).sum()
+        leaves = [on(t, torch.float32, True) for t in ins]
+        out = (sequence.layer_norm(*leaves) * on(dy, torch.float32)).sum()
+    else:
+        reset, lengths = flags(gen, 3, 11, "padded")
+        dy = rand(gen, 3, 11, 21, kind=torch.float32)
+        if which == "conv":
+            ins = [rand(gen, 3, 11, 21, kind=torch.float32), rand(gen, 21, 4, kind=torch.float32), rand(gen, 21, kind=torch.float32), rand(gen, 3, 3, 21, kind=torch.float32)]
+            f, plain = (lambda a: sequence.causal_conv(*a[:3], state=a[3], reset=on(reset), lengths=on(lengths))), plain_conv
+        else:
+            ins = list(scan_inputs(gen, 3, 11, 21, 6, torch.float32))
+            f, plain = (lambda a: sequence.selective_scan(*a[:8], state=a[8], reset=on(reset), lengths=on(lengths))), plain_scan
+        dl = rand(gen, *ins[-1].shape, kind=torch.float32)
+
+        def value(a):
+            y, last = plain(*a, reset, lengths, dy, dl)[:2]
+            return (y * dy).sum() + (last * dl).sum()
+        leaves = [on(t, torch.float32, True) for t in ins]
+        y, last = f(leaves)
+        out = (y * on(dy, torch.float32)).sum() + (last * on(dl, torch.float32)).sum()
+    grads = torch.autograd.grad(out, leaves)
+    for k, g in enumerate(grads):
+        way, h = rand(gen, *ins[k].shape), 1e-4
+        up, down = ([t + s * h * way if j == k else t for j, t in enumerate(ins)] for s in (1, -1))
+        want, got = float(value(up) - value(down)) / (2 * h), float((g.double().cpu() * way).sum())
+        scale = float((g.double().cpu() * way).abs().sum())
+        assert abs(got - want) <= 1e-3 * scale, (which, k, got, want, scale)
+
+
+@gpu
+def test_strides_give_the_same_values():
+    gen = seeded(9)
+    ins = scan_inputs(gen, 4, 35, 72, 16, torch.bfloat16)
+    reset = torch.rand((4, 35), generator=gen) < 0.1
+    u, dt, A, B, C, D, z, bias, state = (on(t, torch.bfloat16 if k in (0, 1, 3, 4, 6) else torch.float32) for k, t in enumerate(ins))
+    gr, w, b, held = on(reset), on(rand(gen, 72, 4), torch.float32), on(rand(gen, 72), torch.float32), on(rand(gen, 4, 3, 72), torch.bfloat16)
+
+    def time_major(t):
+        return t.transpose(0, 1).contiguous().transpose(0, 1)
+
+    both = torch.cat([u, z], -1)                     # halves of one projection
+    wide = torch.cat([B, C], -1)
+    one = sequence.selective_scan(u, dt, A, B, C, D, z, bias, state=state, reset=gr)
+    other = sequence.selective_scan(time_major(both)[..., :72], time_major(dt), A.t().contiguous().t(), time_major(wide)[..., :16], wide[..., 16:], D, both[..., 72:], bias, state=state.transpose(1, 2).contiguous().transpose(1, 2),
+                                    reset=time_major(gr).to(torch.uint8))
+    assert torch.equal(one[0], other[0]) and torch.equal(one[1], other[1])
+    one = sequence.causal_conv(u, w, b, state=held, reset=gr)
+    other = sequence.causal_conv(time_major(both)[..., :72], w.t().contiguous().t(), b, state=time_major(held), reset=time_major(gr))
+    assert torch.equal(one[0], other[0]) and torch.equal(one[1], other[1])
+    turned = u.transpose(1, 2).contiguous().transpose(1, 2)          # the channels not contiguous
+    assert torch.equal(sequence.causal_conv(turned, w, b, state=held, reset=gr)[0], one[0])
+
+
+@gpu
+def test_rows_and_tokens_of_none():
+    gen = seeded(2)
+    u, dt, A, B, C, D, z, bias, state = (on(t, torch.float32, True) for t in scan_inputs(gen, 3, 4, 10, 16, torch.float32))
+    empty = lambda t: t[:, :0]
+    y, last = sequence.selective_scan(empty(u), empty(dt), A, empty(B), empty(C), D, empty(z), bias, state=state)
+    assert y.shape == (3, 0, 10) and torch.equal(last, state)
+    dl = torch.randn_like(last)
+    dA, ds = torch.autograd.grad((y, last), (A, state), (torch.zeros_like(y), dl))
+    assert torch.equal(dA, torch.zeros_like(A)) and torch.equal(ds, dl)
+    y, last = sequence.selective_scan(u[:0], dt[:0], A, B[:0], C[:0], D, z[:0], bias)
+    assert y.shape == (0, 4, 10) and last.shape == (0, 10, 16)
+    assert torch.equal(torch.autograd.grad(y.sum(), A)[0], torch.zeros_like(A))
+    w, held = torch.randn(10, 4, device="cuda", requires_grad=True), torch.randn(3, 3, 10, device="cuda", requires_grad=True)
+    y, last = sequence.causal_conv(empty(u), w, state=held)
+    assert y.shape == (3, 0, 10) and torch.equal(last, held)
+    dl = torch.randn_like(last)
+    dw, ds = torch.autograd.grad((y, last), (w, held), (torch.zeros_like(y), dl))
+    assert torch.equal(dw, torch.zeros_like(w)) and torch.equal(ds, dl)
+    y, last = sequence.causal_conv(u[:0], w)
+    assert y.shape == (0, 4, 10) and last.shape == (0, 3, 10)
+    with torch.no_grad():
+        assert sequence.causal_conv_step(u[:0, 0], w, state=held[:0]).shape == (0, 10)
+        assert sequence.selective_scan_step(u[:0, 0], dt[:0, 0], A, B[:0, 0], C[:0, 0], state=state[:0]).shape == (0, 10)
+
+
+@gpu
+def test_nothing_passes_an_episodes_beginning():
+    """an initial state, and tokens before a beginning, of NaN and infinities: not seen behind it; their gradients are zero"""
+    gen = seeded(8)
+    u, dt, A, B, C, D, z, bias, state = (on(t, torch.float32) for t in scan_inputs(gen, 2, 45, 40, 16, torch.float32))
+    reset = torch.zeros(2, 45, dtype=torch.bool, device="cuda")
+    reset[:, 0] = reset[1, 36] = True
+    state[0], state[1] = float("nan"), float("inf")
+    state.requires_grad_()
+    y, last = sequence.selective_scan(u, dt, A, B, C, D, z, bias, state=state, reset=reset)
+    assert torch.isfinite(y).all() and torch.isfinite(last).all()
+    assert torch.equal(torch.autograd.grad(y.sum() + last.sum(), state)[0], torch.zeros_like(state))
+    bad = u.clone()
+    bad[1, 35] = float("nan")
+    y2, last2 = sequence.selective_scan(bad, dt, A, B, C, D, z, bias, state=state.detach(), reset=reset)
+    assert torch.equal(y2[1, 36:], y[1, 36:]) and torch.equal(last2, last) and torch.equal(y2[0], y[0]) and torch.isnan(y2[1, 35]).all()
+    w = torch.randn(40, 4, device="cuda")
+    held = torch.full((2, 3, 40), float("nan"), device="cuda")
+    y, last = sequence.causal_conv(u, w, state=held, reset=reset)
+    assert torch.isfinite(y).all() and torch.isfinite(last).all()
+    y2, _ = sequence.causal_conv(bad, w, state=held, reset=reset)
+    assert torch.equal(y2[1, 36:], y[1, 36:])
+    with torch.no_grad():
+        gone = reset[:, 0].clone()
+        h = state.detach().clone()
+        assert torch.isfinite(sequence.selective_scan_step(u[:, 0], dt[:, 0], A, B[:, 0], C[:, 0], D, z[:, 0], bias, state=h, reset=gone)).all() and torch.isfinite(h).all()
+        assert torch.isfinite(sequence.causal_conv_step(u[:, 0], w, state=held, reset=gone)).all() and torch.isfinite(held).all()
+
+
+@gpu
+def test_lengths_out_of_range_are_taken_into_it():
+    gen = seeded(4)
+    u, dt, A, B, C, D, z, bias, state = (on(t, torch.float32) for t in scan_inputs(gen, 2, 40, 20, 8, torch.float32))
+    w = torch.randn(20, 3, device="cuda")
+    far, near = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([-5, 1 << 30], [0, 40]))
+    for f in (lambda n: sequence.selective_scan(u, dt, A, B, C, D, z, bias, state=state, lengths=n), lambda n: sequence.causal_conv(u, w, lengths=n)):
+        assert all(torch.equal(a, b) for a, b in zip(f(far), f(near)))
+
+
+@gpu
+def test_another_stream():
+    gen = seeded(6)
+    x = on(rand(gen, 300, 200), torch.float32)
+    want = sequence.layer_norm(x)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = sequence.layer_norm(x * 1.0)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+
+
+def layer(p, x, reset, conv_state, scan_state):
+    """one layer of a policy with memory, as recurrent_policy has it"""
+    n = sequence.layer_norm(x, p["w"], p["b"])
+    v, z = (n @ p["in"]).chunk(2, -1)
+    v, conv_state = sequence.causal_conv(v, p["cw"], p["cb"], state=conv_state, reset=reset)
+    B, C, dt = (v @ p["sel"]).split([16, 16, 48], -1)
+    y, scan_state = sequence.selective_scan(v, dt, p["A"], B, C, p["D"], z, p["dtb"], state=scan_state, reset=reset)
+    return x + y @ p["out"], conv_state, scan_state
+
+
+def layer_parts(gen):
+    f = lambda *s, scale=1.0: on(rand(gen, *s, scale=scale, kind=torch.float32), torch.float32)
+    p = {"w": 1 + f(32, scale=0.1), "b": f(32, scale=0.1), "in": f(32, 96, scale=0.2), "cw": f(48, 4, scale=0.5), "cb": f(48, scale=0.1), "sel": f(48, 80, scale=0.15),
+         "A": -torch.rand(48, 16, generator=torch.Generator().manual_seed(1)).cuda() * 3 - 0.1, "D": f(48), "dtb": f(48) - 2, "out": f(48, 32, scale=0.15)}
+    x = f(5, 21, 32)
+    reset = on(torch.rand((5, 21), generator=gen) < 0.15)
+    return p, x, reset, f(5, 3, 48), f(5, 48, 16)
+
+
+@gpu
+def test_a_layer_in_one_pass_in_two_and_token_by_token():
+    gen = seeded(77)
+    p, x, reset, cs, ss = layer_parts(gen)
+    whole, c1, s1 = layer(p, x, reset, cs, ss)
+    first, c2, s2 = layer(p, x[:, :13], reset[:, :13], cs, ss)
+    second, c2, s2 = layer(p, x[:, 13:], reset[:, 13:], c2, s2)
+    close_ = dict(rtol=1e-4, atol=1e-4)             # the matrix products of torch differ by their shapes: 96 sums of order one, in float32
+    assert torch.allclose(torch.cat([first, second], 1), whole, **close_) and torch.allclose(c2, c1, **close_) and torch.allclose(s2, s1, **close_)
+    c3, s3, steps = cs.clone(), ss.clone(), []
+    with torch.no_grad():
+        for t in range(21):
+            n = sequence.layer_norm(x[:, t], p["w"], p["b"])
+            v, z = (n @ p["in"]).chunk(2, -1)
+            v = sequence.causal_conv_step(v, p["cw"], p["cb"], state=c3, reset=reset[:, t])
+            B, C, dt = (v @ p["sel"]).split([16, 16, 48], -1)
+            steps.append(x[:, t] + sequence.selective_scan_step(v, dt, p["A"], B, C, p["D"], z, p["dtb"], state=s3, reset=reset[:, t]) @ p["out"])
+    assert torch.allclose(torch.stack(steps, 1), whole, **close_) and torch.allclose(c3, c1, **close_) and torch.allclose(s3, s1, **close_)
+
+
+@gpu
+def test_a_layers_forward_and_backward_pass_in_a_graph():
+    """replayed several times with eager work between, on new inputs, and two graphs one after the other"""
+    gen = seeded(78)
+    p, x, reset, cs, ss = layer_parts(gen)
+    leaves = [t.requires_grad_() for t in p.values()]
+
+    def once():
+        y, c, s = layer(p, x, reset, cs, ss)
+        grads = torch.autograd.grad(y.square().sum() + s.square().sum(), leaves)
+        return [t.detach() for t in (y, c, s, *grads)]          # no autograd graph of these leaves outlives the call: a capture must not meet one
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            once()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = once()
+        graphs.append((g, out))
+    for k in range(4):
+        with torch.no_grad():
+            x.copy_(torch.randn_like(x))
+        want = [t.clone() for t in once()]
+        torch.cuda.synchronize()
+        for g, out in graphs:
+            g.replay()
+            junk = torch.randn(1 << 20, device="cuda").sum()          # eager work of the program's own
+            torch.cuda.synchronize()
+            for a, b in zip(out, want):
+                # torch's own products may take another kernel in the graph; float32 sums of under a thousand terms
+                assert torch.allclose(a, b, rtol=2e-3, atol=2e-3 * float(b.abs().max())), k
+        del want, junk
+
+
+@gpu
+def test_results_do_not_vary():
+    gen = seeded(12)
+    ins = [on(t, torch.float32, True) for t in scan_inputs(gen, 9, 100, 200, 16, torch.float32)]
+    runs = []
+    for _ in range(3):
+        y, last = sequence.selective_scan(*ins[:8], state=ins[8])
+        runs.append((y, last, *torch.autograd.grad(y.square().sum(), ins)))
+    for r in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(r, runs[0]))
+
+
+# ---- refusals: on the host, before anything reaches a GPU ----
+def conv_case(**change):
+    a = dict(x=torch.zeros(2, 5, 6), weight=torch.zeros(6, 4), bias=torch.zeros(6), state=torch.zeros(2, 3, 6), reset=torch.zeros(2, 5, dtype=torch.bool), lengths=torch.zeros(2, dtype=torch.int32))
+    a.update(change)
+    return a
+
+
+def scan_case(**change):
+    a = dict(u=torch.zeros(2, 5, 6), dt=torch.zeros(2, 5, 6), A=torch.zeros(6, 3), B=torch.zeros(2, 5, 3), C=torch.zeros(2, 5, 3), D=torch.zeros(6), z=torch.zeros(2, 5, 6), dt_bias=torch.zeros(6),
+             state=torch.zeros(2, 6, 3), reset=torch.zeros(2, 5, dtype=torch.bool), lengths=torch.zeros(2, dtype=torch.int32))
+    a.update(change)
+    return a
+
+
+def step_case(**change):
+    a = dict(u=torch.zeros(2, 6), dt=torch.zeros(2, 6), A=torch.zeros(6, 3), B=torch.zeros(2, 3), C=torch.zeros(2, 3), D=torch.zeros(6), z=torch.zeros(2, 6), dt_bias=torch.zeros(6), state=torch.zeros(2, 6, 3))
+    a.update(change)
+    return a
+
+
+@pytest.mark.parametrize("call,error,says", [
+    (lambda: sequence.layer_norm([1.0]), TypeError, "tensor"),
+    (lambda: sequence.layer_norm(torch.zeros(2, 3, dtype=torch.float64)), TypeError, "float64"),
+    (lambda: sequence.layer_norm(torch.zeros(())), ValueError, "dimension"),
+    (lambda: sequence.layer_norm(torch.zeros(2, 0)), ValueError, "channels"),
+    (lambda: sequence.layer_norm(torch.zeros(1, 16385)), ValueError, "16384"),
+    (lambda: sequence.layer_norm(torch.zeros(2, 3), torch.zeros(4)), ValueError, "weight has shape"),
+    (lambda: sequence.layer_norm(torch.zeros(2, 3), torch.zeros(3, dtype=torch.float16)), TypeError, "weight"),
+    (lambda: sequence.layer_norm(torch.zeros(2, 3, dtype=torch.float16), torch.zeros(3), torch.zeros(3, dtype=torch.float16)), TypeError, "one type"),
+    (lambda: sequence.layer_norm(torch.zeros(2, 3), eps=-1.0), ValueError, "eps"),
+    (lambda: sequence.layer_norm(torch.zeros(2, 3), eps=float("nan")), ValueError, "eps"),
+    (lambda: sequence.layer_norm(torch.zeros(2, 3)), ValueError, "no CPU fallback"),
+    (lambda: sequence.causal_conv(**conv_case()), ValueError, "no CPU fallback"),
+    (lambda: sequence.causal_conv(**conv_case(x=torch.zeros(5, 6))), ValueError, "dimensions"),
+    (lambda: sequence.causal_conv(**conv_case(x=torch.zeros(2, 5, 6, dtype=torch.int32))), TypeError, "int32"),
+    (lambda: sequence.causal_conv(**conv_case(weight=torch.zeros(6, 5))), ValueError, "taps"),
+    (lambda: sequence.causal_conv(**conv_case(weight=torch.zeros(6, 1))), ValueError, "taps"),
+    (lambda: sequence.causal_conv(**conv_case(weight=torch.zeros(7, 4))), ValueError, "weight"),
+    (lambda: sequence.causal_conv(**conv_case(bias=torch.zeros(6, dtype=torch.float16))), TypeError, "bias"),
+    (lambda: sequence.causal_conv(**conv_case(state=torch.zeros(2, 4, 6))), ValueError, "state"),
+    (lambda: sequence.causal_conv(**conv_case(state=torch.zeros(2, 3, 6, dtype=torch.float16))), TypeError, "state"),
+    (lambda: sequence.causal_conv(**conv_case(reset=torch.zeros(2, 4, dtype=torch.bool))), ValueError, "reset"),
+    (lambda: sequence.causal_conv(**conv_case(reset=torch.zeros(2, 5))), TypeError, "reset"),
+    (lambda: sequence.causal_conv(**conv_case(lengths=torch.zeros(2, dtype=torch.int64))), TypeError, "lengths"),
+    (lambda: sequence.causal_conv(**conv_case(lengths=torch.zeros(3, dtype=torch.int32))), ValueError, "lengths"),
+    (lambda: sequence.causal_conv_step(torch.zeros(2, 6), torch.zeros(6, 4), state=None), TypeError, "state"),
+    (lambda: sequence.causal_conv_step(torch.zeros(2, 6), torch.zeros(6, 4), state=torch.zeros(2, 6, 3).transpose(1, 2)), ValueError, "contiguous"),
+    (lambda: sequence.causal_conv_step(torch.zeros(2, 6), torch.zeros(6, 4), state=torch.zeros(2, 3, 6)), ValueError, "no CPU fallback"),
+    (lambda: sequence.causal_conv_step(torch.zeros(2, 6), torch.zeros(6, 4), state=torch.zeros(2, 3, 6), reset=torch.zeros(2, 1, dtype=torch.bool)), ValueError, "reset"),
+    (lambda: sequence.selective_scan(**scan_case()), ValueError, "no CPU fallback"),
+    (lambda: sequence.selective_scan(**scan_case(u=torch.zeros(2, 6))), ValueError, "dimensions"),
+    (lambda: sequence.selective_scan(**scan_case(dt=torch.zeros(2, 5, 5))), ValueError, "dt"),
+    (lambda: sequence.selective_scan(**scan_case(dt=torch.zeros(2, 5, 6, dtype=torch.float16))), TypeError, "dt"),
+    (lambda: sequence.selective_scan(**scan_case(A=torch.zeros(6, 33))), ValueError, "states"),
+    (lambda: sequence.selective_scan(**scan_case(A=torch.zeros(6, 0), B=torch.zeros(2, 5, 0), C=torch.zeros(2, 5, 0))), ValueError, "states"),
+    (lambda: sequence.selective_scan(**scan_case(A=torch.zeros(6, 3, dtype=torch.float16))), TypeError, "A is"),
+    (lambda: sequence.selective_scan(**scan_case(B=torch.zeros(2, 5, 4))), ValueError, "B has"),
+    (lambda: sequence.selective_scan(**scan_case(C=torch.zeros(2, 4, 3))), ValueError, "C has"),
+    (lambda: sequence.selective_scan(**scan_case(D=torch.zeros(5))), ValueError, "D has"),
+    (lambda: sequence.selective_scan(**scan_case(dt_bias=torch.zeros(6, dtype=torch.bfloat16))), TypeError, "dt_bias"),
+    (lambda: sequence.selective_scan(**scan_case(state=torch.zeros(2, 3, 6))), ValueError, "state"),
+    (lambda: sequence.selective_scan(**scan_case(z=torch.zeros(2, 5, 6, device="meta"))), ValueError, "meta"),
+    (lambda: sequence.selective_scan_step(**step_case()), ValueError, "no CPU fallback"),
+    (lambda: sequence.selective_scan_step(**step_case(state=torch.zeros(2, 6, 6)[:, :, :3])), ValueError, "contiguous"),
+    (lambda: sequence.selective_scan_step(**step_case(state=torch.zeros(2, 6, 3, dtype=torch.float16))), TypeError, "state"),
+    (lambda: sequence.selective_scan_step(**step_case(B=torch.zeros(3, 3))), ValueError, "B has"),
+])
+def test_refusals(call, error, says):
+    with pytest.raises(error, match=says):
+        call()
+
+
+def test_the_library_refuses_what_a_binding_may_get_wrong():
+    """mws_* themselves, without a GPU: bad structs come back as negative codes with a message, before any HIP call"""
+    lib = sequence.load()
+    for f in (lib.mws_norm_forward, lib.mws_norm_backward, lib.mws_conv_forward, lib.mws_conv_backward, lib.mws_conv_step, lib.mws_scan_forward, lib.mws_scan_backward, lib.mws_scan_step):
+        assert f(None, None) == -1 and "no arguments" in lib.mws_last_error().decode()
+
+    def norm(rows=1, width=4, kind=0, par=0, x=0, eps=1e-5, space=0):
+        return sequence._NORM.pack(x, 0, 0, 0, 0, 0, 0, 0, 0, rows, 4, 4, space, width, kind, par, eps)
+    for args, text in ((norm(kind=3), "type"), (norm(par=1), "parameters"), (norm(rows=-1), "rows"), (norm(width=0), "width"), (norm(width=16385), "width"), (norm(eps=float("nan")), "eps"),
+                       (norm(), "x is NULL"), (norm(x=64), "y is NULL")):
+        assert lib.mws_norm_forward(args, None) == -1 and text in lib.mws_last_error().decode()
+    assert lib.mws_norm_forward(norm(rows=0), None) == 0
+    assert lib.mws_norm_backward(norm(x=64), None) == -1 and "dy" in lib.mws_last_error().decode()
+    need = sequence._NORM.pack(64, 0, 0, 64, 0, 0, 64, 0, 0, 1, 4, 4, 0, 4, 0, 0, 1e-5)
+    assert lib.mws_norm_workspace(need) > 0 and lib.mws_norm_backward(need, None) == -1 and "workspace" in lib.mws_last_error().decode()
+
+    def conv(batch=1, length=1, width=4, taps=4, kind=0, x=64, weight=64):
+        return sequence._CONV.pack(x, weight, *[0] * 13, batch, length, *[0] * 7, width, taps, kind, 0)
+    for args, text in ((conv(taps=5), "taps"), (conv(taps=1), "taps"), (conv(kind=-1), "type"), (conv(width=0), "width"), (conv(length=-1), "rows"), (conv(batch=1 << 20, length=1 << 20), "rows"),
+                       (conv(weight=0), "weight"), (conv(x=0), "x is NULL"), (conv(), "y is NULL")):
+        assert lib.mws_conv_forward(args, None) == -1 and text in lib.mws_last_error().decode()
+    assert lib.mws_conv_step(conv(length=2), None) == -1 and "one token" in lib.mws_last_error().decode()
+
+    def scan(batch=1, length=1, width=4, states=16, kind=0, u=64, A=64, space=0):
+        p = [u, u, 0, u, u, 0, A] + [0] * 19
+        return sequence._SCAN.pack(*p, batch, length, *[0] * 14, space, width, states, kind, 0)
+    for args, text in ((scan(states=33), "states"), (scan(states=0), "states"), (scan(kind=9), "type"), (scan(width=-1), "width"), (scan(batch=-1), "rows"), (scan(A=0), "A is NULL"),
+                       (scan(u=0), "NULL"), (scan(), "y is NULL")):
+        assert lib.mws_scan_forward(args, None) == -1 and text in lib.mws_last_error().decode()
+    assert lib.mws_scan_step(scan(length=3), None) == -1 and "one token" in lib.mws_last_error().decode()
+    assert lib.mws_scan_workspace(scan(batch=2, length=7), 0) >= 2 * 7 * 32 * 4 and lib.mws_scan_kept(scan(batch=2, length=33)) == 2 * 2 * 16 * 4
+    assert lib.mws_sizeof(0) == sequence._NORM.size and lib.mws_sizeof(3) == -1
+
+
+def test_without_the_library_it_says_how_to_build_it(monkeypatch, tmp_path):
+    monkeypatch.setattr(sequence, "_lib", None)
+    monkeypatch.setattr(sequence, "LIB_PATH", str(tmp_path / "libmwseq.so"))
+    with pytest.raises(RuntimeError, match="build"):
+        sequence.load()
