@@ -6,6 +6,8 @@ operation is off by at most 2^-24 relative to its operands' magnitude (the hardw
 an output with n operations on its longest path is off by at most n 2^-24 times its MAGNITUDE, the same sum with every term's absolute
 value, which the plain implementations compute as well.  n is counted beside each test.
 """
+import struct
+
 import numpy as np
 import pytest
 import torch
@@ -13,6 +15,8 @@ import torch
 from metaworld_amd import sequence
 
 gpu = pytest.mark.gpu
+# the argument structs of include/mwseq.h, field by field
+NORM, CONV, SCAN = struct.Struct("@9Q4q3if"), struct.Struct("@15Q9q4i"), struct.Struct("@26Q17q4i")
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 U = 2.0 ** -24
 
@@ -587,6 +591,24 @@ def test_a_layers_forward_and_backward_pass_in_a_graph():
 
 
 @gpu
+def test_what_autograd_refuses():
+    x, w = torch.randn(2, 5, 8, device="cuda", requires_grad=True), torch.randn(8, 4, device="cuda", requires_grad=True)
+    for y in (sequence.layer_norm(x), sequence.causal_conv(x, w)[0], sequence.selective_scan(x, x, -torch.ones(8, 4, device="cuda"), x[..., :4], x[..., :4])[0]):
+        with pytest.raises(RuntimeError, match="once differentiable"):
+            torch.autograd.grad(y.sum(), x, create_graph=True)
+    flags_ = torch.zeros(2, 5, dtype=torch.bool, device="cuda")
+    y, _ = sequence.causal_conv(x, w, reset=flags_)
+    flags_.fill_(True)                       # an input of the backward pass changed in between
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y.sum(), x)
+    held = torch.zeros(2, 3, 8, device="cuda")
+    with pytest.raises(RuntimeError, match="no_grad"):
+        sequence.causal_conv_step(x[:, 0], w, state=held)
+    with pytest.raises(RuntimeError, match="no_grad"):
+        sequence.selective_scan_step(x[:, 0], x[:, 0], -torch.ones(8, 4, device="cuda"), x[:, 0, :4], x[:, 0, :4], state=torch.zeros(2, 8, 4, device="cuda"))
+
+
+@gpu
 def test_results_do_not_vary():
     gen = seeded(12)
     ins = [on(t, torch.float32, True) for t in scan_inputs(gen, 9, 100, 200, 16, torch.float32)]
@@ -619,8 +641,8 @@ def step_case(**change):
 
 
 @pytest.mark.parametrize("call,error,says", [
-    (lambda: sequence.layer_norm([1.0]), TypeError, "tensor"),
-    (lambda: sequence.layer_norm(torch.zeros(2, 3, dtype=torch.float64)), TypeError, "float64"),
+    (lambda: sequence.layer_norm([1.0]), TypeError, "Tensor"),
+    (lambda: sequence.layer_norm(torch.zeros(2, 3, dtype=torch.float64)), TypeError, "Double"),
     (lambda: sequence.layer_norm(torch.zeros(())), ValueError, "dimension"),
     (lambda: sequence.layer_norm(torch.zeros(2, 0)), ValueError, "channels"),
     (lambda: sequence.layer_norm(torch.zeros(1, 16385)), ValueError, "16384"),
@@ -632,7 +654,7 @@ def step_case(**change):
     (lambda: sequence.layer_norm(torch.zeros(2, 3)), ValueError, "no CPU fallback"),
     (lambda: sequence.causal_conv(**conv_case()), ValueError, "no CPU fallback"),
     (lambda: sequence.causal_conv(**conv_case(x=torch.zeros(5, 6))), ValueError, "dimensions"),
-    (lambda: sequence.causal_conv(**conv_case(x=torch.zeros(2, 5, 6, dtype=torch.int32))), TypeError, "int32"),
+    (lambda: sequence.causal_conv(**conv_case(x=torch.zeros(2, 5, 6, dtype=torch.int32))), TypeError, "Int"),
     (lambda: sequence.causal_conv(**conv_case(weight=torch.zeros(6, 5))), ValueError, "taps"),
     (lambda: sequence.causal_conv(**conv_case(weight=torch.zeros(6, 1))), ValueError, "taps"),
     (lambda: sequence.causal_conv(**conv_case(weight=torch.zeros(7, 4))), ValueError, "weight"),
@@ -672,22 +694,22 @@ def test_refusals(call, error, says):
 
 def test_the_library_refuses_what_a_binding_may_get_wrong():
     """mws_* themselves, without a GPU: bad structs come back as negative codes with a message, before any HIP call"""
-    lib = sequence.load()
+    lib = sequence.library()
     for f in (lib.mws_norm_forward, lib.mws_norm_backward, lib.mws_conv_forward, lib.mws_conv_backward, lib.mws_conv_step, lib.mws_scan_forward, lib.mws_scan_backward, lib.mws_scan_step):
         assert f(None, None) == -1 and "no arguments" in lib.mws_last_error().decode()
 
     def norm(rows=1, width=4, kind=0, par=0, x=0, eps=1e-5, space=0):
-        return sequence._NORM.pack(x, 0, 0, 0, 0, 0, 0, 0, 0, rows, 4, 4, space, width, kind, par, eps)
+        return NORM.pack(x, 0, 0, 0, 0, 0, 0, 0, 0, rows, 4, 4, space, width, kind, par, eps)
     for args, text in ((norm(kind=3), "type"), (norm(par=1), "parameters"), (norm(rows=-1), "rows"), (norm(width=0), "width"), (norm(width=16385), "width"), (norm(eps=float("nan")), "eps"),
                        (norm(), "x is NULL"), (norm(x=64), "y is NULL")):
         assert lib.mws_norm_forward(args, None) == -1 and text in lib.mws_last_error().decode()
     assert lib.mws_norm_forward(norm(rows=0), None) == 0
     assert lib.mws_norm_backward(norm(x=64), None) == -1 and "dy" in lib.mws_last_error().decode()
-    need = sequence._NORM.pack(64, 0, 0, 64, 0, 0, 64, 0, 0, 1, 4, 4, 0, 4, 0, 0, 1e-5)
+    need = NORM.pack(64, 0, 0, 64, 0, 0, 64, 0, 0, 1, 4, 4, 0, 4, 0, 0, 1e-5)
     assert lib.mws_norm_workspace(need) > 0 and lib.mws_norm_backward(need, None) == -1 and "workspace" in lib.mws_last_error().decode()
 
     def conv(batch=1, length=1, width=4, taps=4, kind=0, x=64, weight=64):
-        return sequence._CONV.pack(x, weight, *[0] * 13, batch, length, *[0] * 7, width, taps, kind, 0)
+        return CONV.pack(x, weight, *[0] * 13, batch, length, *[0] * 7, width, taps, kind, 0)
     for args, text in ((conv(taps=5), "taps"), (conv(taps=1), "taps"), (conv(kind=-1), "type"), (conv(width=0), "width"), (conv(length=-1), "rows"), (conv(batch=1 << 20, length=1 << 20), "rows"),
                        (conv(weight=0), "weight"), (conv(x=0), "x is NULL"), (conv(), "y is NULL")):
         assert lib.mws_conv_forward(args, None) == -1 and text in lib.mws_last_error().decode()
@@ -695,17 +717,18 @@ def test_the_library_refuses_what_a_binding_may_get_wrong():
 
     def scan(batch=1, length=1, width=4, states=16, kind=0, u=64, A=64, space=0):
         p = [u, u, 0, u, u, 0, A] + [0] * 19
-        return sequence._SCAN.pack(*p, batch, length, *[0] * 14, space, width, states, kind, 0)
+        return SCAN.pack(*p, batch, length, *[0] * 14, space, width, states, kind, 0)
     for args, text in ((scan(states=33), "states"), (scan(states=0), "states"), (scan(kind=9), "type"), (scan(width=-1), "width"), (scan(batch=-1), "rows"), (scan(A=0), "A is NULL"),
                        (scan(u=0), "NULL"), (scan(), "y is NULL")):
         assert lib.mws_scan_forward(args, None) == -1 and text in lib.mws_last_error().decode()
     assert lib.mws_scan_step(scan(length=3), None) == -1 and "one token" in lib.mws_last_error().decode()
     assert lib.mws_scan_workspace(scan(batch=2, length=7), 0) >= 2 * 7 * 32 * 4 and lib.mws_scan_kept(scan(batch=2, length=33)) == 2 * 2 * 16 * 4
-    assert lib.mws_sizeof(0) == sequence._NORM.size and lib.mws_sizeof(3) == -1
+    assert lib.mws_sizeof(0) == NORM.size and lib.mws_sizeof(3) == -1
 
 
 def test_without_the_library_it_says_how_to_build_it(monkeypatch, tmp_path):
-    monkeypatch.setattr(sequence, "_lib", None)
+    monkeypatch.setattr(sequence, "_binding", None)
     monkeypatch.setattr(sequence, "LIB_PATH", str(tmp_path / "libmwseq.so"))
-    with pytest.raises(RuntimeError, match="build"):
-        sequence.load()
+    for call in (sequence.library, lambda: sequence.layer_norm(torch.zeros(2, 3))):
+        with pytest.raises(RuntimeError, match="build"):
+            call()
