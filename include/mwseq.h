@@ -31,6 +31,7 @@ enum { MWS_ARGUMENT = -1, MWS_LAUNCH = -2 };
 #define MWS_CONV_MIN_TAPS 2
 #define MWS_CONV_MAX_TAPS 4
 #define MWS_SCAN_MAX_STATES 32
+#define MWS_SCAN_MAX_STRIDE (1 << 26)   /* from one token to the next of u, dt, z and dy, in values */
 
 /* y = (x - mean) / sqrt(var + eps) * weight + bias over rows of `width`; weight and bias may be NULL */
 typedef struct mws_norm_args {

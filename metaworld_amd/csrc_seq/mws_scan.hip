@@ -15,13 +15,16 @@
 // Where batch x channels leave the card empty, the time axis is cut into segments of whole chunks: scan_segment takes each
 // segment's end state from zero and its sum of d (the product of its a is exp(A sum d)), scan_join runs over the segments, and the
 // scan itself starts every segment from its joined state.  The same holds for g, from the end.
+#include <type_traits>
 #include "mws_common.hpp"
 
 namespace mws {
 
-// Tokens between two states kept for the backward pass; segments are whole chunks.  And a block's channels at most: the backward
-// pass keeps the states inside a chunk in shared memory, 64 KB for a block at most.
-constexpr int chunk_of(int ns) { return ns >= 32 ? 16 : 32; }
+// Tokens are walked in groups of kGroup, whose episodes' beginnings are one mask; segments are whole groups.  kept_of: tokens between
+// two states kept for the backward pass; sub_of: tokens that the backward pass holds in registers at a time (states x tokens = 128
+// registers).  lanes_of: a block's channels at most.
+constexpr int kGroup = 32;
+constexpr int kept_of(int ns) { return ns >= 32 ? 16 : 8; }
 constexpr int sub_of(int ns) { return ns >= 32 ? 4 : 8; }
 constexpr int lanes_of(int ns) { return ns >= 32 ? 128 : 256; }
 
@@ -41,6 +44,28 @@ struct ScanArgs {
     int width, states, across, segments, span, groups;            // across: blocks over the channels; span: tokens of a segment
 };
 
+// The channels of a token and of the seven after it as a buffer: the tokens' address is scalar, a lane adds its channel's bytes.  A
+// lane past the channels adds kOutside instead: with that it reads zeros and writes nothing, without a branch, as does every lane
+// of a tensor that is not there.  (Eight tokens and the channels end below kBytes: MWS_SCAN_MAX_STRIDE.)
+constexpr uint32_t kBytes = 0x80000000u, kOutside = 0xC0000000u;
+template <class R> struct Line {
+    __amdgpu_buffer_rsrc_t r;
+    uint32_t stride;
+    __device__ __forceinline__ Line(const R *p, int64_t from, int64_t step)
+        : r(__builtin_amdgcn_make_buffer_rsrc((void *)(p != nullptr ? p + from : p), 0, (int)(p != nullptr ? kBytes : 0), 0x00020000)), stride((uint32_t)step * (uint32_t)sizeof(R)) {}
+    __device__ __forceinline__ R get(uint32_t bytes, int token = 0) const {
+        if constexpr (sizeof(R) == 2) return (R)__builtin_amdgcn_raw_buffer_load_b16(r, bytes, token * stride, 0);
+        else {
+            unsigned v = __builtin_amdgcn_raw_buffer_load_b32(r, bytes, token * stride, 0);
+            return __builtin_bit_cast(R, v);
+        }
+    }
+    __device__ __forceinline__ void put(R v, uint32_t bytes, int token = 0) const {
+        if constexpr (sizeof(R) == 2) __builtin_amdgcn_raw_buffer_store_b16(v, r, bytes, token * stride, 0);
+        else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), r, bytes, token * stride, 0);
+    }
+};
+
 __device__ __forceinline__ int64_t row_length(const int32_t *lengths, int64_t b, int64_t length) {
     if (lengths == nullptr) return length;
     int64_t n = lengths[b];
@@ -55,12 +80,12 @@ __device__ __forceinline__ float softplus_(float x) {
     return x > 20.0f ? x : r;
 }
 
-// bit i: an episode begins at token t0 + i of the chunk
-template <int CHUNK> __device__ __forceinline__ uint32_t chunk_mask(const ScanArgs &a, int64_t b, int64_t t0, int64_t end) {
+// bit i: an episode begins at token t0 + i of the group
+__device__ __forceinline__ uint32_t group_mask(const ScanArgs &a, int64_t b, int64_t t0, int64_t end) {
     if (a.reset == nullptr) return 0;
     int lane = threadIdx.x % kWave;
     int64_t t = t0 + lane;
-    return (uint32_t)__ballot(lane < CHUNK && t < end && a.reset[b * a.reset_batch + t * a.reset_time] != 0);
+    return (uint32_t)__ballot(lane < kGroup && t < end && a.reset[b * a.reset_batch + t * a.reset_time] != 0);
 }
 
 // ---- B and C in float, padded with zeros to NS states ----
@@ -108,11 +133,17 @@ template <int NS> __device__ __forceinline__ void put_row(float *p, int64_t row,
     for (int n = 0; n < NS; n++) (p + (row * NS + n) * a.width)[e] = h[n];
 }
 
+template <int NS> __device__ __forceinline__ void kept_row(const ScanArgs &a, int64_t row, uint32_t bytes, float (&h)[NS]) {
+#pragma unroll
+    for (int n = 0; n < NS; n++) h[n] = Line<float>(a.kept, (row * NS + n) * a.width, 0).get(bytes);
+}
+
 struct Place {          // what a block of the grid works on
     int64_t b, t0, t1, end;
     uint32_t e;
     int at, seg;
     bool on;
+    __device__ __forceinline__ uint32_t bytes(int size) const { return on ? (uint32_t)at * (uint32_t)size : kOutside; }
     __device__ __forceinline__ Place(const ScanArgs &a, int64_t item, int part) {
         at = part * (int)blockDim.x + (int)threadIdx.x;
         on = at < a.width;
@@ -125,59 +156,70 @@ struct Place {          // what a block of the grid works on
 
 template <class T, int NS> __global__ __launch_bounds__(256) void scan_forward(ScanArgs a) {
     using raw = typename T::raw;
-    constexpr int G = 4, kChunk = chunk_of(NS);
+    constexpr int G = 4;
     Place p(a, blockIdx.x / a.across, blockIdx.x % a.across);
     int64_t stop = p.t1 < p.end ? p.t1 : p.end;
-    raw *y = (raw *)a.y + p.b * a.length * a.width;
+    raw *y = (raw *)a.y + (p.b * a.length + p.t0) * a.width;
     bool whole_end = p.end <= p.t1 && (p.end > p.t0 || p.seg == 0);      // the row ends in this segment
+    const uint32_t bytes = p.bytes(sizeof(raw));
     if (p.t0 < stop || whole_end) {
         float h[NS], A2[NS];
         rates<NS>(a, p.e, A2);
         if (p.seg == 0) first_state<NS>(a.state, a, p.b, p.e, h);
         else get_row<NS>(a.seg, p.b * a.segments + p.seg, a, p.e, h);
         float D = a.D != nullptr ? a.D[p.e] : 0.0f, bias = a.dt_bias != nullptr ? a.dt_bias[p.e] : 0.0f;
-        const raw *u = (const raw *)a.u + p.b * a.u_batch, *dt = (const raw *)a.dt + p.b * a.dt_batch;
-        const raw *z = a.z != nullptr ? (const raw *)a.z + p.b * a.z_batch : nullptr;
-        Fixed *bc = fixed(a.bc + p.b * a.length * 2 * NS);
-        for (int64_t c0 = p.t0; c0 < stop; c0 += kChunk) {
-            uint32_t begins = chunk_mask<kChunk>(a, p.b, c0, p.end);
-            if (a.kept != nullptr && p.on) put_row<NS>(a.kept, p.b * a.chunks + c0 / kChunk, a, p.e, h);
-            int64_t c1 = c0 + kChunk < stop ? c0 + kChunk : stop;
-            for (int64_t t = c0; t < c1; t += G) {
-                raw ru[G], rd[G], rz[G];
+        const raw *u = (const raw *)a.u + p.b * a.u_batch + p.t0 * a.u_time, *dt = (const raw *)a.dt + p.b * a.dt_batch + p.t0 * a.dt_time;
+        const raw *z = a.z != nullptr ? (const raw *)a.z + p.b * a.z_batch + p.t0 * a.z_time : nullptr;
+        Fixed *bc = fixed(a.bc + (p.b * a.length + p.t0) * 2 * NS);
+        float *kept = a.kept != nullptr ? a.kept + (p.b * a.chunks + p.t0 / kept_of(NS)) * NS * a.width : nullptr;
+        auto token = [&](raw ru, raw rd, raw rz, bool first, const Line<raw> &out, int q) __attribute__((always_inline)) {
+            Pair<NS> m;
+            m.read(bc);
+            float uf = up<T>(ru), d = softplus_(up<T>(rd) + bias), du = d * uf, o = D * uf, o2 = 0;
+            if (first)
 #pragma unroll
-                for (int q = 0; q < G; q++) {
-                    int64_t at = t + q < c1 ? t + q : c1 - 1;
-                    ru[q] = (u + at * a.u_time)[p.e], rd[q] = (dt + at * a.dt_time)[p.e];
-                    if (z != nullptr) rz[q] = (z + at * a.z_time)[p.e];
+                for (int n = 0; n < NS; n++) h[n] = 0;
+#pragma unroll
+            for (int n = 0; n < NS; n++) {
+                h[n] = __builtin_fmaf(exp2_(d * A2[n]), h[n], du * m.B[n]);
+                if (n & 1) o2 = __builtin_fmaf(m.C[n], h[n], o2);
+                else o = __builtin_fmaf(m.C[n], h[n], o);
+            }
+            o += o2;
+            if (z != nullptr) {
+                float zf = up<T>(rz);
+                o *= zf * sigmoid_(zf);
+            }
+            out.put(down<T>(o), bytes, q);
+            bc += 2 * NS;
+            __builtin_amdgcn_sched_barrier(0);       // the next token's scalar loads do not fit beside this one's
+        };
+        for (int64_t c0 = p.t0; c0 < stop; c0 += kGroup) {
+            uint32_t begins = group_mask(a, p.b, c0, p.end);
+            int count = (int)(c0 + kGroup < stop ? kGroup : stop - c0);
+            for (int i = 0; i < count; i += G) {
+                if (kept != nullptr && i % kept_of(NS) == 0) {
+#pragma unroll
+                    for (int n = 0; n < NS; n++) Line<float>(kept, (int64_t)n * a.width, 0).put(h[n], p.bytes(4));
+                    kept += (int64_t)NS * a.width;
                 }
+                Line<raw> lu(u, 0, a.u_time), ld(dt, 0, a.dt_time), lz(z, 0, a.z_time), ly(y, 0, a.width);
+                if (i + G <= count) {
+                    raw ru[G], rd[G], rz[G];
 #pragma unroll
-                for (int q = 0; q < G; q++) {
-                    if (t + q >= c1) break;
-                    Pair<NS> m;
-                    m.read(bc + (t + q) * 2 * NS);
-                    float uf = up<T>(ru[q]), d = softplus_(up<T>(rd[q]) + bias), du = d * uf, o = D * uf, o2 = 0;
-                    if (begins >> q & 1)
+                    for (int q = 0; q < G; q++) ru[q] = lu.get(bytes, q), rd[q] = ld.get(bytes, q), rz[q] = lz.get(bytes, q);
 #pragma unroll
-                        for (int n = 0; n < NS; n++) h[n] = 0;
-#pragma unroll
-                    for (int n = 0; n < NS; n++) {
-                        h[n] = __builtin_fmaf(exp2_(d * A2[n]), h[n], du * m.B[n]);
-                        if (n & 1) o2 = __builtin_fmaf(m.C[n], h[n], o2);
-                        else o = __builtin_fmaf(m.C[n], h[n], o);
-                    }
-                    o += o2;
-                    if (z != nullptr) {
-                        float zf = up<T>(rz[q]);
-                        o *= zf * sigmoid_(zf);
-                    }
-                    if (p.on) (y + (t + q) * a.width)[p.e] = down<T>(o);
-                }
+                    for (int q = 0; q < G; q++) token(ru[q], rd[q], rz[q], begins >> q & 1, ly, q);
+                } else
+                    for (int q = 0; i + q < count; q++) token(lu.get(bytes, q), ld.get(bytes, q), lz.get(bytes, q), begins >> q & 1, ly, q);
                 begins >>= G;
+                u += G * a.u_time, dt += G * a.dt_time, y += G * (int64_t)a.width;
+                if (z != nullptr) z += G * a.z_time;
             }
         }
         if (a.last != nullptr && whole_end && p.on) last_state<NS>(a.last, a, p.b, p.e, h);
     }
+    y = (raw *)a.y + p.b * a.length * a.width;
     if (p.on)
         for (int64_t t = p.t0 > p.end ? p.t0 : p.end; t < p.t1; t++) (y + t * a.width)[p.e] = down<T>(0.0f);
 }
@@ -185,7 +227,7 @@ template <class T, int NS> __global__ __launch_bounds__(256) void scan_forward(S
 // a segment's end state from zero, and its sum of d
 template <class T, int NS> __global__ __launch_bounds__(256) void scan_segment(ScanArgs a) {
     using raw = typename T::raw;
-    constexpr int G = 4, kChunk = chunk_of(NS);
+    constexpr int G = 4, kChunk = kGroup;
     Place p(a, blockIdx.x / a.across, blockIdx.x % a.across);
     int64_t stop = p.t1 < p.end ? p.t1 : p.end;
     float h[NS], A2[NS], sum = 0;
@@ -197,7 +239,7 @@ template <class T, int NS> __global__ __launch_bounds__(256) void scan_segment(S
     const raw *u = (const raw *)a.u + p.b * a.u_batch, *dt = (const raw *)a.dt + p.b * a.dt_batch;
     Fixed *bc = fixed(a.bc + p.b * a.length * 2 * NS);
     for (int64_t c0 = p.t0; c0 < stop; c0 += kChunk) {
-        uint32_t begins = chunk_mask<kChunk>(a, p.b, c0, p.end);
+        uint32_t begins = group_mask(a, p.b, c0, p.end);
         cut = cut || begins != 0;
         int64_t c1 = c0 + kChunk < stop ? c0 + kChunk : stop;
         for (int64_t t = c0; t < c1; t += G) {
@@ -233,7 +275,7 @@ template <class T, int NS> __global__ __launch_bounds__(256) void scan_segment(S
 // what g leaves before a segment's first token, from zero after its last
 template <class T, int NS> __global__ __launch_bounds__(256) void scan_segment_back(ScanArgs a) {
     using raw = typename T::raw;
-    constexpr int kChunk = chunk_of(NS);
+    constexpr int kChunk = kGroup;
     Place p(a, blockIdx.x / a.across, blockIdx.x % a.across);
     int64_t stop = p.t1 < p.end ? p.t1 : p.end;
     float g[NS], A2[NS], sum = 0;
@@ -247,7 +289,7 @@ template <class T, int NS> __global__ __launch_bounds__(256) void scan_segment_b
     Fixed *bc = fixed(a.bc + p.b * a.length * 2 * NS);
     if (p.t0 < stop)
         for (int64_t c0 = p.t0 + (stop - 1 - p.t0) / kChunk * kChunk; c0 >= p.t0; c0 -= kChunk) {
-            uint32_t begins = chunk_mask<kChunk>(a, p.b, c0, p.end);
+            uint32_t begins = group_mask(a, p.b, c0, p.end);
             cut = cut || begins != 0;
             int64_t c1 = c0 + kChunk < stop ? c0 + kChunk : stop;
             for (int64_t t = c1 - 1; t >= c0; t--) {
@@ -341,18 +383,19 @@ template <int M> __device__ __forceinline__ float wave_sums(float (&v)[M / 2]) {
     return v[0];
 }
 
-// The backward pass walks over a segment's chunks from the last.  In a chunk it goes forward once from the kept state and leaves the
-// state before every SUB-th token in shared memory; then, from the last SUB tokens, forward again with what each token keeps of the
-// state before it, a_t h_{t-1}, in registers (SUB x NS = 128 of them), and backward over them.  dB and dC are summed over the wave's
-// channels token by token (wave_sums), over the block's waves once a chunk, over blocks by scan_bc_out.
+// The backward pass walks over a segment from its end, kept state by kept state.  From one it goes forward over SUB tokens with what
+// each of them keeps of the state before it, a_t h_{t-1}, in registers (SUB x NS = 128 of them; with more tokens to a kept state
+// than that, a first walk leaves the states between in shared memory), and then backward over them.  dB and dC are summed over the
+// wave's channels token by token (wave_sums), over the block's waves after SUB tokens, over blocks by scan_bc_out.  Tokens past the
+// row's end count with d = u = dy = 0, which leaves g as it is and adds nothing.
 template <class T, int NS> __global__ __launch_bounds__(256, 2) void scan_backward(ScanArgs a) {
     using raw = typename T::raw;
-    constexpr int kChunk = chunk_of(NS), SUB = sub_of(NS), kSubs = kChunk / SUB, M = 2 * NS;
+    constexpr int KEPT = kept_of(NS), SUB = sub_of(NS), kSubs = KEPT / SUB, M = 2 * NS;
     extern __shared__ float pool[];
     int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), waves = blockDim.x / kWave;
-    float *states = pool + (size_t)wave * (kSubs - 1) * NS * kWave + lane;       // [subs - 1][NS][64] of this wave
-    float *sums = pool + (size_t)waves * (kSubs - 1) * NS * kWave;               // [waves][chunk][M]
-    int part = blockIdx.x % a.across, group = blockIdx.x / a.across;
+    float *sums = pool;                                                          // [2][waves][SUB][M]
+    float *states = pool + 2 * waves * SUB * M + (size_t)wave * (kSubs - 1) * NS * kWave + lane;       // [subs - 1][NS][64] of this wave
+    int part = blockIdx.x % a.across, group = blockIdx.x / a.across, turn = 0;
     float dA[NS], dD = 0, dbias = 0, A2[NS];
     {
         int at = part * (int)blockDim.x + (int)threadIdx.x;
@@ -366,8 +409,9 @@ template <class T, int NS> __global__ __launch_bounds__(256, 2) void scan_backwa
         bool whole_end = p.end <= p.t1 && (p.end > p.t0 || p.seg == 0);
         raw *du = (raw *)a.du + p.b * a.length * a.width, *ddt = (raw *)a.ddt + p.b * a.length * a.width;
         raw *dz = a.z != nullptr ? (raw *)a.dz + p.b * a.length * a.width : nullptr;
-        float g[NS];
+        const uint32_t bytes = p.bytes(sizeof(raw));
         if (p.t0 < stop || whole_end) {
+            float g[NS];
             if (a.segments > 1) get_row<NS>(a.seg, p.b * a.segments + p.seg, a, p.e, g);
             else first_state<NS>(a.dlast, a, p.b, p.e, g);
             if (!p.on)
@@ -376,100 +420,135 @@ template <class T, int NS> __global__ __launch_bounds__(256, 2) void scan_backwa
             float D = a.D != nullptr ? a.D[p.e] : 0.0f, bias = a.dt_bias != nullptr ? a.dt_bias[p.e] : 0.0f;
             const raw *u = (const raw *)a.u + p.b * a.u_batch, *dt = (const raw *)a.dt + p.b * a.dt_batch, *dy = (const raw *)a.dy + p.b * a.dy_batch;
             const raw *z = a.z != nullptr ? (const raw *)a.z + p.b * a.z_batch : nullptr;
-            Fixed *bc = fixed(a.bc + p.b * a.length * 2 * NS);
+
+            // SUB tokens from t, `here` of which are the row's; bit i of `begins`: an episode begins at token t + i
+            auto walk = [&](int64_t t, int here, uint32_t begins, float (&h)[NS], auto some) __attribute__((always_inline)) {
+                constexpr bool kSome = decltype(some)::value;          // an episode begins among them
+                float keep[SUB][NS], d[SUB], uf[SUB];
+                raw rd[SUB], early[3];
+                Line<raw> lu(u, t * a.u_time, a.u_time), ld(dt, t * a.dt_time, a.dt_time), ly(dy, t * a.dy_time, a.dy_time), lz(z, t * a.z_time, a.z_time);
+#pragma unroll
+                for (int q = 0; q < SUB; q++) {
+                    int at = q < here ? q : here - 1;
+                    raw ru = lu.get(bytes, at);
+                    rd[q] = ld.get(bytes, at);
+                    uf[q] = q < here ? up<T>(ru) : 0.0f;
+                }
+                early[0] = ld.get(bytes, here - 1), early[1] = ly.get(bytes, here - 1), early[2] = lz.get(bytes, here - 1);
+                Fixed *bc = fixed(a.bc + (p.b * a.length + t) * 2 * NS);
+#pragma unroll
+                for (int q = 0; q < SUB; q++) {
+                    Fixed *m = bc + (q < here ? q : here - 1) * 2 * NS;
+                    d[q] = q < here ? softplus_(up<T>(rd[q]) + bias) : 0.0f;
+                    float x = d[q] * uf[q];
+                    bool first = kSome && (begins >> q & 1);
+#pragma unroll
+                    for (int n = 0; n < NS; n++) {
+                        keep[q][n] = first ? 0.0f : exp2_(d[q] * A2[n]) * h[n];
+                        h[n] = __builtin_fmaf(x, m[n], keep[q][n]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                // from here on the compiler does not know d and bc: it would rather keep every exp, state and B of the walk before
+                // (2 x SUB x NS vector and SUB x NS scalar registers more) than take them again
+#pragma unroll
+                for (int q = 0; q < SUB; q++) asm volatile("" : "+v"(d[q]));
+                asm volatile("" : "+s"(bc));
+                float *to = sums + (turn * waves + wave) * SUB * M;
+                Line<raw> gu(du, t * a.width, a.width), gd(ddt, t * a.width, a.width), gz(dz, t * a.width, a.width);
+#pragma unroll
+                for (int q = SUB - 1; q >= 0; q--) {
+                    Pair<NS> m;
+                    m.read(bc + (q < here ? q : here - 1) * 2 * NS);
+                    float raw_d = up<T>(early[0]) + bias, out = q < here ? up<T>(early[1]) : 0.0f, zf = 0, gate = 1, sig = 0;
+                    if (z != nullptr) {
+                        zf = up<T>(early[2]);
+                        sig = sigmoid_(zf);
+                        gate = zf * sig;
+                    }
+                    if (q > 0) {                 // the token before, one token ahead
+                        int at = q - 1 < here ? q - 1 : here - 1;
+                        early[0] = ld.get(bytes, at), early[1] = ly.get(bytes, at), early[2] = lz.get(bytes, at);
+                    }
+                    float o = out * gate, x = d[q] * uf[q], gB = 0, gk = 0, y = D * uf[q], v[NS];
+#pragma unroll
+                    for (int n = 0; n < NS; n++) {
+                        float hn = __builtin_fmaf(x, m.B[n], keep[q][n]);
+                        y = __builtin_fmaf(m.C[n], hn, y);
+                        g[n] = __builtin_fmaf(o, m.C[n], g[n]);
+                        v[n] = first_sum(g[n] * x, o * hn);
+                        gB = __builtin_fmaf(g[n], m.B[n], gB);
+                        float k = g[n] * keep[q][n];
+                        gk = __builtin_fmaf(k, A2[n], gk);
+                        dA[n] = __builtin_fmaf(k, d[q], dA[n]);
+                        g[n] *= exp2_(d[q] * A2[n]);
+                    }
+                    if (kSome && (begins >> q & 1))
+#pragma unroll
+                        for (int n = 0; n < NS; n++) g[n] = 0;
+                    float dd = __builtin_fmaf(uf[q], gB, gk * kLn2), draw = q < here ? dd * sigmoid_(raw_d) : 0.0f;
+                    dD = __builtin_fmaf(o, uf[q], dD);
+                    dbias += draw;
+                    if (q < here) {
+                        gu.put(down<T>(__builtin_fmaf(D, o, d[q] * gB)), bytes, q);
+                        gd.put(down<T>(draw), bytes, q);
+                        if (z != nullptr) gz.put(down<T>(out * y * sig * (1.0f + zf * (1.0f - sig))), bytes, q);
+                    }
+                    float total = wave_sums<M>(v);
+                    if (lane % (kWave / M) == 0) to[q * M + lane / (kWave / M)] = total;
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                // the other half of `sums` is read by nobody after this barrier, and this half is written again after the next
+                __syncthreads();
+                const float *from = sums + turn * waves * SUB * M;
+                float *bc_to = a.part_bc + ((int64_t)part * a.batch * a.length + p.b * a.length + t) * M;
+                for (int k = threadIdx.x; k < here * M; k += blockDim.x) {
+                    float v = 0;
+                    for (int w = 0; w < waves; w++) v += from[w * SUB * M + k];
+                    bc_to[k] = v;
+                }
+                turn ^= 1;
+            };
+
             if (p.t0 < stop)
-                for (int64_t c0 = p.t0 + (stop - 1 - p.t0) / kChunk * kChunk; c0 >= p.t0; c0 -= kChunk) {
-                    uint32_t begins = chunk_mask<kChunk>(a, p.b, c0, p.end);
-                    int count = (int)(c0 + kChunk < stop ? kChunk : stop - c0), subs = (count + SUB - 1) / SUB;
-                    float h[NS];
-                    get_row<NS>(a.kept, p.b * a.chunks + c0 / kChunk, a, p.e, h);
-                    for (int s = 0; s + 1 < subs; s++) {
+                for (int64_t c0 = p.t0 + (stop - 1 - p.t0) / kGroup * kGroup; c0 >= p.t0; c0 -= kGroup) {
+                    uint32_t begins = group_mask(a, p.b, c0, p.end);
+                    int count = (int)(c0 + kGroup < stop ? kGroup : stop - c0);
+                    for (int i = (count - 1) / KEPT * KEPT; i >= 0; i -= KEPT) {
+                        float h[NS];
+                        const int64_t row = p.b * a.chunks + (c0 + i) / KEPT;
+                        kept_row<NS>(a, row, p.bytes(4), h);
+                        int subs = kSubs == 1 || count - i <= SUB ? 1 : (count - i < KEPT ? count - i + SUB - 1 : KEPT) / SUB;
+                        if constexpr (kSubs > 1) {
+                            for (int k = 0; k + 1 < subs; k++) {
 #pragma unroll
-                        for (int q = 0; q < SUB; q++) {
-                            int64_t t = c0 + s * SUB + q;
-                            float d = softplus_(up<T>((dt + t * a.dt_time)[p.e]) + bias), x = d * up<T>((u + t * a.u_time)[p.e]);
-                            if (begins >> (s * SUB + q) & 1)
+                                for (int q = 0; q < SUB; q++) {
+                                    int64_t t = c0 + i + k * SUB + q;
+                                    float d = softplus_(up<T>((dt + t * a.dt_time)[p.e]) + bias), x = d * up<T>((u + t * a.u_time)[p.e]);
+                                    if (begins >> (i + k * SUB + q) & 1)
 #pragma unroll
-                                for (int n = 0; n < NS; n++) h[n] = 0;
-                            Fixed *m = bc + t * 2 * NS;
+                                        for (int n = 0; n < NS; n++) h[n] = 0;
+                                    Fixed *m = fixed(a.bc + (p.b * a.length + t) * 2 * NS);
 #pragma unroll
-                            for (int n = 0; n < NS; n++) h[n] = __builtin_fmaf(exp2_(d * A2[n]), h[n], x * m[n]);
-                        }
-#pragma unroll
-                        for (int n = 0; n < NS; n++) states[(s * NS + n) * kWave] = h[n];
-                    }
-                    for (int s = subs - 1; s >= 0; s--) {
-                        if (s > 0)
-#pragma unroll
-                            for (int n = 0; n < NS; n++) h[n] = states[((s - 1) * NS + n) * kWave];
-                        else get_row<NS>(a.kept, p.b * a.chunks + c0 / kChunk, a, p.e, h);
-                        float keep[SUB][NS], d[SUB], uf[SUB], raws[SUB];
-                        int here = count - s * SUB < SUB ? count - s * SUB : SUB;
-#pragma unroll
-                        for (int q = 0; q < SUB; q++) {
-                            if (q < here) {
-                                int64_t t = c0 + s * SUB + q;
-                                raws[q] = up<T>((dt + t * a.dt_time)[p.e]) + bias;
-                                uf[q] = up<T>((u + t * a.u_time)[p.e]);
-                                d[q] = softplus_(raws[q]);
-                                float x = d[q] * uf[q];
-                                bool first = begins >> (s * SUB + q) & 1;
-                                Fixed *m = bc + t * 2 * NS;
-#pragma unroll
-                                for (int n = 0; n < NS; n++) {
-                                    keep[q][n] = first ? 0.0f : exp2_(d[q] * A2[n]) * h[n];
-                                    h[n] = __builtin_fmaf(x, m[n], keep[q][n]);
+                                    for (int n = 0; n < NS; n++) h[n] = __builtin_fmaf(exp2_(d * A2[n]), h[n], x * m[n]);
                                 }
+#pragma unroll
+                                for (int n = 0; n < NS; n++) states[(k * NS + n) * kWave] = h[n];
                             }
                         }
+                        for (int k = subs - 1; k >= 0; k--) {
+                            if constexpr (kSubs > 1) {
+                                if (k > 0)
 #pragma unroll
-                        for (int q = SUB - 1; q >= 0; q--) {
-                            if (q < here) {
-                                int64_t t = c0 + s * SUB + q;
-                                Pair<NS> m;
-                                m.read(bc + t * 2 * NS);
-                                float out = p.on ? up<T>((dy + t * a.dy_time)[p.e]) : 0.0f, zf = 0, gate = 1, sig = 0;
-                                if (z != nullptr) {
-                                    zf = up<T>((z + t * a.z_time)[p.e]);
-                                    sig = sigmoid_(zf);
-                                    gate = zf * sig;
-                                }
-                                float o = out * gate, x = d[q] * uf[q], gB = 0, gk = 0, y = D * uf[q], v[NS];
-#pragma unroll
-                                for (int n = 0; n < NS; n++) {
-                                    float hn = __builtin_fmaf(x, m.B[n], keep[q][n]);
-                                    y = __builtin_fmaf(m.C[n], hn, y);
-                                    g[n] = __builtin_fmaf(o, m.C[n], g[n]);
-                                    v[n] = first_sum(g[n] * x, o * hn);
-                                    gB = __builtin_fmaf(g[n], m.B[n], gB);
-                                    float k = g[n] * keep[q][n];
-                                    gk = __builtin_fmaf(k, A2[n], gk);
-                                    dA[n] = __builtin_fmaf(k, d[q], dA[n]);
-                                    g[n] *= exp2_(d[q] * A2[n]);
-                                }
-                                if (begins >> (s * SUB + q) & 1)
-#pragma unroll
-                                    for (int n = 0; n < NS; n++) g[n] = 0;
-                                float dd = __builtin_fmaf(uf[q], gB, gk * kLn2), draw = dd * sigmoid_(raws[q]);
-                                dD = __builtin_fmaf(o, uf[q], dD);
-                                dbias += draw;
-                                if (p.on) {
-                                    (du + t * a.width)[p.e] = down<T>(__builtin_fmaf(D, o, d[q] * gB));
-                                    (ddt + t * a.width)[p.e] = down<T>(draw);
-                                    if (z != nullptr) (dz + t * a.width)[p.e] = down<T>(out * y * sig * (1.0f + zf * (1.0f - sig)));
-                                }
-                                float total = wave_sums<M>(v);
-                                if (lane % (kWave / M) == 0) sums[(wave * kChunk + s * SUB + q) * M + lane / (kWave / M)] = total;
+                                    for (int n = 0; n < NS; n++) h[n] = states[((k - 1) * NS + n) * kWave];
+                                else if (subs > 1) kept_row<NS>(a, row, p.bytes(4), h);
                             }
+                            int from = i + k * SUB, here = count - from < SUB ? count - from : SUB;
+                            uint32_t mine = begins >> from & ((1u << SUB) - 1);
+                            if (mine != 0) walk(c0 + from, here, mine, h, std::true_type());
+                            else walk(c0 + from, here, 0, h, std::false_type());
                         }
                     }
-                    __syncthreads();
-                    for (int k = threadIdx.x; k < count * M; k += blockDim.x) {
-                        float v = 0;
-                        for (int w = 0; w < waves; w++) v += sums[w * kChunk * M + k];
-                        a.part_bc[((int64_t)part * a.batch * a.length + p.b * a.length + c0) * M + k] = v;
-                    }
-                    __syncthreads();
                 }
             if (p.on && p.seg == 0 && a.segments == 1 && a.dstate != nullptr) last_state<NS>(a.dstate, a, p.b, p.e, g);
         }
@@ -577,13 +656,13 @@ static ScanPlan scan_plan(const mws_scan_args *a, bool backward) {
     int waves = (int)ceil_div(a->width, kWave);
     p.lanes = (waves < lanes_of(p.ns) / kWave ? waves : lanes_of(p.ns) / kWave) * kWave;
     p.across = (int)ceil_div(a->width, p.lanes);
-    p.chunks = ceil_div(a->length, chunk_of(p.ns));
-    int64_t blocks = a->batch * p.across, wanted = ceil_div(2 * kSimds, blocks > 0 ? blocks * (p.lanes / kWave) : 1);
-    int64_t segments = wanted < p.chunks ? wanted : p.chunks;
+    p.chunks = ceil_div(a->length, kept_of(p.ns));
+    int64_t groups = ceil_div(a->length > 0 ? a->length : 1, kGroup), blocks = a->batch * p.across, wanted = ceil_div(2 * kSimds, blocks > 0 ? blocks * (p.lanes / kWave) : 1);
+    int64_t segments = wanted < groups ? wanted : groups;
     if (segments < 4) segments = 1;
-    int64_t chunks = p.chunks > 0 ? p.chunks : 1, each = ceil_div(chunks, segments);
-    p.segments = (int)ceil_div(chunks, each);
-    p.span = (int)(each * chunk_of(p.ns));
+    int64_t each = ceil_div(groups, segments);
+    p.segments = (int)ceil_div(groups, each);
+    p.span = (int)(each * kGroup);
     int64_t items = a->batch * p.segments, most = 2048 / p.across > 0 ? 2048 / p.across : 1;
     p.groups = (int)(items < most ? items : most);
     int64_t at = 0, tokens = a->batch * a->length;
@@ -608,6 +687,8 @@ static int32_t scan_check(const mws_scan_args *a, const char *what, bool backwar
     if (a->width < 1 || a->width > (1 << 24)) return fail("%s: width %d", what, a->width);
     if (a->batch < 0 || a->length < 0 || a->batch > (1 << 30) || a->length > (1 << 30) || a->batch * (a->length + 1) > ((int64_t)1 << 33)) return fail("%s: %lld rows of %lld tokens", what, (long long)a->batch, (long long)a->length);
     if (step && a->length != 1) return fail("%s: one token at a time", what);
+    for (int64_t stride : {a->u_time, a->dt_time, a->z_time, a->dy_time})
+        if (stride < 0 || stride > MWS_SCAN_MAX_STRIDE) return fail("%s: tokens %lld values apart", what, (long long)stride);
     if (!pointers) return 0;
     if (a->A == nullptr) return fail("%s: A is NULL", what);
     if (a->batch == 0) return 0;
@@ -652,13 +733,13 @@ template <class T, int NS> static void forward_go(const ScanPlan &p, const ScanA
     hipLaunchKernelGGL((scan_forward<T, NS>), grid, block, 0, stream, d);
 }
 template <class T, int NS> static void backward_go(const mws_scan_args *a, const ScanPlan &p, const ScanArgs &d, hipStream_t stream) {
-    constexpr int kChunk = chunk_of(NS), SUB = sub_of(NS);
+    constexpr int SUB = sub_of(NS);
     dim3 block(p.lanes);
     if (p.segments > 1) {
         hipLaunchKernelGGL((scan_segment_back<T, NS>), dim3((unsigned)(d.batch * p.segments * p.across)), block, 0, stream, d);
         join_go(d, NS, true, stream);
     }
-    size_t lds = (size_t)(p.lanes / kWave) * ((kChunk / SUB - 1) * NS * kWave + kChunk * 2 * NS) * sizeof(float);
+    size_t lds = (size_t)(p.lanes / kWave) * ((kept_of(NS) / SUB - 1) * NS * kWave + 2 * SUB * 2 * NS) * sizeof(float);
     if (d.batch > 0) hipLaunchKernelGGL((scan_backward<T, NS>), dim3((unsigned)(p.groups * p.across)), block, lds, stream, d);
     int64_t count = d.batch * d.length * 2 * NS;
     if (count > 0)
@@ -697,7 +778,7 @@ using namespace mws;
 
 extern "C" int64_t mws_scan_kept(const mws_scan_args *a) {
     if (int32_t e = scan_check(a, "mws_scan_kept", false, false, false)) return e;
-    return a->batch * ceil_div(a->length, chunk_of(scan_ns(a))) * scan_ns(a) * a->width;
+    return a->batch * ceil_div(a->length, kept_of(scan_ns(a))) * scan_ns(a) * a->width;
 }
 
 extern "C" int64_t mws_scan_workspace(const mws_scan_args *a, int32_t backward) {

@@ -56,6 +56,7 @@ void want_tokens(const Tensor &x, bool time, const Tensor &reset, const Tensor &
 // ---- launches ----
 Tensor rows(const Tensor &t) { return !t.defined() || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
 Tensor dense(const Tensor &t) { return t.defined() ? t.contiguous() : t; }
+Tensor near(const Tensor &t) { return !t.defined() || (t.dim() == 3 && t.stride(1) > MWS_SCAN_MAX_STRIDE) ? dense(t) : rows(t); }
 Tensor like(const Tensor &t) { return t.defined() ? at::empty(t.sizes(), t.options()) : t; }
 void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 const float *floats(const Tensor &t) { return (const float *)ptr(t); }
@@ -268,7 +269,7 @@ struct SelectiveScan : torch::autograd::Function<SelectiveScan> {
         want_once();
         auto s = ctx->get_saved_variables();
         ScanIn t = {s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], s[9], s[10]};
-        Tensor dy = grads[0].defined() ? rows(grads[0]) : at::zeros(t.u.sizes(), t.u.options()), dlast = dense(grads[1]);
+        Tensor dy = grads[0].defined() ? near(grads[0]) : at::zeros(t.u.sizes(), t.u.options()), dlast = dense(grads[1]);
         variable_list d;
         for (int k = 0; k < 9; k++) d.push_back(like(s[k]));
         mws_scan_args a = scan_args(t);
@@ -303,7 +304,7 @@ ScanIn scan_check(const Tensor &u, const Tensor &dt, const Tensor &A, const Tens
     return t;
 }
 void scan_rows(ScanIn &t) {
-    t.u = rows(t.u), t.dt = rows(t.dt), t.B = rows(t.B), t.C = rows(t.C), t.D = rows(t.D), t.z = rows(t.z), t.dt_bias = rows(t.dt_bias), t.A = t.A.contiguous();
+    t.u = near(t.u), t.dt = near(t.dt), t.B = rows(t.B), t.C = rows(t.C), t.D = rows(t.D), t.z = near(t.z), t.dt_bias = rows(t.dt_bias), t.A = t.A.contiguous();
 }
 variable_list selective_scan(const Tensor &u, const Tensor &dt, const Tensor &A, const Tensor &B, const Tensor &C, const Maybe &D, const Maybe &z, const Maybe &dt_bias, const Maybe &state,
                              const Maybe &reset, const Maybe &lengths) {
