@@ -15,7 +15,6 @@
 // Where batch x channels leave the card empty, the time axis is cut into segments of whole chunks: scan_segment takes each
 // segment's end state from zero and its sum of d (the product of its a is exp(A sum d)), scan_join runs over the segments, and the
 // scan itself starts every segment from its joined state.  The same holds for g, from the end.
-#include <type_traits>
 #include "mws_common.hpp"
 
 namespace mws {
@@ -388,7 +387,7 @@ template <int M> __device__ __forceinline__ float wave_sums(float (&v)[M / 2]) {
 // than that, a first walk leaves the states between in shared memory), and then backward over them.  dB and dC are summed over the
 // wave's channels token by token (wave_sums), over the block's waves after SUB tokens, over blocks by scan_bc_out.  Tokens past the
 // row's end count with d = u = dy = 0, which leaves g as it is and adds nothing.
-template <class T, int NS> __global__ __launch_bounds__(256, 2) void scan_backward(ScanArgs a) {
+template <class T, int NS> __global__ __launch_bounds__(256, NS >= 32 ? 2 : 2) void scan_backward(ScanArgs a) {
     using raw = typename T::raw;
     constexpr int KEPT = kept_of(NS), SUB = sub_of(NS), kSubs = KEPT / SUB, M = 2 * NS;
     extern __shared__ float pool[];
@@ -422,8 +421,7 @@ template <class T, int NS> __global__ __launch_bounds__(256, 2) void scan_backwa
             const raw *z = a.z != nullptr ? (const raw *)a.z + p.b * a.z_batch : nullptr;
 
             // SUB tokens from t, `here` of which are the row's; bit i of `begins`: an episode begins at token t + i
-            auto walk = [&](int64_t t, int here, uint32_t begins, float (&h)[NS], auto some) __attribute__((always_inline)) {
-                constexpr bool kSome = decltype(some)::value;          // an episode begins among them
+            auto walk = [&](int64_t t, int here, uint32_t begins, float (&h)[NS]) __attribute__((always_inline)) {
                 float keep[SUB][NS], d[SUB], uf[SUB];
                 raw rd[SUB], early[3];
                 Line<raw> lu(u, t * a.u_time, a.u_time), ld(dt, t * a.dt_time, a.dt_time), ly(dy, t * a.dy_time, a.dy_time), lz(z, t * a.z_time, a.z_time);
@@ -441,11 +439,16 @@ template <class T, int NS> __global__ __launch_bounds__(256, 2) void scan_backwa
                     Fixed *m = bc + (q < here ? q : here - 1) * 2 * NS;
                     d[q] = q < here ? softplus_(up<T>(rd[q]) + bias) : 0.0f;
                     float x = d[q] * uf[q];
-                    bool first = kSome && (begins >> q & 1);
+                    if (begins >> q & 1)
+#pragma unroll
+                        for (int n = 0; n < NS; n++) h[n] = 0;
 #pragma unroll
                     for (int n = 0; n < NS; n++) {
-                        keep[q][n] = first ? 0.0f : exp2_(d[q] * A2[n]) * h[n];
+                        keep[q][n] = exp2_(d[q] * A2[n]) * h[n];
                         h[n] = __builtin_fmaf(x, m[n], keep[q][n]);
+                        if (n % 4 == 3)
+#pragma unroll
+                            for (int k = n - 3; k <= n; k++) asm volatile("" : "+v"(keep[q][k]), "+v"(h[k]));
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -473,17 +476,23 @@ template <class T, int NS> __global__ __launch_bounds__(256, 2) void scan_backwa
                     float o = out * gate, x = d[q] * uf[q], gB = 0, gk = 0, y = D * uf[q], v[NS];
 #pragma unroll
                     for (int n = 0; n < NS; n++) {
+                        if (n % 4 == 0)
+#pragma unroll
+                            for (int k = n; k < n + 4; k++) asm volatile("" : "+v"(keep[q][k]), "+v"(g[k]));
                         float hn = __builtin_fmaf(x, m.B[n], keep[q][n]);
                         y = __builtin_fmaf(m.C[n], hn, y);
                         g[n] = __builtin_fmaf(o, m.C[n], g[n]);
                         v[n] = first_sum(g[n] * x, o * hn);
                         gB = __builtin_fmaf(g[n], m.B[n], gB);
-                        float k = g[n] * keep[q][n];
-                        gk = __builtin_fmaf(k, A2[n], gk);
-                        dA[n] = __builtin_fmaf(k, d[q], dA[n]);
+                        float gh = g[n] * keep[q][n];
+                        gk = __builtin_fmaf(gh, A2[n], gk);
+                        dA[n] = __builtin_fmaf(gh, d[q], dA[n]);
                         g[n] *= exp2_(d[q] * A2[n]);
+                        if (n % 4 == 3)
+#pragma unroll
+                            for (int k = n - 3; k <= n; k++) asm volatile("" : "+v"(dA[k]), "+v"(g[k]), "+v"(v[k]));
                     }
-                    if (kSome && (begins >> q & 1))
+                    if (begins >> q & 1)
 #pragma unroll
                         for (int n = 0; n < NS; n++) g[n] = 0;
                     float dd = __builtin_fmaf(uf[q], gB, gk * kLn2), draw = q < here ? dd * sigmoid_(raw_d) : 0.0f;
@@ -544,9 +553,7 @@ template <class T, int NS> __global__ __launch_bounds__(256, 2) void scan_backwa
                                 else if (subs > 1) kept_row<NS>(a, row, p.bytes(4), h);
                             }
                             int from = i + k * SUB, here = count - from < SUB ? count - from : SUB;
-                            uint32_t mine = begins >> from & ((1u << SUB) - 1);
-                            if (mine != 0) walk(c0 + from, here, mine, h, std::true_type());
-                            else walk(c0 + from, here, 0, h, std::false_type());
+                            walk(c0 + from, here, begins >> from, h);
                         }
                     }
                 }
