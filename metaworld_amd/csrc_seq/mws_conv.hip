@@ -58,14 +58,25 @@ template <class T, int V> struct Chan {
     }
 };
 
+// a lane's V x K weights lie next to each other
 template <class T, int V, int K> __device__ __forceinline__ void taps(const ConvArgs &a, int e, Chan<T, V> (&w)[K], Chan<T, V> &b) {
+    if (e + V <= a.width) {
+        if (a.wide) {
+            Vec<F32, V * K> r = load<F32, V * K>((const float *)a.weight + (int64_t)e * K);
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-        bool on = e + i < a.width;
+            for (int i = 0; i < V * K; i++) w[i % K].v[i / K] = r.v[i];
+        } else {
+            Vec<T, V * K> r = load<T, V * K>((const typename T::raw *)a.weight + (int64_t)e * K);
 #pragma unroll
-        for (int j = 0; j < K; j++) w[j].v[i] = on ? param<T>(a.weight, (int64_t)(e + i) * K + j, a.wide) : 0.0f;
-        b.v[i] = on && a.bias != nullptr ? param<T>(a.bias, e + i, a.wide) : 0.0f;
-    }
+            for (int i = 0; i < V * K; i++) w[i % K].v[i / K] = up<T>(r.v[i]);
+        }
+    } else
+#pragma unroll
+        for (int i = 0; i < V; i++)
+#pragma unroll
+            for (int j = 0; j < K; j++) w[j].v[i] = e + i < a.width ? param<T>(a.weight, (int64_t)(e + i) * K + j, a.wide) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; i++) b.v[i] = e + i < a.width && a.bias != nullptr ? param<T>(a.bias, e + i, a.wide) : 0.0f;
 }
 
 // the input at token p of row b (p >= -(K - 1); below zero: the state)
@@ -102,10 +113,17 @@ template <class T, int V, int K> __global__ __launch_bounds__(256) void conv_for
                 for (int i = 0; i < j; i++) x[i].zero();
         }
         begins >>= K - 1;
-        for (int64_t t = t0; t < stop; t += 4) {
-            Vec<T, V> in[4];
+        // four tokens at a time, the next four under way meanwhile
+        const raw *from = (const raw *)a.x + b * a.x_batch + e;
+        Vec<T, V> in[4], next[4];
 #pragma unroll
-            for (int q = 0; q < 4; q++) in[q] = input<T, V, K>(a, b, t + q < stop ? t + q : stop - 1, e, n);
+        for (int q = 0; q < 4; q++) next[q] = load_some<T, V>(from + (t0 + q < stop ? t0 + q : stop - 1) * a.x_time, n);
+        for (int64_t t = t0; t < stop; t += 4) {
+#pragma unroll
+            for (int q = 0; q < 4; q++) in[q] = next[q];
+            if (t + 4 < stop)
+#pragma unroll
+                for (int q = 0; q < 4; q++) next[q] = load_some<T, V>(from + (t + 4 + q < stop ? t + 4 + q : stop - 1) * a.x_time, n);
 #pragma unroll
             for (int q = 0; q < 4; q++) {
                 if (t + q >= stop) break;
@@ -167,7 +185,7 @@ template <class T, int V, int K> __global__ __launch_bounds__(256) void conv_bac
         int age = K;                                     // tokens since the episode's first
         raw *dx = (raw *)a.dx + b * a.length * a.width + e, *dstate = (raw *)a.dstate + b * (K - 1) * a.width + e;
         // dx of token p, whose terms are complete: those of the tokens, and of the state that the row leaves
-        auto emit = [&](int64_t p, Chan<T, V> v) {
+        auto emit = [&](int64_t p, Chan<T, V> v) __attribute__((always_inline)) {
             if (p >= t1 || (p < t0 && t0 > 0)) return;
             int64_t j = p - (end - (K - 1));
             if (a.dlast != nullptr && j >= 0 && j < K - 1 && (tail >> (j + 1)) == 0) {
@@ -193,15 +211,21 @@ template <class T, int V, int K> __global__ __launch_bounds__(256) void conv_bac
                 }
             }
             begins >>= K - 1;
-            const raw *dyp = (const raw *)a.dy + b * a.dy_batch + e;
-            while (t < stop) {
-                Vec<T, V> in[4], out[4];
+            const raw *dyp = (const raw *)a.dy + b * a.dy_batch + e, *xp = (const raw *)a.x + b * a.x_batch + e;
+            Vec<T, V> in[4], out[4], next_in[4], next_out[4];
+            auto fetch = [&](int64_t from) __attribute__((always_inline)) {
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
-                    int64_t p = t + q < stop ? t + q : stop - 1;
-                    in[q] = input<T, V, K>(a, b, p, e, n);
-                    out[q] = load_some<T, V>(dyp + p * a.dy_time, n);
+                    int64_t p = from + q < stop ? from + q : stop - 1;
+                    next_in[q] = load_some<T, V>(xp + p * a.x_time, n);
+                    next_out[q] = load_some<T, V>(dyp + p * a.dy_time, n);
                 }
+            };
+            fetch(t0);
+            while (t < stop) {
+#pragma unroll
+                for (int q = 0; q < 4; q++) in[q] = next_in[q], out[q] = next_out[q];
+                if (t + 4 < stop) fetch(t + 4);
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
                     if (t >= stop) break;
@@ -273,33 +297,45 @@ template <class T, int V, int K> __global__ __launch_bounds__(256) void conv_bac
         }
 }
 
-// one token: the window is the state and x; every value of the state is read and written once
-template <class T, int V, int K> __global__ __launch_bounds__(256) void conv_step(ConvArgs a, int64_t groups) {
+// One token: the window is the state and x; every value of the state is read and written once.  A lane keeps its channels' weights
+// for up to kStepRows rows; a row is under way while the one before is worked on.
+constexpr int kStepRows = 8;
+template <class T, int V, int K> __global__ __launch_bounds__(256) void conv_step(ConvArgs a, int64_t groups, int64_t each) {
     using raw = typename T::raw;
     int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (at >= a.batch * groups) return;
-    int64_t b = at / groups;
+    if (at >= each * groups) return;
     int e = (int)(at % groups) * V, n = a.width - e;
-    Chan<T, V> w[K], s;
-    taps<T, V, K>(a, e, w, s);
-    bool first = a.reset != nullptr && a.reset[b * a.reset_batch] != 0;
-    Vec<T, V> in[K];
+    int64_t b0 = at / groups;                             // rows b0, b0 + each, ..
+    Chan<T, V> w[K], bias;
+    taps<T, V, K>(a, e, w, bias);
+    Vec<T, V> next[K];
+    bool next_first = false;
+    auto fetch = [&](int64_t b) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < K; j++) {
-        in[j] = input<T, V, K>(a, b, j - (K - 1), e, n);
-        if (first && j + 1 < K)
+        for (int j = 0; j < K; j++) next[j] = input<T, V, K>(a, b, j - (K - 1), e, n);
+        next_first = a.reset != nullptr && a.reset[b * a.reset_batch] != 0;
+    };
+    fetch(b0);
+    for (int64_t b = b0; b < a.batch; b += each) {
+        Vec<T, V> in[K];
+        bool first = next_first;
 #pragma unroll
-            for (int i = 0; i < V; i++) in[j].v[i] = 0;
+        for (int j = 0; j < K; j++) in[j] = next[j];
+        if (b + each < a.batch) fetch(b + each);
+        Chan<T, V> s = bias;
+#pragma unroll
+        for (int j = 0; j < K; j++)
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                if (first && j + 1 < K) in[j].v[i] = 0;
+                s.v[i] += w[j].v[i] * up<T>(in[j].v[i]);
+            }
+#pragma unroll
+        for (int i = 0; i < V; i++) s.v[i] *= sigmoid_(s.v[i]);
+        store_some<T, V>((raw *)a.y + b * a.width + e, s.rounded(), n);
+#pragma unroll
+        for (int j = 0; j + 1 < K; j++) store_some<T, V>((raw *)a.last + (b * (K - 1) + j) * a.width + e, in[j + 1], n);
     }
-#pragma unroll
-    for (int j = 0; j < K; j++)
-#pragma unroll
-        for (int i = 0; i < V; i++) s.v[i] += w[j].v[i] * up<T>(in[j].v[i]);
-#pragma unroll
-    for (int i = 0; i < V; i++) s.v[i] *= sigmoid_(s.v[i]);
-    store_some<T, V>((raw *)a.y + b * a.width + e, s.rounded(), n);
-#pragma unroll
-    for (int j = 0; j + 1 < K; j++) store_some<T, V>((raw *)a.last + (b * (K - 1) + j) * a.width + e, in[j + 1], n);
 }
 
 struct ConvOut {
@@ -319,6 +355,7 @@ struct ConvOut {
 
 // A tile of 32 tokens re-reads K - 1 of its neighbour's; where that leaves less than four waves to a SIMD, tiles get shorter.
 static int conv_v(const mws_conv_args *a) { return a->type == MWS_F32 ? 4 : 8; }
+constexpr int kBackV = 4;          // channels of a lane backward: with eight the weights, inputs, sums and gradients of K taps take 211 registers
 static int conv_tile(const mws_conv_args *a) {
     int64_t across = a->batch * ceil_div(a->width, kWave * conv_v(a));
     int tile = kMostTile;
@@ -328,7 +365,7 @@ static int conv_tile(const mws_conv_args *a) {
 static int64_t conv_tiles(const mws_conv_args *a) { return a->length > 0 ? ceil_div(a->length, conv_tile(a)) : 1; }
 // backward: each block's partial sums are K + 1 values a channel; two blocks to a compute unit, over the channels' groups
 static int64_t conv_blocks(const mws_conv_args *a) {
-    int64_t need = ceil_div(a->batch * conv_tiles(a), 4), groups = ceil_div(a->width, kWave * conv_v(a));
+    int64_t need = ceil_div(a->batch * conv_tiles(a), 4), groups = ceil_div(a->width, kWave * kBackV);
     int64_t most = groups < 16 ? 1024 / groups : 64;
     return need < most ? need : most;
 }
@@ -366,10 +403,11 @@ enum { kForward, kBackward, kStep };
 template <class T, int V, int K> static void conv_go(const mws_conv_args *a, const ConvArgs &d, int what, hipStream_t stream) {
     unsigned groups = (unsigned)ceil_div(a->width, kWave * V);
     if (what == kForward) hipLaunchKernelGGL((conv_forward<T, V, K>), dim3((unsigned)ceil_div(d.batch * d.tiles, 4), groups), dim3(256), 0, stream, d);
-    else if (what == kBackward) hipLaunchKernelGGL((conv_backward<T, V, K>), dim3((unsigned)conv_blocks(a), groups), dim3(256), 0, stream, d);
+    else if (what == kBackward)
+        hipLaunchKernelGGL((conv_backward<T, kBackV, K>), dim3((unsigned)conv_blocks(a), (unsigned)ceil_div(a->width, kWave * kBackV)), dim3(256), 0, stream, d);
     else {
-        int64_t each = ceil_div(a->width, V);
-        hipLaunchKernelGGL((conv_step<T, V, K>), dim3((unsigned)ceil_div(d.batch * each, 256)), dim3(256), 0, stream, d, each);
+        int64_t across = ceil_div(a->width, V), each = step_lanes(d.batch, across, kStepRows);
+        hipLaunchKernelGGL((conv_step<T, V, K>), dim3((unsigned)ceil_div(each * across, 256)), dim3(256), 0, stream, d, across, each);
     }
 }
 template <class T, int V> static void conv_taps(const mws_conv_args *a, const ConvArgs &d, int what, hipStream_t stream) {

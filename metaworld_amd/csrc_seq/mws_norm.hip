@@ -20,21 +20,32 @@ struct NormArgs {
     int64_t rows, x_stride, dy_stride;
     int width;
     bool wide;                   // float parameters
-    float eps;
+    float share, eps;            // 1 / width
 };
 
-template <int TPR> __device__ __forceinline__ float row_sum(float v, float *meet) {
-    if constexpr (TPR <= kWave) return lane_sum<TPR>(v);
-    else {
-        v = lane_sum<kWave>(v);
-        int wave = threadIdx.x / kWave;
-        __syncthreads();                     // the last sum has been read
-        if (threadIdx.x % kWave == 0) meet[wave] = v;
+// the sum over a row's threads, to all of them.  Over several waves through shared memory: `turn` alternates between its halves, so
+// that one barrier is enough (who writes a half again has passed the barrier after its last reading)
+template <int TPR> __device__ __forceinline__ float row_sum(float v, float (*meet)[16], int &turn) {
+    v = lane_sum<(TPR < kWave ? TPR : kWave)>(v);
+    if constexpr (TPR > kWave) {
+        if (threadIdx.x % kWave == 0) meet[turn][threadIdx.x / kWave] = v;
         __syncthreads();
-        float s = 0;
+        v = 0;
 #pragma unroll
-        for (int k = 0; k < TPR / kWave; k++) s += meet[k];
-        return s;
+        for (int k = 0; k < TPR / kWave; k++) v += meet[turn][k];
+        turn ^= 1;
+    }
+    return v;
+}
+template <int TPR> __device__ __forceinline__ void row_sums(float &v, float &u, float (*meet)[16], float (*meet2)[16], int &turn) {
+    v = lane_sum<(TPR < kWave ? TPR : kWave)>(v), u = lane_sum<(TPR < kWave ? TPR : kWave)>(u);
+    if constexpr (TPR > kWave) {
+        if (threadIdx.x % kWave == 0) meet[turn][threadIdx.x / kWave] = v, meet2[turn][threadIdx.x / kWave] = u;
+        __syncthreads();
+        v = u = 0;
+#pragma unroll
+        for (int k = 0; k < TPR / kWave; k++) v += meet[turn][k], u += meet2[turn][k];
+        turn ^= 1;
     }
 }
 
@@ -69,11 +80,15 @@ template <class T, int V, int PER, int TPR> struct Row {
             }
     }
     // centres the row and returns r; columns past the width stay zero
-    __device__ __forceinline__ float centre(int lane, int width, float eps, float *meet) {
+    __device__ __forceinline__ float centre(int lane, int width, float share, float eps, float (*meet)[16], int &turn) {
         float s = 0;
 #pragma unroll
         for (int k = 0; k < PER * V; k++) s += v[k];
-        float mean = row_sum<TPR>(s, meet) / (float)width, q = 0;
+        s = row_sum<TPR>(s, meet, turn);
+        // the quotient to the last bit (a product and the correction of its error): a row of equal values has to come out as zeros,
+        // and 1 / sqrt(eps) times an error of the mean is seen
+        float mean = s * share, q = 0;
+        mean = __builtin_fmaf(__builtin_fmaf(-mean, (float)width, s), share, mean);
 #pragma unroll
         for (int k = 0; k < PER; k++)
 #pragma unroll
@@ -83,14 +98,14 @@ template <class T, int V, int PER, int TPR> struct Row {
                 v[k * V + i] = c;
                 q += c * c;
             }
-        return 1.0f / sqrtf(row_sum<TPR>(q, meet) / (float)width + eps);
+        return __builtin_amdgcn_rsqf(row_sum<TPR>(q, meet, turn) * share + eps);
     }
 };
 
 template <class T, int V, int PER, int TPR> __global__ __launch_bounds__(TPR > kWave ? TPR : 256) void norm_forward(NormArgs a) {
     constexpr int kRows = TPR <= kWave ? 256 / TPR : 1;      // rows of one block at a time
-    __shared__ float meet[16];
-    int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+    __shared__ float meet[2][16];
+    int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR, turn = 0;
     Row<T, V, PER, TPR> w, b, x;
     w.read_param(a.weight, lane, a.width, a.wide, 1.0f);
     b.read_param(a.bias, lane, a.width, a.wide, 0.0f);
@@ -98,7 +113,7 @@ template <class T, int V, int PER, int TPR> __global__ __launch_bounds__(TPR > k
         int64_t row = row0 + sub;
         bool on = row < a.rows;
         x.read((const typename T::raw *)a.x + (on ? row : a.rows - 1) * a.x_stride, lane, a.width);
-        float r = x.centre(lane, a.width, a.eps, meet);
+        float r = x.centre(lane, a.width, a.share, a.eps, meet, turn);
 #pragma unroll
         for (int k = 0; k < PER * V; k++) x.v[k] = x.v[k] * r * w.v[k] + b.v[k];
         if (on) x.write((typename T::raw *)a.y + row * a.width, lane, a.width);
@@ -107,8 +122,8 @@ template <class T, int V, int PER, int TPR> __global__ __launch_bounds__(TPR > k
 
 template <class T, int V, int PER, int TPR> __global__ __launch_bounds__(TPR > kWave ? TPR : 256) void norm_backward(NormArgs a) {
     constexpr int kRows = TPR <= kWave ? 256 / TPR : 1;
-    __shared__ float meet[16];
-    int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+    __shared__ float meet[2][16], meet2[2][16];
+    int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR, turn = 0;
     Row<T, V, PER, TPR> w, x, g;
     float dw[PER * V], db[PER * V];
 #pragma unroll
@@ -120,7 +135,7 @@ template <class T, int V, int PER, int TPR> __global__ __launch_bounds__(TPR > k
         int64_t at = on ? row : a.rows - 1;
         x.read((const typename T::raw *)a.x + at * a.x_stride, lane, a.width);
         g.read((const typename T::raw *)a.dy + at * a.dy_stride, lane, a.width);
-        float r = x.centre(lane, a.width, a.eps, meet), s = 0, q = 0;
+        float r = x.centre(lane, a.width, a.share, a.eps, meet, turn), s = 0, q = 0;
 #pragma unroll
         for (int k = 0; k < PER * V; k++) {
             float n = x.v[k] * r, d = g.v[k];
@@ -132,8 +147,9 @@ template <class T, int V, int PER, int TPR> __global__ __launch_bounds__(TPR > k
             s += d;                    // columns past the width were read as zeros
             q += d * n;
         }
-        s = row_sum<TPR>(s, meet) / (float)a.width;
-        q = row_sum<TPR>(q, meet) / (float)a.width;
+        row_sums<TPR>(s, q, meet, meet2, turn);
+        s *= a.share;
+        q *= a.share;
         if (a.dx != nullptr) {
 #pragma unroll
             for (int k = 0; k < PER * V; k++) x.v[k] = r * (g.v[k] - s - x.v[k] * q);
@@ -178,16 +194,17 @@ struct NormOut {
     }
 };
 
-// How many blocks walk over the rows: enough to fill the card (8 blocks of 4 waves to a compute unit forward; half of that
-// backward, whose partial sums are 8 bytes a column and block).
+// Threads of a row: eight values each from 1025 columns on (16384 x 4096 bf16 forward 65 us, backward 116 us; with sixteen 71 and
+// 160 us).  Blocks walk over the rows, 4096 waves in all (262144 x 512 bf16 forward 129 us, backward 174 us; with twice as many 133
+// and 195 us); twice that forward in blocks of 1024 threads, two of which fit a compute unit (4000 x 16384 fp32 111 us, not 182).
 static int norm_rows(int tpr) { return tpr <= kWave ? 256 / tpr : 1; }
 static int norm_tpr(const mws_norm_args *a) {
     int v = a->type == MWS_F32 ? 4 : 8, w = a->width;
-    return w <= 8 * v ? 8 : w <= 16 * v ? 16 : w <= 32 * v ? 32 : w <= 1024 ? 64 : w <= 2048 ? 128 : w <= 4096 ? 256 : w <= 8192 ? 512 : 1024;
+    return w <= 8 * v ? 8 : w <= 16 * v ? 16 : w <= 32 * v ? 32 : w <= 1024 ? 64 : w <= 2048 ? 256 : w <= 4096 ? 512 : 1024;
 }
 static int64_t norm_blocks(const mws_norm_args *a, bool backward) {
     int tpr = norm_tpr(a);
-    int64_t most = (backward ? 1024 : 2048) / (tpr > 256 ? tpr / 256 : 1) * (tpr == 128 ? 2 : 1), need = ceil_div(a->rows, norm_rows(tpr));
+    int64_t most = tpr <= 256 ? 1024 : tpr == 512 || !backward ? 512 : 256, need = ceil_div(a->rows, norm_rows(tpr));
     return need < most ? need : most;
 }
 
@@ -199,7 +216,7 @@ template <class T, int V> static void norm_launch(const mws_norm_args *a, const 
         if (backward) hipLaunchKernelGGL((norm_backward<T, V, PER, TPR>), grid, dim3(TPR > kWave ? TPR : 256), 0, stream, d);       \
         else hipLaunchKernelGGL((norm_forward<T, V, PER, TPR>), grid, dim3(TPR > kWave ? TPR : 256), 0, stream, d);                 \
     } while (0)
-    constexpr int P = 16 / V;                // sixteen values of a row to a thread at most: five rows' worth of registers backward
+    constexpr int P = 16 / V;                // sixteen values of a row to a thread at most, eight in blocks of several waves: five rows' worth of registers backward
     switch (norm_tpr(a)) {
         case 8: MWS_GO(1, 8); break;
         case 16: MWS_GO(1, 16); break;
@@ -209,10 +226,11 @@ template <class T, int V> static void norm_launch(const mws_norm_args *a, const 
             else if (w <= 128 * V) MWS_GO(2, 64);
             else MWS_GO(P, 64);
             break;
-        case 128: MWS_GO(P, 128); break;
-        case 256: MWS_GO(P, 256); break;
-        case 512: MWS_GO(P, 512); break;
-        default: MWS_GO(P, 1024); break;
+        case 256: MWS_GO(P / 2, 256); break;
+        case 512: MWS_GO(P / 2, 512); break;
+        default:
+            if (w <= 8192) MWS_GO(P / 2, 1024);
+            else MWS_GO(P, 1024);
     }
 #undef MWS_GO
 }
@@ -231,7 +249,7 @@ static int32_t norm_check(const mws_norm_args *a, bool backward) {
 }
 
 static NormArgs norm_device(const mws_norm_args *a) {
-    NormArgs d = {a->x, a->weight, a->bias, a->dy, a->y, a->dx, nullptr, a->rows, a->x_stride, a->dy_stride, a->width, a->param_type == MWS_F32, a->eps};
+    NormArgs d = {a->x, a->weight, a->bias, a->dy, a->y, a->dx, nullptr, a->rows, a->x_stride, a->dy_stride, a->width, a->param_type == MWS_F32, 1.0f / (float)a->width, a->eps};
     return d;
 }
 static void norm_run(const mws_norm_args *a, const NormArgs &d, bool backward, hipStream_t stream) {

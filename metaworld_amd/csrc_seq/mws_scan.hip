@@ -339,20 +339,6 @@ __global__ __launch_bounds__(256) void scan_join(ScanArgs a, int ns, bool backwa
 
 // ---- sums of M values over the 64 lanes of a wave: every step adds one half of the lanes to the other and halves the values that
 // a lane carries, so that M values take about 2 M instructions.  Lane l gets the sum of value l / (64 / M). ----
-__device__ __forceinline__ void swap32(float &x, float &y) {
-    auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y), false, false);
-    unsigned r0 = r[0], r1 = r[1];       // (a bit cast of an element itself takes the vector's first)
-    x = __builtin_bit_cast(float, r0), y = __builtin_bit_cast(float, r1);
-}
-__device__ __forceinline__ void swap16(float &x, float &y) {
-    auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y), false, false);
-    unsigned r0 = r[0], r1 = r[1];       // (a bit cast of an element itself takes the vector's first)
-    x = __builtin_bit_cast(float, r0), y = __builtin_bit_cast(float, r1);
-}
-template <int CTRL> __device__ __forceinline__ float dpp(float x) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
-}
-constexpr int kRor8 = 0x128, kHalfMirror = 0x141, kQuad2 = 0x4E, kQuad1 = 0xB1;    // the lane 8 on in its row; 7 - lane in its half row; lane ^ 2; lane ^ 1
 template <int CTRL, int COUNT> __device__ __forceinline__ void fold(float *v, bool high) {      // COUNT values to COUNT / 2, or one value over both halves
     if constexpr (COUNT == 1) v[0] += dpp<CTRL>(v[0]);
     else {
@@ -604,45 +590,61 @@ struct ScanOut {
 // ---- one token ----
 // Q lanes share a channel, four states each: the state goes through registers in 16-byte pieces, in order of memory.  Bound by memory:
 // 8 bytes a state.  Q = 0: a lane takes a channel's states one by one, for numbers of states that four lanes cannot share evenly.
-template <class T, int Q> __global__ __launch_bounds__(256) void scan_step(ScanArgs a, const void *B, const void *C, int64_t B_batch, int64_t C_batch) {
+// A lane keeps its channel's parameters for up to kStepRows rows; a row's state is under way while the one before is worked on.
+constexpr int kStepRows = 4;
+template <class T, int Q> __global__ __launch_bounds__(256) void scan_step(ScanArgs a, const void *B, const void *C, int64_t B_batch, int64_t C_batch, int64_t each) {
     using raw = typename T::raw;
-    constexpr int kLanesOf = Q > 0 ? Q : 1;
+    constexpr int kLanesOf = Q > 0 ? Q : 1, W = Q > 0 ? 4 : 1;
     int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, row = at / kLanesOf;
-    if (row >= a.batch * a.width) return;            // whole groups of Q lanes leave together
+    if (row >= each * a.width) return;               // whole groups of Q lanes leave together
     int q = (int)(at % kLanesOf), e = (int)(row % a.width);
-    int64_t b = row / a.width;
-    float uf = up<T>(((const raw *)a.u)[b * a.u_batch + e]);
-    float d = softplus_(up<T>(((const raw *)a.dt)[b * a.dt_batch + e]) + (a.dt_bias != nullptr ? a.dt_bias[e] : 0.0f)), x = d * uf, o = 0;
-    bool first = a.reset != nullptr && a.reset[b * a.reset_batch] != 0;
-    const raw *Bp = (const raw *)B + b * B_batch, *Cp = (const raw *)C + b * C_batch;
-    const float *from = a.state + row * a.states, *A = a.A + (int64_t)e * a.states;
-    float *to = a.last + row * a.states;
+    int64_t b0 = row / a.width;                      // rows b0, b0 + each, ..
+    float bias = a.dt_bias != nullptr ? a.dt_bias[e] : 0.0f, D = a.D != nullptr ? a.D[e] : 0.0f;
+    const float *A = a.A + (int64_t)e * a.states;
+    Vec<F32, W> A2, next, h;
     if constexpr (Q > 0) {
-        Vec<F32, 4> h = load<F32, 4>(from + q * 4), r = load<F32, 4>(A + q * 4);
-        Vec<T, 4> Bv = load<T, 4>(Bp + q * 4), Cv = load<T, 4>(Cp + q * 4);
+        A2 = load<F32, W>(A + q * 4);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            float keep = first ? 0.0f : exp2_(d * (r.v[i] * kLog2e)) * h.v[i];
-            h.v[i] = __builtin_fmaf(x, up<T>(Bv.v[i]), keep);
-            o = __builtin_fmaf(up<T>(Cv.v[i]), h.v[i], o);
-        }
-        store<F32, 4>(to + q * 4, h);
-        o = lane_sum<Q>(o);
-    } else {
-        for (int n = 0; n < a.states; n++) {
-            float keep = first ? 0.0f : exp2_(d * (A[n] * kLog2e)) * from[n];
-            float h = __builtin_fmaf(x, up<T>(Bp[n]), keep);
-            o = __builtin_fmaf(up<T>(Cp[n]), h, o);
-            to[n] = h;
-        }
+        for (int i = 0; i < W; i++) A2.v[i] *= kLog2e;
     }
-    if (q == 0) {
-        if (a.D != nullptr) o = __builtin_fmaf(a.D[e], uf, o);
-        if (a.z != nullptr) {
-            float zf = up<T>(((const raw *)a.z)[b * a.z_batch + e]);
-            o *= zf * sigmoid_(zf);
+    raw next_u = 0, next_dt = 0, next_z = 0;
+    auto fetch = [&](int64_t b) __attribute__((always_inline)) {
+        next_u = ((const raw *)a.u)[b * a.u_batch + e], next_dt = ((const raw *)a.dt)[b * a.dt_batch + e];
+        if (a.z != nullptr) next_z = ((const raw *)a.z)[b * a.z_batch + e];
+        if constexpr (Q > 0) next = load<F32, W>(a.state + (b * a.width + e) * a.states + q * 4);
+    };
+    fetch(b0);
+    for (int64_t b = b0; b < a.batch; b += each) {
+        float uf = up<T>(next_u), d = softplus_(up<T>(next_dt) + bias), zf = up<T>(next_z), x = d * uf, o = 0;
+        h = next;
+        if (b + each < a.batch) fetch(b + each);
+        bool first = a.reset != nullptr && a.reset[b * a.reset_batch] != 0;
+        const raw *Bp = (const raw *)B + b * B_batch, *Cp = (const raw *)C + b * C_batch;
+        float *to = a.last + (b * a.width + e) * a.states;
+        if constexpr (Q > 0) {
+            Vec<T, W> Bv = load<T, W>(Bp + q * 4), Cv = load<T, W>(Cp + q * 4);
+#pragma unroll
+            for (int i = 0; i < W; i++) {
+                float keep = first ? 0.0f : exp2_(d * A2.v[i]) * h.v[i];
+                h.v[i] = __builtin_fmaf(x, up<T>(Bv.v[i]), keep);
+                o = __builtin_fmaf(up<T>(Cv.v[i]), h.v[i], o);
+            }
+            store<F32, W>(to + q * 4, h);
+            o = lane_sum<Q>(o);
+        } else {
+            const float *from = a.state + (b * a.width + e) * a.states;
+            for (int n = 0; n < a.states; n++) {
+                float keep = first ? 0.0f : exp2_(d * (A[n] * kLog2e)) * from[n];
+                float hn = __builtin_fmaf(x, up<T>(Bp[n]), keep);
+                o = __builtin_fmaf(up<T>(Cp[n]), hn, o);
+                to[n] = hn;
+            }
         }
-        ((raw *)a.y)[row] = down<T>(o);
+        if (q == 0) {
+            o = __builtin_fmaf(D, uf, o);
+            if (a.z != nullptr) o *= zf * sigmoid_(zf);
+            ((raw *)a.y)[b * a.width + e] = down<T>(o);
+        }
     }
 }
 
@@ -770,8 +772,9 @@ static void scan_run(const mws_scan_args *a, const ScanPlan &p, const ScanArgs &
 }
 template <class T> static void step_go(const mws_scan_args *a, const ScanArgs &d, hipStream_t stream) {
     int q = a->states == 4 ? 1 : a->states == 8 ? 2 : a->states == 16 ? 4 : a->states == 32 ? 8 : 0;
-    dim3 grid((unsigned)ceil_div(d.batch * d.width * (q > 0 ? q : 1), 256));
-#define MWS_GO(Q) hipLaunchKernelGGL((scan_step<T, Q>), grid, dim3(256), 0, stream, d, a->B, a->C, a->B_batch, a->C_batch)
+    int64_t lanes = (int64_t)d.width * (q > 0 ? q : 1), each = step_lanes(d.batch, lanes, kStepRows);
+    dim3 grid((unsigned)ceil_div(each * lanes, 256));
+#define MWS_GO(Q) hipLaunchKernelGGL((scan_step<T, Q>), grid, dim3(256), 0, stream, d, a->B, a->C, a->B_batch, a->C_batch, each)
     if (q == 1) MWS_GO(1);
     else if (q == 2) MWS_GO(2);
     else if (q == 4) MWS_GO(4);
