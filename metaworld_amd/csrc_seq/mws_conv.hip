@@ -60,104 +60,117 @@ template <class T, int V> struct Chan {
 
 // a lane's V x K weights lie next to each other
 template <class T, int V, int K> __device__ __forceinline__ void taps(const ConvArgs &a, int e, Chan<T, V> (&w)[K], Chan<T, V> &b) {
-    if (e + V <= a.width) {
-        if (a.wide) {
-            Vec<F32, V * K> r = load<F32, V * K>((const float *)a.weight + (int64_t)e * K);
+    if (a.wide) {
+        Vec<F32, V * K> r = load<F32, V * K>((const float *)a.weight + (int64_t)e * K);
 #pragma unroll
-            for (int i = 0; i < V * K; i++) w[i % K].v[i / K] = r.v[i];
-        } else {
-            Vec<T, V * K> r = load<T, V * K>((const typename T::raw *)a.weight + (int64_t)e * K);
+        for (int i = 0; i < V * K; i++) w[i % K].v[i / K] = r.v[i];
+    } else {
+        Vec<T, V * K> r = load<T, V * K>((const typename T::raw *)a.weight + (int64_t)e * K);
 #pragma unroll
-            for (int i = 0; i < V * K; i++) w[i % K].v[i / K] = up<T>(r.v[i]);
-        }
-    } else
+        for (int i = 0; i < V * K; i++) w[i % K].v[i / K] = up<T>(r.v[i]);
+    }
 #pragma unroll
-        for (int i = 0; i < V; i++)
-#pragma unroll
-            for (int j = 0; j < K; j++) w[j].v[i] = e + i < a.width ? param<T>(a.weight, (int64_t)(e + i) * K + j, a.wide) : 0.0f;
-#pragma unroll
-    for (int i = 0; i < V; i++) b.v[i] = e + i < a.width && a.bias != nullptr ? param<T>(a.bias, e + i, a.wide) : 0.0f;
+    for (int i = 0; i < V; i++) b.v[i] = a.bias != nullptr ? param<T>(a.bias, e + i, a.wide) : 0.0f;
 }
 
 // the input at token p of row b (p >= -(K - 1); below zero: the state)
-template <class T, int V, int K> __device__ __forceinline__ Vec<T, V> input(const ConvArgs &a, int64_t b, int64_t p, int e, int n) {
+template <class T, int V, int K> __device__ __forceinline__ Vec<T, V> input(const ConvArgs &a, int64_t b, int64_t p, int e) {
     using raw = typename T::raw;
-    if (p >= 0) return load_some<T, V>((const raw *)a.x + b * a.x_batch + p * a.x_time + e, n);
-    if (a.state != nullptr) return load_some<T, V>((const raw *)a.state + (b * (K - 1) + p + K - 1) * a.width + e, n);
+    if (p >= 0) return load<T, V>((const raw *)a.x + b * a.x_batch + p * a.x_time + e);
+    if (a.state != nullptr) return load<T, V>((const raw *)a.state + (b * (K - 1) + p + K - 1) * a.width + e);
     Vec<T, V> r;
 #pragma unroll
     for (int i = 0; i < V; i++) r.v[i] = 0;
     return r;
 }
 
+// A lane's channels.  Where the width is no multiple of V the last lane steps back to V whole ones: it makes some values a second time,
+// the same ones, and every access stays whole.  (Not where the state is updated in place.)
+template <int V> struct Mine {
+    int e;
+    bool on;
+    __device__ __forceinline__ Mine(int lane_of_row, int width) : e(lane_of_row * V), on(e < width) { e = e + V <= width ? e : width - V; }
+};
+
 template <class T, int V, int K> __global__ __launch_bounds__(256) void conv_forward(ConvArgs a) {
     using raw = typename T::raw;
-    int lane = threadIdx.x % kWave, e = (blockIdx.y * kWave + lane) * V, n = a.width - e;
+    const Mine<V> m(blockIdx.y * kWave + threadIdx.x % kWave, a.width);
     int64_t item = (int64_t)blockIdx.x * (blockDim.x / kWave) + uniform(threadIdx.x / kWave);
     if (item >= a.batch * a.tiles) return;
     int64_t b = item / a.tiles, t0 = (item % a.tiles) * a.tile, t1 = t0 + a.tile < a.length ? t0 + a.tile : a.length;
     int64_t end = row_length(a.lengths, b, a.length), stop = t1 < end ? t1 : end;
-    if (n <= 0) e = 0;
     Chan<T, V> w[K], bias, x[K];
-    taps<T, V, K>(a, e, w, bias);
-    raw *y = (raw *)a.y + (b * a.length) * a.width + e;
+    taps<T, V, K>(a, m.e, w, bias);
+    raw *y = (raw *)a.y + (b * a.length + t0) * a.width + m.e;
     // bit i: token t0 - (K - 1) + i
     uint64_t begins = reset_mask(a.reset, b * a.reset_batch, a.reset_time, t0 - (K - 1), a.tile + K - 1, end);
-    if (t0 < stop) {
+    int count = (int)(stop > t0 ? stop - t0 : 0);
+    if (count > 0) {
         x[0].zero();
 #pragma unroll
         for (int j = 1; j < K; j++) {
-            x[j].set(input<T, V, K>(a, b, t0 - K + j, e, n));
+            x[j].set(input<T, V, K>(a, b, t0 - K + j, m.e));
             if (begins >> (j - 1) & 1)
 #pragma unroll
                 for (int i = 0; i < j; i++) x[i].zero();
         }
         begins >>= K - 1;
-        // four tokens at a time, the next four under way meanwhile
-        const raw *from = (const raw *)a.x + b * a.x_batch + e;
-        Vec<T, V> in[4], next[4];
+        const raw *from = (const raw *)a.x + b * a.x_batch + t0 * a.x_time + m.e;
+        auto token = [&](const Vec<T, V> &in, bool first) __attribute__((always_inline)) {
 #pragma unroll
-        for (int q = 0; q < 4; q++) next[q] = load_some<T, V>(from + (t0 + q < stop ? t0 + q : stop - 1) * a.x_time, n);
-        for (int64_t t = t0; t < stop; t += 4) {
+            for (int j = 0; j + 1 < K; j++) x[j] = x[j + 1];
+            if (first)
 #pragma unroll
-            for (int q = 0; q < 4; q++) in[q] = next[q];
-            if (t + 4 < stop)
+                for (int j = 0; j + 1 < K; j++) x[j].zero();
+            x[K - 1].set(in);
+            Chan<T, V> s = bias;
 #pragma unroll
-                for (int q = 0; q < 4; q++) next[q] = load_some<T, V>(from + (t + 4 + q < stop ? t + 4 + q : stop - 1) * a.x_time, n);
+            for (int i = 0; i < V; i++) {
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                if (t + q >= stop) break;
-#pragma unroll
-                for (int j = 0; j + 1 < K; j++) x[j] = x[j + 1];
-                if (begins >> q & 1)
-#pragma unroll
-                    for (int j = 0; j + 1 < K; j++) x[j].zero();
-                x[K - 1].set(in[q]);
-                Chan<T, V> s = bias;
-#pragma unroll
-                for (int i = 0; i < V; i++) {
-#pragma unroll
-                    for (int j = 0; j < K; j++) s.v[i] += w[j].v[i] * x[j].v[i];
-                    s.v[i] *= sigmoid_(s.v[i]);
-                }
-                if (n > 0) store_some<T, V>(y + (t + q) * a.width, s.rounded(), n);
+                for (int j = 0; j < K; j++) s.v[i] += w[j].v[i] * x[j].v[i];
+                s.v[i] *= sigmoid_(s.v[i]);
             }
-            begins >>= 4;
+            if (m.on) store<T, V>(y, s.rounded());
+            y += a.width;
+        };
+        // four tokens at a time, the next four under way meanwhile
+        Vec<T, V> next[4];
+        int i = 0;
+        if (count >= 4) {
+#pragma unroll
+            for (int q = 0; q < 4; q++) next[q] = load<T, V>(from + q * a.x_time);
+            for (; i + 4 <= count; i += 4) {
+                Vec<T, V> in[4];
+#pragma unroll
+                for (int q = 0; q < 4; q++) in[q] = next[q];
+                from += 4 * a.x_time;
+                if (i + 8 <= count)
+#pragma unroll
+                    for (int q = 0; q < 4; q++) next[q] = load<T, V>(from + q * a.x_time);
+#pragma unroll
+                for (int q = 0; q < 4; q++) token(in[q], begins >> q & 1);
+                begins >>= 4;
+            }
+        }
+        for (; i < count; i++) {
+            token(load<T, V>(from), begins & 1);
+            from += a.x_time, begins >>= 1;
         }
     }
     Vec<T, V> none;
 #pragma unroll
     for (int i = 0; i < V; i++) none.v[i] = 0;
+    y = (raw *)a.y + b * a.length * a.width + m.e;
     for (int64_t t = t0 > end ? t0 : end; t < t1; t++)
-        if (n > 0) store_some<T, V>(y + t * a.width, none, n);
+        if (m.on) store<T, V>(y + t * a.width, none);
     // the state after the last token: the inputs of its episode among the last K - 1, by the tile that holds this token
     if (a.last != nullptr && t0 == (end > 0 ? (end - 1) / a.tile : 0) * a.tile) {
         uint64_t tail = reset_mask(a.reset, b * a.reset_batch, a.reset_time, end - (K - 1), K - 1, end);
 #pragma unroll
         for (int j = 0; j + 1 < K; j++) {
             bool seen = (tail >> (j + 1)) == 0;          // none begins after token end - (K - 1) + j
-            Vec<T, V> r = seen ? input<T, V, K>(a, b, end - (K - 1) + j, e, n) : none;
-            if (n > 0) store_some<T, V>((raw *)a.last + (b * (K - 1) + j) * a.width + e, r, n);
+            Vec<T, V> r = seen ? input<T, V, K>(a, b, end - (K - 1) + j, m.e) : none;
+            if (m.on) store<T, V>((raw *)a.last + (b * (K - 1) + j) * a.width + m.e, r);
         }
     }
 }
@@ -166,10 +179,11 @@ template <class T, int V, int K> __global__ __launch_bounds__(256) void conv_for
 // terms come from the tokens past the tile.  The state's K - 1 inputs count as tokens before the first.
 template <class T, int V, int K> __global__ __launch_bounds__(256) void conv_backward(ConvArgs a) {
     using raw = typename T::raw;
-    int lane = threadIdx.x % kWave, e = (blockIdx.y * kWave + lane) * V, n = a.width - e, wave = uniform(threadIdx.x / kWave), waves = blockDim.x / kWave;
-    if (n <= 0) e = 0;
+    int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), waves = blockDim.x / kWave;
+    const Mine<V> m(blockIdx.y * kWave + lane, a.width);
+    const bool put_dx = m.on && a.dx != nullptr, put_state = m.on && a.dstate != nullptr;
     Chan<T, V> w[K], bias, dw[K], db;
-    taps<T, V, K>(a, e, w, bias);
+    taps<T, V, K>(a, m.e, w, bias);
 #pragma unroll
     for (int j = 0; j < K; j++) dw[j].zero();
     db.zero();
@@ -177,33 +191,17 @@ template <class T, int V, int K> __global__ __launch_bounds__(256) void conv_bac
         int64_t b = item / a.tiles, t0 = (item % a.tiles) * a.tile, t1 = t0 + a.tile < a.length ? t0 + a.tile : a.length;
         int64_t end = row_length(a.lengths, b, a.length), stop = t1 + K - 1 < end ? t1 + K - 1 : end, own = t1 < end ? t1 : end;
         uint64_t begins = reset_mask(a.reset, b * a.reset_batch, a.reset_time, t0 - (K - 1), a.tile + 2 * (K - 1), end);
-        uint64_t tail = reset_mask(a.reset, b * a.reset_batch, a.reset_time, end - (K - 1), K - 1, end);
         Chan<T, V> x[K], pend[K];
         x[0].zero();
 #pragma unroll
         for (int j = 0; j < K; j++) pend[j].zero();
-        int age = K;                                     // tokens since the episode's first
-        raw *dx = (raw *)a.dx + b * a.length * a.width + e, *dstate = (raw *)a.dstate + b * (K - 1) * a.width + e;
-        // dx of token p, whose terms are complete: those of the tokens, and of the state that the row leaves
-        auto emit = [&](int64_t p, Chan<T, V> v) __attribute__((always_inline)) {
-            if (p >= t1 || (p < t0 && t0 > 0)) return;
-            int64_t j = p - (end - (K - 1));
-            if (a.dlast != nullptr && j >= 0 && j < K - 1 && (tail >> (j + 1)) == 0) {
-                Chan<T, V> d;
-                d.set(load_some<T, V>((const raw *)a.dlast + (b * (K - 1) + j) * a.width + e, n));
-#pragma unroll
-                for (int i = 0; i < V; i++) v.v[i] += d.v[i];
-            }
-            if (n <= 0) return;
-            if (p >= 0) {
-                if (a.dx != nullptr) store_some<T, V>(dx + p * a.width, v.rounded(), n);
-            } else if (a.dstate != nullptr) store_some<T, V>(dstate + (p + K - 1) * a.width, v.rounded(), n);
-        };
-        int64_t t = t0;
-        if (t0 < end) {
+        int age = K;                                     // tokens since the episode's first, K at most
+        raw *dx = (raw *)a.dx + (b * a.length + t0) * a.width + m.e, *dstate = (raw *)a.dstate + b * (K - 1) * a.width + m.e;
+        int count = (int)(stop > t0 ? stop - t0 : 0), mine = (int)(own > t0 ? own - t0 : 0);
+        if (count > 0) {
 #pragma unroll
             for (int j = 1; j < K; j++) {
-                x[j].set(input<T, V, K>(a, b, t0 - K + j, e, n));
+                x[j].set(input<T, V, K>(a, b, t0 - K + j, m.e));
                 if (begins >> (j - 1) & 1) {
                     age = K - 1 - j;
 #pragma unroll
@@ -211,73 +209,90 @@ template <class T, int V, int K> __global__ __launch_bounds__(256) void conv_bac
                 }
             }
             begins >>= K - 1;
-            const raw *dyp = (const raw *)a.dy + b * a.dy_batch + e, *xp = (const raw *)a.x + b * a.x_batch + e;
-            Vec<T, V> in[4], out[4], next_in[4], next_out[4];
-            auto fetch = [&](int64_t from) __attribute__((always_inline)) {
+            const raw *dyp = (const raw *)a.dy + b * a.dy_batch + t0 * a.dy_time + m.e, *xp = (const raw *)a.x + b * a.x_batch + t0 * a.x_time + m.e;
+            auto token = [&](const Vec<T, V> &in, const Vec<T, V> &out, bool first, bool here, int p) __attribute__((always_inline)) {
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    int64_t p = from + q < stop ? from + q : stop - 1;
-                    next_in[q] = load_some<T, V>(xp + p * a.x_time, n);
-                    next_out[q] = load_some<T, V>(dyp + p * a.dy_time, n);
+                for (int j = 0; j + 1 < K; j++) x[j] = x[j + 1];
+                age = age < K ? age + 1 : K;
+                if (first) {
+                    age = 0;
+#pragma unroll
+                    for (int j = 0; j + 1 < K; j++) x[j].zero();
                 }
-            };
-            fetch(t0);
-            while (t < stop) {
+                x[K - 1].set(in);
+                Chan<T, V> s = bias, d;
+                d.set(out);
 #pragma unroll
-                for (int q = 0; q < 4; q++) in[q] = next_in[q], out[q] = next_out[q];
-                if (t + 4 < stop) fetch(t + 4);
+                for (int i = 0; i < V; i++) {
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    if (t >= stop) break;
+                    for (int j = 0; j < K; j++) s.v[i] += w[j].v[i] * x[j].v[i];
+                    float sig = sigmoid_(s.v[i]);
+                    d.v[i] *= sig * (1.0f + s.v[i] * (1.0f - sig));
+                }
 #pragma unroll
-                    for (int j = 0; j + 1 < K; j++) x[j] = x[j + 1];
-                    age = age < K ? age + 1 : K;
-                    if (begins & 1) {
-                        age = 0;
+                for (int j = 0; j + 1 < K; j++)
+                    if (age >= K - 1 || K - 1 - j <= age)
 #pragma unroll
-                        for (int j = 0; j + 1 < K; j++) x[j].zero();
-                    }
-                    begins >>= 1;
-                    x[K - 1].set(in[q]);
-                    Chan<T, V> s = bias, d;
-                    d.set(out[q]);
+                        for (int i = 0; i < V; i++) pend[j].v[i] += w[j].v[i] * d.v[i];
+#pragma unroll
+                for (int i = 0; i < V; i++) pend[K - 1].v[i] = w[K - 1].v[i] * d.v[i];
+                if (here)
 #pragma unroll
                     for (int i = 0; i < V; i++) {
+                        db.v[i] += d.v[i];
 #pragma unroll
-                        for (int j = 0; j < K; j++) s.v[i] += w[j].v[i] * x[j].v[i];
-                        float sig = sigmoid_(s.v[i]);
-                        d.v[i] *= sig * (1.0f + s.v[i] * (1.0f - sig));
+                        for (int j = 0; j < K; j++) dw[j].v[i] += d.v[i] * x[j].v[i];
                     }
+                // added up here: the compiler would put the sums off to where they are next asked for and keep their terms instead
 #pragma unroll
-                    for (int j = 0; j < K; j++)
-                        if (K - 1 - j <= age)
+                for (int i = 0; i < V; i++) {
+                    asm volatile("" : "+v"(db.v[i]));
 #pragma unroll
-                            for (int i = 0; i < V; i++) pend[j].v[i] += w[j].v[i] * d.v[i];
-                    if (t < own) {
-#pragma unroll
-                        for (int i = 0; i < V; i++) {
-                            db.v[i] += d.v[i];
-#pragma unroll
-                            for (int j = 0; j < K; j++) dw[j].v[i] += d.v[i] * x[j].v[i];
-                        }
-                    }
-                    emit(t - (K - 1), pend[0]);
-#pragma unroll
-                    for (int j = 0; j + 1 < K; j++) pend[j] = pend[j + 1];
-                    pend[K - 1].zero();
-                    t++;
+                    for (int j = 0; j < K; j++) asm volatile("" : "+v"(dw[j].v[i]), "+v"(pend[j].v[i]));
                 }
+                // token p has its last term (it is not among the row's last K - 1, which the state that the row leaves reaches)
+                if (p >= 0) {
+                    if (put_dx) store<T, V>(dx + (int64_t)p * a.width, pend[0].rounded());
+                } else if (t0 == 0 && put_state) store<T, V>(dstate + (int64_t)(p + K - 1) * a.width, pend[0].rounded());
+#pragma unroll
+                for (int j = 0; j + 1 < K; j++) pend[j] = pend[j + 1];
+            };
+            int i = 0;
+            for (; i + 4 <= mine; i += 4) {
+                Vec<T, V> in[4], out[4];
+#pragma unroll
+                for (int q = 0; q < 4; q++) in[q] = load<T, V>(xp + q * a.x_time), out[q] = load<T, V>(dyp + q * a.dy_time);
+#pragma unroll
+                for (int q = 0; q < 4; q++) token(in[q], out[q], begins >> q & 1, true, i + q - (K - 1));
+                begins >>= 4, xp += 4 * a.x_time, dyp += 4 * a.dy_time;
+            }
+            for (; i < count; i++) {
+                token(load<T, V>(xp), load<T, V>(dyp), begins & 1, i < mine, i - (K - 1));
+                begins >>= 1, xp += a.x_time, dyp += a.dy_time;
             }
         }
-        // tokens t - (K - 1) .. t - 1 wait for no further term (t: the row's end, K - 1 past the tile, or its first token where the row ended before)
-        if (t0 < end || t0 == 0)
+        // the K - 1 tokens before the end of the walk, where that is the row's: past the tile they are another wave's
+        if (t0 + count == end && (count > 0 || t0 == 0)) {
+            uint64_t tail = reset_mask(a.reset, b * a.reset_batch, a.reset_time, end - (K - 1), K - 1, end);
 #pragma unroll
-            for (int j = 0; j + 1 < K; j++)
-                if (t - (K - 1) + j < end) emit(t - (K - 1) + j, pend[j]);
+            for (int j = 0; j + 1 < K; j++) {
+                int p = count - (K - 1) + j;
+                if (t0 + p >= t1 || (p < 0 && t0 > 0)) continue;
+                if (a.dlast != nullptr && (tail >> (j + 1)) == 0) {
+                    Chan<T, V> d;
+                    d.set(load<T, V>((const raw *)a.dlast + (b * (K - 1) + j) * a.width + m.e));
+#pragma unroll
+                    for (int i = 0; i < V; i++) pend[j].v[i] += d.v[i];
+                }
+                if (p >= 0) {
+                    if (put_dx) store<T, V>(dx + (int64_t)p * a.width, pend[j].rounded());
+                } else if (put_state) store<T, V>(dstate + (int64_t)(p + K - 1) * a.width, pend[j].rounded());
+            }
+        }
         Chan<T, V> none;
         none.zero();
-        if (a.dx != nullptr && n > 0)
-            for (int64_t p = t0 > end ? t0 : end; p < t1; p++) store_some<T, V>(dx + p * a.width, none.rounded(), n);
+        if (put_dx)
+            for (int64_t t = t0 > end ? t0 : end; t < t1; t++) store<T, V>(dx + (t - t0) * a.width, none.rounded());
     }
     if (a.part == nullptr) return;
     __shared__ float meet[4][kWave];
@@ -289,10 +304,10 @@ template <class T, int V, int K> __global__ __launch_bounds__(256) void conv_bac
             __syncthreads();
             meet[wave][lane] = j < K ? dw[j < K ? j : 0].v[i] : db.v[i];
             __syncthreads();
-            if (wave == 0 && i < n) {
+            if (wave == 0 && m.on) {
                 float s = 0;
                 for (int k = 0; k < waves; k++) s += meet[k][lane];
-                part[(int64_t)j * a.width + e + i] = s;
+                part[(int64_t)j * a.width + m.e + i] = s;
             }
         }
 }
@@ -304,7 +319,7 @@ template <class T, int V, int K> __global__ __launch_bounds__(256) void conv_ste
     using raw = typename T::raw;
     int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (at >= each * groups) return;
-    int e = (int)(at % groups) * V, n = a.width - e;
+    const int e = (int)(at % groups) * V;                 // V divides the width
     int64_t b0 = at / groups;                             // rows b0, b0 + each, ..
     Chan<T, V> w[K], bias;
     taps<T, V, K>(a, e, w, bias);
@@ -312,7 +327,7 @@ template <class T, int V, int K> __global__ __launch_bounds__(256) void conv_ste
     bool next_first = false;
     auto fetch = [&](int64_t b) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < K; j++) next[j] = input<T, V, K>(a, b, j - (K - 1), e, n);
+        for (int j = 0; j < K; j++) next[j] = input<T, V, K>(a, b, j - (K - 1), e);
         next_first = a.reset != nullptr && a.reset[b * a.reset_batch] != 0;
     };
     fetch(b0);
@@ -332,9 +347,9 @@ template <class T, int V, int K> __global__ __launch_bounds__(256) void conv_ste
             }
 #pragma unroll
         for (int i = 0; i < V; i++) s.v[i] *= sigmoid_(s.v[i]);
-        store_some<T, V>((raw *)a.y + b * a.width + e, s.rounded(), n);
+        store<T, V>((raw *)a.y + b * a.width + e, s.rounded());
 #pragma unroll
-        for (int j = 0; j + 1 < K; j++) store_some<T, V>((raw *)a.last + (b * (K - 1) + j) * a.width + e, in[j + 1], n);
+        for (int j = 0; j + 1 < K; j++) store<T, V>((raw *)a.last + (b * (K - 1) + j) * a.width + e, in[j + 1]);
     }
 }
 
@@ -353,9 +368,16 @@ struct ConvOut {
     }
 };
 
-// A tile of 32 tokens re-reads K - 1 of its neighbour's; where that leaves less than four waves to a SIMD, tiles get shorter.
-static int conv_v(const mws_conv_args *a) { return a->type == MWS_F32 ? 4 : 8; }
-constexpr int kBackV = 4;          // channels of a lane backward: with eight the weights, inputs, sums and gradients of K taps take 211 registers
+// Channels of a lane: one 16-byte access, or one value where the row is narrower than that (or, where the state is updated in place,
+// no multiple of it).  A tile of 32 tokens re-reads K - 1 of its neighbour's; where that leaves less than four waves to a SIMD, tiles
+// get shorter.
+static int conv_v(const mws_conv_args *a) {
+    int v = a->type == MWS_F32 ? 4 : 8;
+    return a->width >= v ? v : 1;
+}
+// backward four of any type: with eight the weights, inputs, sums and gradients of the taps leave two waves to a SIMD (512 x 128 x 1024
+// bf16 102 us, with eight 118 us)
+static int conv_back_v(const mws_conv_args *a) { return a->width >= 4 ? 4 : 1; }
 static int conv_tile(const mws_conv_args *a) {
     int64_t across = a->batch * ceil_div(a->width, kWave * conv_v(a));
     int tile = kMostTile;
@@ -365,7 +387,7 @@ static int conv_tile(const mws_conv_args *a) {
 static int64_t conv_tiles(const mws_conv_args *a) { return a->length > 0 ? ceil_div(a->length, conv_tile(a)) : 1; }
 // backward: each block's partial sums are K + 1 values a channel; two blocks to a compute unit, over the channels' groups
 static int64_t conv_blocks(const mws_conv_args *a) {
-    int64_t need = ceil_div(a->batch * conv_tiles(a), 4), groups = ceil_div(a->width, kWave * kBackV);
+    int64_t need = ceil_div(a->batch * conv_tiles(a), 4), groups = ceil_div(a->width, kWave * conv_back_v(a));
     int64_t most = groups < 16 ? 1024 / groups : 64;
     return need < most ? need : most;
 }
@@ -402,9 +424,13 @@ static ConvArgs conv_device(const mws_conv_args *a) {
 enum { kForward, kBackward, kStep };
 template <class T, int V, int K> static void conv_go(const mws_conv_args *a, const ConvArgs &d, int what, hipStream_t stream) {
     unsigned groups = (unsigned)ceil_div(a->width, kWave * V);
+    if constexpr (V <= 4) {
+        if (what == kBackward) {
+            hipLaunchKernelGGL((conv_backward<T, V, K>), dim3((unsigned)conv_blocks(a), groups), dim3(256), 0, stream, d);
+            return;
+        }
+    }
     if (what == kForward) hipLaunchKernelGGL((conv_forward<T, V, K>), dim3((unsigned)ceil_div(d.batch * d.tiles, 4), groups), dim3(256), 0, stream, d);
-    else if (what == kBackward)
-        hipLaunchKernelGGL((conv_backward<T, kBackV, K>), dim3((unsigned)conv_blocks(a), (unsigned)ceil_div(a->width, kWave * kBackV)), dim3(256), 0, stream, d);
     else {
         int64_t across = ceil_div(a->width, V), each = step_lanes(d.batch, across, kStepRows);
         hipLaunchKernelGGL((conv_step<T, V, K>), dim3((unsigned)ceil_div(each * across, 256)), dim3(256), 0, stream, d, across, each);
@@ -415,10 +441,17 @@ template <class T, int V> static void conv_taps(const mws_conv_args *a, const Co
     else if (a->taps == 3) conv_go<T, V, 3>(a, d, what, stream);
     else conv_go<T, V, 4>(a, d, what, stream);
 }
+template <class T, int V> static void conv_width(const mws_conv_args *a, const ConvArgs &d, int what, hipStream_t stream) {
+    if (what == kBackward) {
+        if (a->width >= 4) conv_taps<T, 4>(a, d, what, stream);
+        else conv_taps<T, 1>(a, d, what, stream);
+    } else if (what == kStep ? a->width % V == 0 : a->width >= V) conv_taps<T, V>(a, d, what, stream);
+    else conv_taps<T, 1>(a, d, what, stream);
+}
 static void conv_run(const mws_conv_args *a, const ConvArgs &d, int what, hipStream_t stream) {
-    if (a->type == MWS_F32) conv_taps<F32, 4>(a, d, what, stream);
-    else if (a->type == MWS_BF16) conv_taps<BF16, 8>(a, d, what, stream);
-    else conv_taps<F16, 8>(a, d, what, stream);
+    if (a->type == MWS_F32) conv_width<F32, 4>(a, d, what, stream);
+    else if (a->type == MWS_BF16) conv_width<BF16, 8>(a, d, what, stream);
+    else conv_width<F16, 8>(a, d, what, stream);
 }
 }  // namespace mws
 
