@@ -65,6 +65,15 @@ template <class R> struct Line {
     }
 };
 
+// The kernel's arguments as they lie in memory, to be read where they are needed: held in registers from the kernel's start on they
+// would not fit the scalar registers beside a token's B and C.
+using FixedArgs = const __attribute__((address_space(4))) ScanArgs;
+__device__ __forceinline__ FixedArgs *fresh_args() {
+    FixedArgs *k = (FixedArgs *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(k));
+    return k;
+}
+
 __device__ __forceinline__ int64_t row_length(const int32_t *lengths, int64_t b, int64_t length) {
     if (lengths == nullptr) return length;
     int64_t n = lengths[b];
@@ -80,22 +89,29 @@ __device__ __forceinline__ float softplus_(float x) {
 }
 
 // bit i: an episode begins at token t0 + i of the group
-__device__ __forceinline__ uint32_t group_mask(const ScanArgs &a, int64_t b, int64_t t0, int64_t end) {
+template <class Args> __device__ __forceinline__ uint32_t group_mask(const Args &a, int64_t b, int64_t t0, int64_t end) {
     if (a.reset == nullptr) return 0;
     int lane = threadIdx.x % kWave;
     int64_t t = t0 + lane;
     return (uint32_t)__ballot(lane < kGroup && t < end && a.reset[b * a.reset_batch + t * a.reset_time] != 0);
 }
 
-// ---- B and C in float, padded with zeros to NS states ----
-template <class T> __global__ __launch_bounds__(256) void spread(const void *B, const void *C, float *bc, int64_t length, int64_t B_batch, int64_t B_time, int64_t C_batch,
-                                                                  int64_t C_time, int states, int ns, int64_t count) {
-    int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (at >= count) return;
-    int n = (int)(at % ns);
-    int64_t rest = at / ns, token = rest >> 1, b = token / length, t = token % length;
-    const typename T::raw *from = (const typename T::raw *)(rest & 1 ? C : B) + (rest & 1 ? b * C_batch + t * C_time : b * B_batch + t * B_time);
-    bc[at] = n < states ? up<T>(from[n]) : 0.0f;
+// ---- B and C in float, padded with zeros to NS states: a thread takes four of them ----
+template <class T, int NS> __global__ __launch_bounds__(256) void spread(const void *B, const void *C, float *bc, int64_t batch, int64_t length, int64_t B_batch, int64_t B_time, int64_t C_batch,
+                                                                         int64_t C_time, int states) {
+    constexpr int kOf = 2 * NS / 4;                   // threads of a token
+    int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, t = i / kOf;
+    if (t >= length) return;
+    int at = (int)(i % kOf) * 4;
+    const bool second = at >= NS;
+    const int n = second ? at - NS : at;
+    for (int64_t b = blockIdx.y; b < batch; b += gridDim.y) {
+        const typename T::raw *from = (const typename T::raw *)(second ? C : B) + (second ? b * C_batch + t * C_time : b * B_batch + t * B_time) + n;
+        Vec<F32, 4> v;
+#pragma unroll
+        for (int k = 0; k < 4; k++) v.v[k] = n + k < states ? up<T>(from[k]) : 0.0f;
+        store<F32, 4>(bc + ((b * length + t) * 2 * NS + at), v);
+    }
 }
 
 // one token's B and C: the address is the same for the wave and nothing of this kernel writes there, which the constant address
@@ -132,7 +148,7 @@ template <int NS> __device__ __forceinline__ void put_row(float *p, int64_t row,
     for (int n = 0; n < NS; n++) (p + (row * NS + n) * a.width)[e] = h[n];
 }
 
-template <int NS> __device__ __forceinline__ void kept_row(const ScanArgs &a, int64_t row, uint32_t bytes, float (&h)[NS]) {
+template <int NS, class Args> __device__ __forceinline__ void kept_row(const Args &a, int64_t row, uint32_t bytes, float (&h)[NS]) {
 #pragma unroll
     for (int n = 0; n < NS; n++) h[n] = Line<float>(a.kept, (row * NS + n) * a.width, 0).get(bytes);
 }
@@ -143,7 +159,7 @@ struct Place {          // what a block of the grid works on
     int at, seg;
     bool on;
     __device__ __forceinline__ uint32_t bytes(int size) const { return on ? (uint32_t)at * (uint32_t)size : kOutside; }
-    __device__ __forceinline__ Place(const ScanArgs &a, int64_t item, int part) {
+    template <class Args> __device__ __forceinline__ Place(const Args &a, int64_t item, int part) {
         at = part * (int)blockDim.x + (int)threadIdx.x;
         on = at < a.width;
         e = on ? at : a.width - 1;
@@ -228,7 +244,8 @@ template <class T, int NS> __global__ __launch_bounds__(256) void scan_segment(S
     using raw = typename T::raw;
     constexpr int G = 4, kChunk = kGroup;
     Place p(a, blockIdx.x / a.across, blockIdx.x % a.across);
-    int64_t stop = p.t1 < p.end ? p.t1 : p.end;
+    if (p.end <= p.t1) return;           // the row's last segment leaves the row's last state, which scan_forward writes
+    int64_t stop = p.t1;
     float h[NS], A2[NS], sum = 0;
     rates<NS>(a, p.e, A2);
 #pragma unroll
@@ -276,6 +293,7 @@ template <class T, int NS> __global__ __launch_bounds__(256) void scan_segment_b
     using raw = typename T::raw;
     constexpr int kChunk = kGroup;
     Place p(a, blockIdx.x / a.across, blockIdx.x % a.across);
+    if (p.t0 >= p.end || (p.seg == 0 && a.dstate == nullptr)) return;
     int64_t stop = p.t1 < p.end ? p.t1 : p.end;
     float g[NS], A2[NS], sum = 0;
     rates<NS>(a, p.e, A2);
@@ -326,15 +344,29 @@ __global__ __launch_bounds__(256) void scan_join(ScanArgs a, int ns, bool backwa
     float A2 = real ? a.A[(int64_t)e * a.states + n] * kLog2e : 0.0f;
     const float *from = backward ? a.dlast : a.state;
     float h = from != nullptr && real ? from[(b * a.width + e) * a.states + n] : 0.0f;
-    for (int k = 0; k <= last; k++) {
-        int s = backward ? last - k : k;
-        int64_t row = b * a.segments + s;
-        float *mine = a.seg + (row * ns + n) * a.width + e;
-        float left = *mine, sum = a.sum[row * a.width + e];
-        *mine = h;
-        h = sum < 0.0f || h == 0.0f ? left : __builtin_fmaf(exp2_(sum * A2), h, left);
+    // eight segments' values under way at a time: the chain through h does not wait for them
+    for (int k0 = 0; k0 <= last; k0 += 8) {
+        float left[8], sum[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            int k = k0 + j, s = backward ? last - k : k;
+            bool asked = k < last || (k == last && backward && a.dstate != nullptr);
+            int64_t row = b * a.segments + (asked ? s : 0);
+            left[j] = asked ? a.seg[(row * ns + n) * a.width + e] : 0.0f;
+            sum[j] = asked ? a.sum[row * a.width + e] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            int k = k0 + j, s = backward ? last - k : k;
+            if (k > last) break;
+            a.seg[((b * a.segments + s) * ns + n) * a.width + e] = h;
+            h = sum[j] < 0.0f || h == 0.0f ? left[j] : __builtin_fmaf(exp2_(sum[j] * A2), h, left[j]);
+        }
     }
-    if (backward && a.dstate != nullptr && real) a.dstate[(b * a.width + e) * a.states + n] = h;
+    if (backward && a.dstate != nullptr && real) {
+        // a row without tokens leaves what came in
+        a.dstate[(b * a.width + e) * a.states + n] = end > 0 ? h : from != nullptr ? from[(b * a.width + e) * a.states + n] : 0.0f;
+    }
 }
 
 // ---- sums of M values over the 64 lanes of a wave: every step adds one half of the lanes to the other and halves the values that
@@ -389,11 +421,9 @@ template <class T, int NS> __global__ __launch_bounds__(256, NS >= 32 ? 2 : 2) v
 #pragma unroll
     for (int n = 0; n < NS; n++) dA[n] = 0;
     for (int64_t item = group; item < a.batch * a.segments; item += a.groups) {
-        Place p(a, item, part);
+        Place p(*fresh_args(), item, part);
         int64_t stop = p.t1 < p.end ? p.t1 : p.end;
         bool whole_end = p.end <= p.t1 && (p.end > p.t0 || p.seg == 0);
-        raw *du = (raw *)a.du + p.b * a.length * a.width, *ddt = (raw *)a.ddt + p.b * a.length * a.width;
-        raw *dz = a.z != nullptr ? (raw *)a.dz + p.b * a.length * a.width : nullptr;
         const uint32_t bytes = p.bytes(sizeof(raw));
         if (p.t0 < stop || whole_end) {
             float g[NS];
@@ -403,14 +433,14 @@ template <class T, int NS> __global__ __launch_bounds__(256, NS >= 32 ? 2 : 2) v
 #pragma unroll
                 for (int n = 0; n < NS; n++) g[n] = 0;
             float D = a.D != nullptr ? a.D[p.e] : 0.0f, bias = a.dt_bias != nullptr ? a.dt_bias[p.e] : 0.0f;
-            const raw *u = (const raw *)a.u + p.b * a.u_batch, *dt = (const raw *)a.dt + p.b * a.dt_batch, *dy = (const raw *)a.dy + p.b * a.dy_batch;
-            const raw *z = a.z != nullptr ? (const raw *)a.z + p.b * a.z_batch : nullptr;
-
             // SUB tokens from t, `here` of which are the row's; bit i of `begins`: an episode begins at token t + i
             auto walk = [&](int64_t t, int here, uint32_t begins, float (&h)[NS]) __attribute__((always_inline)) {
                 float keep[SUB][NS], d[SUB], uf[SUB];
                 raw rd[SUB], early[3];
-                Line<raw> lu(u, t * a.u_time, a.u_time), ld(dt, t * a.dt_time, a.dt_time), ly(dy, t * a.dy_time, a.dy_time), lz(z, t * a.z_time, a.z_time);
+                FixedArgs *in = fresh_args();
+                Line<raw> lu((const raw *)in->u, p.b * in->u_batch + t * in->u_time, in->u_time), ld((const raw *)in->dt, p.b * in->dt_batch + t * in->dt_time, in->dt_time),
+                    ly((const raw *)in->dy, p.b * in->dy_batch + t * in->dy_time, in->dy_time), lz((const raw *)in->z, p.b * in->z_batch + t * in->z_time, in->z_time);
+                const bool gated = in->z != nullptr;
 #pragma unroll
                 for (int q = 0; q < SUB; q++) {
                     int at = q < here ? q : here - 1;
@@ -419,9 +449,10 @@ template <class T, int NS> __global__ __launch_bounds__(256, NS >= 32 ? 2 : 2) v
                     uf[q] = q < here ? up<T>(ru) : 0.0f;
                 }
                 early[0] = ld.get(bytes, here - 1), early[1] = ly.get(bytes, here - 1), early[2] = lz.get(bytes, here - 1);
-                Fixed *bc = fixed(a.bc + (p.b * a.length + t) * 2 * NS);
+                Fixed *bc = fixed(in->bc + (p.b * in->length + t) * 2 * NS);
 #pragma unroll
                 for (int q = 0; q < SUB; q++) {
+                    if (q % 2 == 0) asm volatile("" : "+s"(bc));         // two tokens' B at a time
                     Fixed *m = bc + (q < here ? q : here - 1) * 2 * NS;
                     d[q] = q < here ? softplus_(up<T>(rd[q]) + bias) : 0.0f;
                     float x = d[q] * uf[q];
@@ -444,13 +475,15 @@ template <class T, int NS> __global__ __launch_bounds__(256, NS >= 32 ? 2 : 2) v
                 for (int q = 0; q < SUB; q++) asm volatile("" : "+v"(d[q]));
                 asm volatile("" : "+s"(bc));
                 float *to = sums + (turn * waves + wave) * SUB * M;
-                Line<raw> gu(du, t * a.width, a.width), gd(ddt, t * a.width, a.width), gz(dz, t * a.width, a.width);
+                FixedArgs *out_to = fresh_args();
+                const int64_t row = (p.b * out_to->length + t) * out_to->width;
+                Line<raw> gu((raw *)out_to->du, row, out_to->width), gd((raw *)out_to->ddt, row, out_to->width), gz((raw *)out_to->dz, row, out_to->width);
 #pragma unroll
                 for (int q = SUB - 1; q >= 0; q--) {
                     Pair<NS> m;
                     m.read(bc + (q < here ? q : here - 1) * 2 * NS);
                     float raw_d = up<T>(early[0]) + bias, out = q < here ? up<T>(early[1]) : 0.0f, zf = 0, gate = 1, sig = 0;
-                    if (z != nullptr) {
+                    if (gated) {
                         zf = up<T>(early[2]);
                         sig = sigmoid_(zf);
                         gate = zf * sig;
@@ -487,7 +520,7 @@ template <class T, int NS> __global__ __launch_bounds__(256, NS >= 32 ? 2 : 2) v
                     if (q < here) {
                         gu.put(down<T>(__builtin_fmaf(D, o, d[q] * gB)), bytes, q);
                         gd.put(down<T>(draw), bytes, q);
-                        if (z != nullptr) gz.put(down<T>(out * y * sig * (1.0f + zf * (1.0f - sig))), bytes, q);
+                        if (gated) gz.put(down<T>(out * y * sig * (1.0f + zf * (1.0f - sig))), bytes, q);
                     }
                     float total = wave_sums<M>(v);
                     if (lane % (kWave / M) == 0) to[q * M + lane / (kWave / M)] = total;
@@ -496,7 +529,8 @@ template <class T, int NS> __global__ __launch_bounds__(256, NS >= 32 ? 2 : 2) v
                 // the other half of `sums` is read by nobody after this barrier, and this half is written again after the next
                 __syncthreads();
                 const float *from = sums + turn * waves * SUB * M;
-                float *bc_to = a.part_bc + ((int64_t)part * a.batch * a.length + p.b * a.length + t) * M;
+                FixedArgs *sums_to = fresh_args();
+                float *bc_to = sums_to->part_bc + (((int64_t)part * sums_to->batch + p.b) * sums_to->length + t) * M;
                 for (int k = threadIdx.x; k < here * M; k += blockDim.x) {
                     float v = 0;
                     for (int w = 0; w < waves; w++) v += from[w * SUB * M + k];
@@ -507,14 +541,16 @@ template <class T, int NS> __global__ __launch_bounds__(256, NS >= 32 ? 2 : 2) v
 
             if (p.t0 < stop)
                 for (int64_t c0 = p.t0 + (stop - 1 - p.t0) / kGroup * kGroup; c0 >= p.t0; c0 -= kGroup) {
-                    uint32_t begins = group_mask(a, p.b, c0, p.end);
+                    uint32_t begins = group_mask(*fresh_args(), p.b, c0, p.end);
                     int count = (int)(c0 + kGroup < stop ? kGroup : stop - c0);
                     for (int i = (count - 1) / KEPT * KEPT; i >= 0; i -= KEPT) {
                         float h[NS];
-                        const int64_t row = p.b * a.chunks + (c0 + i) / KEPT;
-                        kept_row<NS>(a, row, p.bytes(4), h);
+                        FixedArgs *states_of = fresh_args();
+                        const int64_t row = p.b * states_of->chunks + (c0 + i) / KEPT;
+                        kept_row<NS>(*states_of, row, p.bytes(4), h);
                         int subs = kSubs == 1 || count - i <= SUB ? 1 : (count - i < KEPT ? count - i + SUB - 1 : KEPT) / SUB;
                         if constexpr (kSubs > 1) {
+                            const raw *u = (const raw *)a.u + p.b * a.u_batch, *dt = (const raw *)a.dt + p.b * a.dt_batch;
                             for (int k = 0; k + 1 < subs; k++) {
 #pragma unroll
                                 for (int q = 0; q < SUB; q++) {
@@ -536,7 +572,7 @@ template <class T, int NS> __global__ __launch_bounds__(256, NS >= 32 ? 2 : 2) v
                                 if (k > 0)
 #pragma unroll
                                     for (int n = 0; n < NS; n++) h[n] = states[((k - 1) * NS + n) * kWave];
-                                else if (subs > 1) kept_row<NS>(a, row, p.bytes(4), h);
+                                else if (subs > 1) kept_row<NS>(*fresh_args(), row, p.bytes(4), h);
                             }
                             int from = i + k * SUB, here = count - from < SUB ? count - from : SUB;
                             walk(c0 + from, here, begins >> from, h);
@@ -545,6 +581,7 @@ template <class T, int NS> __global__ __launch_bounds__(256, NS >= 32 ? 2 : 2) v
                 }
             if (p.on && p.seg == 0 && a.segments == 1 && a.dstate != nullptr) last_state<NS>(a.dstate, a, p.b, p.e, g);
         }
+        raw *du = (raw *)a.du + p.b * a.length * a.width, *ddt = (raw *)a.ddt + p.b * a.length * a.width, *dz = a.z != nullptr ? (raw *)a.dz + p.b * a.length * a.width : nullptr;
         if (p.on)
             for (int64_t t = p.t0 > p.end ? p.t0 : p.end; t < p.t1; t++) {
                 (du + t * a.width)[p.e] = (ddt + t * a.width)[p.e] = down<T>(0.0f);
@@ -657,22 +694,47 @@ struct ScanPlan {
     int64_t bc, seg, sum, part_bc, part, bytes;      // offsets into the workspace, in floats
 };
 
-// Segments: the time axis is cut where the waves over batch and channels leave the SIMDs without two waves each; cutting doubles
-// the work (each segment is walked twice), so that it is worth it from four segments on.
+// Waves of a block: as many as leave the fewest of them without channels.
+static int block_waves(int waves, int most) {
+    int best = 1, least = waves;
+    for (int w = 2; w <= most; w++) {
+        int used = (waves + w - 1) / w * w;
+        if (used <= least || w == 1) best = w, least = used;
+    }
+    return best;
+}
+
+// Segments.  `places`: the waves that run at a time to some use, two to a SIMD backward (its registers allow no more), four forward.
+// The time is that of the rounds over the places times the tokens of a segment; cutting costs a second walk (forward 0.8 of the
+// first, backward 0.3) and joining.
+static int64_t best_span(int64_t waves, int64_t groups, bool backward) {
+    const double places = (backward ? 2 : 4) * kSimds, walks = backward ? 1.3 : 1.8;
+    auto rounds = [&](double w) {
+        double r = w / places;
+        return r <= 1 ? 1.0 : backward ? (double)(int64_t)(r + 0.999) : r;
+    };
+    int64_t best = groups;
+    double least = rounds((double)waves) * (double)groups;
+    for (int64_t s = 2; s <= groups && s <= 256; s++) {
+        int64_t each = ceil_div(groups, s), count = ceil_div(groups, each);
+        double cost = rounds((double)waves * (double)count) * (double)each * walks + 0.5 + 0.02 * (double)count;
+        if (cost < least) best = each, least = cost;
+    }
+    return best;
+}
+
 static ScanPlan scan_plan(const mws_scan_args *a, bool backward) {
     ScanPlan p = {};
     p.ns = scan_ns(a);
-    int waves = (int)ceil_div(a->width, kWave);
-    p.lanes = (waves < lanes_of(p.ns) / kWave ? waves : lanes_of(p.ns) / kWave) * kWave;
+    int waves = (int)ceil_div(a->width, kWave), of_block = block_waves(waves, lanes_of(p.ns) / kWave);
+    p.lanes = of_block * kWave;
     p.across = (int)ceil_div(a->width, p.lanes);
     p.chunks = ceil_div(a->length, kept_of(p.ns));
-    int64_t groups = ceil_div(a->length > 0 ? a->length : 1, kGroup), blocks = a->batch * p.across, wanted = ceil_div(2 * kSimds, blocks > 0 ? blocks * (p.lanes / kWave) : 1);
-    int64_t segments = wanted < groups ? wanted : groups;
-    if (segments < 4) segments = 1;
-    int64_t each = ceil_div(groups, segments);
+    int64_t groups = ceil_div(a->length > 0 ? a->length : 1, kGroup), each = best_span(a->batch * p.across * of_block, groups, backward);
     p.segments = (int)ceil_div(groups, each);
     p.span = (int)(each * kGroup);
-    int64_t items = a->batch * p.segments, most = 2048 / p.across > 0 ? 2048 / p.across : 1;
+    // blocks over the items, four rounds of the places at most: each leaves partial sums of dA, dD and ddt_bias
+    int64_t items = a->batch * p.segments, most = 8 * kSimds / ((int64_t)of_block * p.across) > 0 ? 8 * kSimds / ((int64_t)of_block * p.across) : 1;
     p.groups = (int)(items < most ? items : most);
     int64_t at = 0, tokens = a->batch * a->length;
     auto take = [&at](int64_t n) {
@@ -713,7 +775,7 @@ static ScanArgs scan_device(const mws_scan_args *a, const ScanPlan &p) {
     ScanArgs d = {};
     float *w = (float *)a->workspace;
     d.u = a->u, d.dt = a->dt, d.z = a->z, d.dy = a->dy, d.A = a->A, d.D = a->D, d.dt_bias = a->dt_bias, d.state = a->state, d.dlast = a->dlast;
-    d.reset = a->reset, d.lengths = a->lengths, d.y = a->y, d.du = a->du, d.ddt = a->ddt, d.dz = a->dz;
+    d.reset = a->reset, d.lengths = a->lengths, d.y = a->y, d.du = a->du, d.ddt = a->ddt, d.dz = a->z != nullptr ? a->dz : nullptr;
     d.last = a->last, d.kept = a->kept, d.dstate = a->dstate;
     if (w != nullptr) d.bc = w + p.bc, d.seg = w + p.seg, d.sum = w + p.sum, d.part_bc = w + p.part_bc, d.part = w + p.part;
     d.batch = a->batch, d.length = a->length, d.chunks = p.chunks;
@@ -723,17 +785,17 @@ static ScanArgs scan_device(const mws_scan_args *a, const ScanPlan &p) {
     return d;
 }
 
-template <class T> static void spread_go(const mws_scan_args *a, const ScanPlan &p, const ScanArgs &d, hipStream_t stream) {
-    int64_t count = a->batch * a->length * 2 * p.ns;
-    if (count > 0)
-        hipLaunchKernelGGL((spread<T>), dim3((unsigned)ceil_div(count, 256)), dim3(256), 0, stream, a->B, a->C, const_cast<float *>(d.bc), a->length, a->B_batch, a->B_time, a->C_batch,
-                           a->C_time, a->states, p.ns, count);
+template <class T, int NS> static void spread_go(const mws_scan_args *a, const ScanArgs &d, hipStream_t stream) {
+    if (a->batch * a->length > 0)
+        hipLaunchKernelGGL((spread<T, NS>), dim3((unsigned)ceil_div(a->length * (2 * NS / 4), 256), (unsigned)(a->batch < 32768 ? a->batch : 32768)), dim3(256), 0, stream, a->B, a->C,
+                           const_cast<float *>(d.bc), a->batch, a->length, a->B_batch, a->B_time, a->C_batch, a->C_time, a->states);
 }
 static void join_go(const ScanArgs &d, int ns, bool backward, hipStream_t stream) {
     hipLaunchKernelGGL(scan_join, dim3((unsigned)ceil_div(d.batch * ns * d.width, 256)), dim3(256), 0, stream, d, ns, backward);
 }
 
-template <class T, int NS> static void forward_go(const ScanPlan &p, const ScanArgs &d, hipStream_t stream) {
+template <class T, int NS> static void forward_go(const mws_scan_args *a, const ScanPlan &p, const ScanArgs &d, hipStream_t stream) {
+    spread_go<T, NS>(a, d, stream);
     dim3 grid((unsigned)(d.batch * p.segments * p.across)), block(p.lanes);
     if (p.segments > 1) {
         hipLaunchKernelGGL((scan_segment<T, NS>), grid, block, 0, stream, d);
@@ -744,6 +806,7 @@ template <class T, int NS> static void forward_go(const ScanPlan &p, const ScanA
 template <class T, int NS> static void backward_go(const mws_scan_args *a, const ScanPlan &p, const ScanArgs &d, hipStream_t stream) {
     constexpr int SUB = sub_of(NS);
     dim3 block(p.lanes);
+    spread_go<T, NS>(a, d, stream);
     if (p.segments > 1) {
         hipLaunchKernelGGL((scan_segment_back<T, NS>), dim3((unsigned)(d.batch * p.segments * p.across)), block, 0, stream, d);
         join_go(d, NS, true, stream);
@@ -757,8 +820,7 @@ template <class T, int NS> static void backward_go(const mws_scan_args *a, const
     launch_sum_parts(d.part, p.groups, (int64_t)(NS + 2) * a->width, out, stream);
 }
 template <class T> static void scan_go(const mws_scan_args *a, const ScanPlan &p, const ScanArgs &d, bool backward, hipStream_t stream) {
-    spread_go<T>(a, p, d, stream);
-#define MWS_GO(NS) (backward ? backward_go<T, NS>(a, p, d, stream) : forward_go<T, NS>(p, d, stream))
+#define MWS_GO(NS) (backward ? backward_go<T, NS>(a, p, d, stream) : forward_go<T, NS>(a, p, d, stream))
     if (p.ns == 4) MWS_GO(4);
     else if (p.ns == 8) MWS_GO(8);
     else if (p.ns == 16) MWS_GO(16);
