@@ -242,43 +242,40 @@ template <class T, int NS> __global__ __launch_bounds__(256) void scan_forward(S
 // a segment's end state from zero, and its sum of d
 template <class T, int NS> __global__ __launch_bounds__(256) void scan_segment(ScanArgs a) {
     using raw = typename T::raw;
-    constexpr int G = 4, kChunk = kGroup;
+    constexpr int G = 4;
     Place p(a, blockIdx.x / a.across, blockIdx.x % a.across);
     if (p.end <= p.t1) return;           // the row's last segment leaves the row's last state, which scan_forward writes
-    int64_t stop = p.t1;
+    const uint32_t bytes = p.bytes(sizeof(raw));
     float h[NS], A2[NS], sum = 0;
     rates<NS>(a, p.e, A2);
 #pragma unroll
     for (int n = 0; n < NS; n++) h[n] = 0;
     bool cut = false;
     float bias = a.dt_bias != nullptr ? a.dt_bias[p.e] : 0.0f;
-    const raw *u = (const raw *)a.u + p.b * a.u_batch, *dt = (const raw *)a.dt + p.b * a.dt_batch;
-    Fixed *bc = fixed(a.bc + p.b * a.length * 2 * NS);
-    for (int64_t c0 = p.t0; c0 < stop; c0 += kChunk) {
+    const raw *u = (const raw *)a.u + p.b * a.u_batch + p.t0 * a.u_time, *dt = (const raw *)a.dt + p.b * a.dt_batch + p.t0 * a.dt_time;
+    Fixed *bc = fixed(a.bc + (p.b * a.length + p.t0) * 2 * NS);
+    for (int64_t c0 = p.t0; c0 < p.t1; c0 += kGroup) {        // whole groups: the row goes on behind the segment
         uint32_t begins = group_mask(a, p.b, c0, p.end);
         cut = cut || begins != 0;
-        int64_t c1 = c0 + kChunk < stop ? c0 + kChunk : stop;
-        for (int64_t t = c0; t < c1; t += G) {
+        for (int i = 0; i < kGroup; i += G) {
+            Line<raw> lu(u, 0, a.u_time), ld(dt, 0, a.dt_time);
             raw ru[G], rd[G];
 #pragma unroll
-            for (int q = 0; q < G; q++) {
-                int64_t at = t + q < c1 ? t + q : c1 - 1;
-                ru[q] = (u + at * a.u_time)[p.e], rd[q] = (dt + at * a.dt_time)[p.e];
-            }
+            for (int q = 0; q < G; q++) ru[q] = lu.get(bytes, q), rd[q] = ld.get(bytes, q);
 #pragma unroll
             for (int q = 0; q < G; q++) {
-                if (t + q >= c1) break;
-                Pair<NS> m;
-                m.read(bc + (t + q) * 2 * NS);
-                float d = softplus_(up<T>(rd[q]) + bias), du = d * up<T>(ru[q]);
+                float d = softplus_(up<T>(rd[q]) + bias), x = d * up<T>(ru[q]);
                 sum += d;
                 if (begins >> q & 1)
 #pragma unroll
                     for (int n = 0; n < NS; n++) h[n] = 0;
 #pragma unroll
-                for (int n = 0; n < NS; n++) h[n] = __builtin_fmaf(exp2_(d * A2[n]), h[n], du * m.B[n]);
+                for (int n = 0; n < NS; n++) h[n] = __builtin_fmaf(exp2_(d * A2[n]), h[n], x * bc[n]);
+                bc += 2 * NS;
+                __builtin_amdgcn_sched_barrier(0);
             }
             begins >>= G;
+            u += G * a.u_time, dt += G * a.dt_time;
         }
     }
     if (p.on) {
@@ -291,40 +288,53 @@ template <class T, int NS> __global__ __launch_bounds__(256) void scan_segment(S
 // what g leaves before a segment's first token, from zero after its last
 template <class T, int NS> __global__ __launch_bounds__(256) void scan_segment_back(ScanArgs a) {
     using raw = typename T::raw;
-    constexpr int kChunk = kGroup;
+    constexpr int G = 4;
     Place p(a, blockIdx.x / a.across, blockIdx.x % a.across);
     if (p.t0 >= p.end || (p.seg == 0 && a.dstate == nullptr)) return;
+    const uint32_t bytes = p.bytes(sizeof(raw));
     int64_t stop = p.t1 < p.end ? p.t1 : p.end;
     float g[NS], A2[NS], sum = 0;
     rates<NS>(a, p.e, A2);
 #pragma unroll
     for (int n = 0; n < NS; n++) g[n] = 0;
     bool cut = false;
+    const bool gated = a.z != nullptr;
     float bias = a.dt_bias != nullptr ? a.dt_bias[p.e] : 0.0f;
-    const raw *dt = (const raw *)a.dt + p.b * a.dt_batch, *dy = (const raw *)a.dy + p.b * a.dy_batch;
-    const raw *z = a.z != nullptr ? (const raw *)a.z + p.b * a.z_batch : nullptr;
-    Fixed *bc = fixed(a.bc + p.b * a.length * 2 * NS);
-    if (p.t0 < stop)
-        for (int64_t c0 = p.t0 + (stop - 1 - p.t0) / kChunk * kChunk; c0 >= p.t0; c0 -= kChunk) {
-            uint32_t begins = group_mask(a, p.b, c0, p.end);
-            cut = cut || begins != 0;
-            int64_t c1 = c0 + kChunk < stop ? c0 + kChunk : stop;
-            for (int64_t t = c1 - 1; t >= c0; t--) {
-                Pair<NS> m;
-                m.read(bc + t * 2 * NS);
-                float d = softplus_(up<T>((dt + t * a.dt_time)[p.e]) + bias), o = up<T>((dy + t * a.dy_time)[p.e]);
-                if (z != nullptr) {
-                    float zf = up<T>((z + t * a.z_time)[p.e]);
+    for (int64_t c0 = p.t0 + (stop - 1 - p.t0) / kGroup * kGroup; c0 >= p.t0; c0 -= kGroup) {
+        uint32_t begins = group_mask(a, p.b, c0, p.end);
+        cut = cut || begins != 0;
+        int count = (int)(c0 + kGroup < stop ? kGroup : stop - c0);
+        for (int i = (count - 1) / G * G; i >= 0; i -= G) {
+            const int64_t t = c0 + i;
+            Line<raw> ld((const raw *)a.dt, p.b * a.dt_batch + t * a.dt_time, a.dt_time), ly((const raw *)a.dy, p.b * a.dy_batch + t * a.dy_time, a.dy_time),
+                lz((const raw *)a.z, p.b * a.z_batch + t * a.z_time, a.z_time);
+            Fixed *bc = fixed(a.bc + (p.b * a.length + t) * 2 * NS);
+            raw rd[G], ry[G], rz[G];
+            const int here = count - i < G ? count - i : G;
+#pragma unroll
+            for (int q = 0; q < G; q++) {
+                int at = q < here ? q : here - 1;
+                rd[q] = ld.get(bytes, at), ry[q] = ly.get(bytes, at), rz[q] = lz.get(bytes, at);
+            }
+#pragma unroll
+            for (int q = G - 1; q >= 0; q--) {
+                if (q >= here) continue;
+                float d = softplus_(up<T>(rd[q]) + bias), o = up<T>(ry[q]);
+                if (gated) {
+                    float zf = up<T>(rz[q]);
                     o *= zf * sigmoid_(zf);
                 }
                 sum += d;
+                Fixed *C = bc + (q * 2 + 1) * NS;
 #pragma unroll
-                for (int n = 0; n < NS; n++) g[n] = exp2_(d * A2[n]) * __builtin_fmaf(o, m.C[n], g[n]);
-                if (begins >> (int)(t - c0) & 1)
+                for (int n = 0; n < NS; n++) g[n] = exp2_(d * A2[n]) * __builtin_fmaf(o, C[n], g[n]);
+                if (begins >> (i + q) & 1)
 #pragma unroll
                     for (int n = 0; n < NS; n++) g[n] = 0;
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
+    }
     if (p.on) {
         int64_t row = p.b * a.segments + p.seg;
         put_row<NS>(a.seg, row, a, p.e, g);
