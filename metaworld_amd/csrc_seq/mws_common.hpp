@@ -139,10 +139,10 @@ template <class Out> inline void launch_sum_parts(const float *part, int count, 
     if (columns > 0) hipLaunchKernelGGL((sum_parts<Out>), dim3((unsigned)((columns + 31) / 32)), dim3(1024), 0, stream, part, count, columns, out);
 }
 
-// ---- host: how many rows of one token a lane takes, so that its parameters are read once: up to `most`, as long as half the card's
+// ---- host: how many rows of one token a lane takes, so that its parameters are read once: up to `most`, as long as a quarter of the card's
 // places for waves stay filled.  Returns the number of lanes over the rows ----
 inline int64_t step_lanes(int64_t rows, int64_t lanes_of_row, int most) {
-    int64_t fill = (int64_t)kSimds * 4 * kWave, few = (rows + most - 1) / most, wanted = (fill + lanes_of_row - 1) / lanes_of_row;
+    int64_t fill = (int64_t)kSimds * 2 * kWave, few = (rows + most - 1) / most, wanted = (fill + lanes_of_row - 1) / lanes_of_row;
     int64_t lanes = wanted > few ? wanted : few;
     return lanes < rows ? lanes : rows;
 }

@@ -104,6 +104,34 @@ class MetaWorldTorchVectorEnv(MetaWorldGpuVectorEnv):
             self._upload_goals(self._next_goal)
         return obs, rew, term, trunc, infos
 
+    def policy_rollout(self, policy, nsteps, record=False):
+        """The learned counterpart of the scripted policies' rollout (mw_policy_rollout): from a reset, `nsteps` steps of a policy with
+        memory (recurrent_policy.RecurrentPolicy: `initial_state`, `act`), whose memory of an environment begins anew with each of its
+        episodes.  -> dict(episodes, successes: int32 [N], finished episodes and those in which info["success"] ever was 1); with
+        `record` also obs [N, nsteps, D], actions [N, nsteps, 4], rewards [N, nsteps] and reset [N, nsteps] (an episode's first token),
+        the segments that the policy trains on."""
+        torch, N = self._torch, self.num_envs
+        obs, _ = self.reset()
+        state, fresh = policy.initial_state(N), self._ones.clone()
+        ever = torch.zeros_like(self._ones)
+        episodes, successes = (torch.zeros(N, dtype=torch.int32, device=self.device) for _ in range(2))
+        out = {}
+        if record:
+            out = {"obs": torch.empty((N, nsteps) + tuple(obs.shape[1:]), dtype=obs.dtype, device=self.device), "actions": torch.empty((N, nsteps, 4), device=self.device),
+                   "rewards": torch.empty((N, nsteps), dtype=torch.float64, device=self.device), "reset": torch.empty((N, nsteps), dtype=torch.bool, device=self.device)}
+        for t in range(nsteps):
+            actions = policy.act(obs, state, fresh).float()
+            after, reward, term, trunc, infos = self.step(actions)
+            if record:
+                out["obs"][:, t], out["actions"][:, t], out["rewards"][:, t], out["reset"][:, t] = obs, actions, reward, fresh
+            fresh = term | trunc
+            ever |= infos["success"] > 0
+            episodes += fresh
+            successes += fresh & ever
+            ever &= ~fresh
+            obs = after
+        return dict(out, episodes=episodes, successes=successes)
+
     def call(self, name, *args, **kwargs):
         out = super().call(name, *args, **kwargs)          # host-side bookkeeping (and, for sample_tasks, a host-path reset)
         self._upload_goals(self._next_goal)
