@@ -19,12 +19,10 @@
 
 namespace mws {
 
-// Tokens are walked in groups of kGroup, whose episodes' beginnings are one mask; segments are whole groups.  kept_of: tokens between
-// two states kept for the backward pass; sub_of: tokens that the backward pass holds in registers at a time (states x tokens = 128
-// registers).  lanes_of: a block's channels at most.
-constexpr int kGroup = 32;
-constexpr int kept_of(int ns) { return ns >= 32 ? 16 : 8; }
-constexpr int sub_of(int ns) { return ns >= 32 ? 4 : 8; }
+// Tokens are walked in groups of kGroup, whose episodes' beginnings are one mask; segments are whole groups.  Every kKept-th token's
+// state is kept for the backward pass, which holds what lies between two of them in registers (states x tokens = 128).  lanes_of: a
+// block's channels at most.
+constexpr int kGroup = 32, kKept = 8;
 constexpr int lanes_of(int ns) { return ns >= 32 ? 128 : 256; }
 
 struct ScanArgs {
@@ -120,37 +118,38 @@ using Fixed = const __attribute__((address_space(4))) float;
 __device__ __forceinline__ Fixed *fixed(const float *p) { return (Fixed *)(uintptr_t)p; }
 template <int NS> struct Pair {
     float B[NS], C[NS];
-    __device__ __forceinline__ void read(Fixed *p) {
+    __device__ __forceinline__ void read(Fixed *p, int all = NS) {
 #pragma unroll
-        for (int n = 0; n < NS; n++) B[n] = p[n], C[n] = p[NS + n];
+        for (int n = 0; n < NS; n++) B[n] = p[n], C[n] = p[all + n];
     }
 };
 
-template <int NS> __device__ __forceinline__ void rates(const ScanArgs &a, uint32_t e, float (&A2)[NS]) {       // A / ln 2, for exp2
+// a lane's states: NS of them from `first` on, of `all` in a row (padded with zeros)
+template <int NS> __device__ __forceinline__ void rates(const ScanArgs &a, uint32_t e, float (&A2)[NS], int first = 0) {       // A / ln 2, for exp2
 #pragma unroll
-    for (int n = 0; n < NS; n++) A2[n] = n < a.states ? a.A[(int64_t)e * a.states + n] * kLog2e : 0.0f;
+    for (int n = 0; n < NS; n++) A2[n] = first + n < a.states ? a.A[(int64_t)e * a.states + first + n] * kLog2e : 0.0f;
 }
-template <int NS> __device__ __forceinline__ void first_state(const float *state, const ScanArgs &a, int64_t b, uint32_t e, float (&h)[NS]) {
+template <int NS> __device__ __forceinline__ void first_state(const float *state, const ScanArgs &a, int64_t b, uint32_t e, float (&h)[NS], int first = 0) {
 #pragma unroll
-    for (int n = 0; n < NS; n++) h[n] = state != nullptr && n < a.states ? state[(b * a.width + e) * a.states + n] : 0.0f;
+    for (int n = 0; n < NS; n++) h[n] = state != nullptr && first + n < a.states ? state[(b * a.width + e) * a.states + first + n] : 0.0f;
 }
-template <int NS> __device__ __forceinline__ void last_state(float *to, const ScanArgs &a, int64_t b, uint32_t e, const float (&h)[NS]) {
+template <int NS> __device__ __forceinline__ void last_state(float *to, const ScanArgs &a, int64_t b, uint32_t e, const float (&h)[NS], int first = 0) {
 #pragma unroll
     for (int n = 0; n < NS; n++)
-        if (n < a.states) to[(b * a.width + e) * a.states + n] = h[n];
+        if (first + n < a.states) to[(b * a.width + e) * a.states + first + n] = h[n];
 }
-template <int NS> __device__ __forceinline__ void get_row(const float *p, int64_t row, const ScanArgs &a, uint32_t e, float (&h)[NS]) {
+template <int NS> __device__ __forceinline__ void get_row(const float *p, int64_t row, const ScanArgs &a, uint32_t e, float (&h)[NS], int all = NS, int first = 0) {
 #pragma unroll
-    for (int n = 0; n < NS; n++) h[n] = (p + (row * NS + n) * a.width)[e];
+    for (int n = 0; n < NS; n++) h[n] = (p + (row * all + first + n) * a.width)[e];
 }
 template <int NS> __device__ __forceinline__ void put_row(float *p, int64_t row, const ScanArgs &a, uint32_t e, const float (&h)[NS]) {
 #pragma unroll
     for (int n = 0; n < NS; n++) (p + (row * NS + n) * a.width)[e] = h[n];
 }
 
-template <int NS, class Args> __device__ __forceinline__ void kept_row(const Args &a, int64_t row, uint32_t bytes, float (&h)[NS]) {
+template <int NS, class Args> __device__ __forceinline__ void kept_row(const Args &a, int64_t row, uint32_t bytes, float (&h)[NS], int all, int first) {
 #pragma unroll
-    for (int n = 0; n < NS; n++) h[n] = Line<float>(a.kept, (row * NS + n) * a.width, 0).get(bytes);
+    for (int n = 0; n < NS; n++) h[n] = Line<float>(a.kept, (row * all + first + n) * a.width, 0).get(bytes);
 }
 
 struct Place {          // what a block of the grid works on
@@ -159,8 +158,8 @@ struct Place {          // what a block of the grid works on
     int at, seg;
     bool on;
     __device__ __forceinline__ uint32_t bytes(int size) const { return on ? (uint32_t)at * (uint32_t)size : kOutside; }
-    template <class Args> __device__ __forceinline__ Place(const Args &a, int64_t item, int part) {
-        at = part * (int)blockDim.x + (int)threadIdx.x;
+    template <class Args> __device__ __forceinline__ Place(const Args &a, int64_t item, int part, int lanes = blockDim.x, int mine = threadIdx.x) {
+        at = part * lanes + mine;
         on = at < a.width;
         e = on ? at : a.width - 1;
         b = item / a.segments, seg = (int)(item % a.segments);
@@ -186,7 +185,7 @@ template <class T, int NS> __global__ __launch_bounds__(256) void scan_forward(S
         const raw *u = (const raw *)a.u + p.b * a.u_batch + p.t0 * a.u_time, *dt = (const raw *)a.dt + p.b * a.dt_batch + p.t0 * a.dt_time;
         const raw *z = a.z != nullptr ? (const raw *)a.z + p.b * a.z_batch + p.t0 * a.z_time : nullptr;
         Fixed *bc = fixed(a.bc + (p.b * a.length + p.t0) * 2 * NS);
-        float *kept = a.kept != nullptr ? a.kept + (p.b * a.chunks + p.t0 / kept_of(NS)) * NS * a.width : nullptr;
+        float *kept = a.kept != nullptr ? a.kept + (p.b * a.chunks + p.t0 / kKept) * NS * a.width : nullptr;
         auto token = [&](raw ru, raw rd, raw rz, bool first, const Line<raw> &out, int q) __attribute__((always_inline)) {
             Pair<NS> m;
             m.read(bc);
@@ -213,7 +212,7 @@ template <class T, int NS> __global__ __launch_bounds__(256) void scan_forward(S
             uint32_t begins = group_mask(a, p.b, c0, p.end);
             int count = (int)(c0 + kGroup < stop ? kGroup : stop - c0);
             for (int i = 0; i < count; i += G) {
-                if (kept != nullptr && i % kept_of(NS) == 0) {
+                if (kept != nullptr && i % kKept == 0) {
 #pragma unroll
                     for (int n = 0; n < NS; n++) Line<float>(kept, (int64_t)n * a.width, 0).put(h[n], p.bytes(4));
                     kept += (int64_t)NS * a.width;
@@ -410,43 +409,48 @@ template <int M> __device__ __forceinline__ float wave_sums(float (&v)[M / 2]) {
     return v[0];
 }
 
-// The backward pass walks over a segment from its end, kept state by kept state.  From one it goes forward over SUB tokens with what
-// each of them keeps of the state before it, a_t h_{t-1}, in registers (SUB x NS = 128 of them; with more tokens to a kept state
-// than that, a first walk leaves the states between in shared memory), and then backward over them.  dB and dC are summed over the
-// wave's channels token by token (wave_sums), over the block's waves after SUB tokens, over blocks by scan_bc_out.  Tokens past the
+// The backward pass walks over a segment from its end, kept state by kept state.  From one it goes forward over kKept tokens with what
+// each of them keeps of the state before it, a_t h_{t-1}, in registers, and then backward over them.  dB and dC are summed over the
+// wave's channels token by token (wave_sums), over the block's waves after kKept tokens, over blocks by scan_bc_out.  Tokens past the
 // row's end count with d = u = dy = 0, which leaves g as it is and adds nothing.
-template <class T, int NS> __global__ __launch_bounds__(256, NS >= 32 ? 2 : 2) void scan_backward(ScanArgs a) {
+// More than 16 states are two halves (H = 2), each a wave's: what a token's gradients need of both, its output and two sums over the
+// states, meets in shared memory, and each of the two waves finishes every second token (405 x 66 x 874 x 32 bf16 4413 us with all
+// states in one wave, most of that for registers that do not fit).
+// Bound by the vector unit: 2048 x 64 x 512 x 16 bf16 take 1.28 ms, 440 instructions a token and wave, at 70 % of its issue slots.
+template <class T, int NS, int H> __global__ __launch_bounds__(256, 2) void scan_backward(ScanArgs a) {
     using raw = typename T::raw;
-    constexpr int KEPT = kept_of(NS), SUB = sub_of(NS), kSubs = KEPT / SUB, M = 2 * NS;
+    constexpr int SUB = kKept, M = 2 * NS, ALL = NS * H;
     extern __shared__ float pool[];
-    int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), waves = blockDim.x / kWave;
+    const int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), waves = blockDim.x / kWave, half = H > 1 ? wave % H : 0, first_n = half * NS;
+    const int lanes = blockDim.x / H, mine = wave / H * kWave + lane;            // the block's channels, and the lane's among them
     float *sums = pool;                                                          // [2][waves][SUB][M]
-    float *states = pool + 2 * waves * SUB * M + (size_t)wave * (kSubs - 1) * NS * kWave + lane;       // [subs - 1][NS][64] of this wave
+    float *meet = pool + 2 * waves * SUB * M;                                    // H > 1: [2][waves][SUB][3][64]
     int part = blockIdx.x % a.across, group = blockIdx.x / a.across, turn = 0;
     float dA[NS], dD = 0, dbias = 0, A2[NS];
     {
-        int at = part * (int)blockDim.x + (int)threadIdx.x;
-        rates<NS>(a, at < a.width ? at : a.width - 1, A2);
+        int at = part * lanes + mine;
+        rates<NS>(a, at < a.width ? at : a.width - 1, A2, first_n);
     }
 #pragma unroll
     for (int n = 0; n < NS; n++) dA[n] = 0;
     for (int64_t item = group; item < a.batch * a.segments; item += a.groups) {
-        Place p(*fresh_args(), item, part);
+        Place p(*fresh_args(), item, part, lanes, mine);
         int64_t stop = p.t1 < p.end ? p.t1 : p.end;
         bool whole_end = p.end <= p.t1 && (p.end > p.t0 || p.seg == 0);
         const uint32_t bytes = p.bytes(sizeof(raw));
         if (p.t0 < stop || whole_end) {
             float g[NS];
-            if (a.segments > 1) get_row<NS>(a.seg, p.b * a.segments + p.seg, a, p.e, g);
-            else first_state<NS>(a.dlast, a, p.b, p.e, g);
+            if (a.segments > 1) get_row<NS>(a.seg, p.b * a.segments + p.seg, a, p.e, g, ALL, first_n);
+            else first_state<NS>(a.dlast, a, p.b, p.e, g, first_n);
             if (!p.on)
 #pragma unroll
                 for (int n = 0; n < NS; n++) g[n] = 0;
             float D = a.D != nullptr ? a.D[p.e] : 0.0f, bias = a.dt_bias != nullptr ? a.dt_bias[p.e] : 0.0f;
-            // SUB tokens from t, `here` of which are the row's; bit i of `begins`: an episode begins at token t + i
+
+            // tokens t .. t + SUB - 1, `here` of which are the row's; bit i of `begins`: an episode begins at token t + i
             auto walk = [&](int64_t t, int here, uint32_t begins, float (&h)[NS]) __attribute__((always_inline)) {
-                float keep[SUB][NS], d[SUB], uf[SUB];
-                raw rd[SUB], early[3];
+                float keep[SUB][NS], d[SUB];
+                raw ru[SUB], rd[SUB], early[4];
                 FixedArgs *in = fresh_args();
                 Line<raw> lu((const raw *)in->u, p.b * in->u_batch + t * in->u_time, in->u_time), ld((const raw *)in->dt, p.b * in->dt_batch + t * in->dt_time, in->dt_time),
                     ly((const raw *)in->dy, p.b * in->dy_batch + t * in->dy_time, in->dy_time), lz((const raw *)in->z, p.b * in->z_batch + t * in->z_time, in->z_time);
@@ -454,18 +458,16 @@ template <class T, int NS> __global__ __launch_bounds__(256, NS >= 32 ? 2 : 2) v
 #pragma unroll
                 for (int q = 0; q < SUB; q++) {
                     int at = q < here ? q : here - 1;
-                    raw ru = lu.get(bytes, at);
-                    rd[q] = ld.get(bytes, at);
-                    uf[q] = q < here ? up<T>(ru) : 0.0f;
+                    ru[q] = lu.get(bytes, at), rd[q] = ld.get(bytes, at);
                 }
-                early[0] = ld.get(bytes, here - 1), early[1] = ly.get(bytes, here - 1), early[2] = lz.get(bytes, here - 1);
-                Fixed *bc = fixed(in->bc + (p.b * in->length + t) * 2 * NS);
+                early[0] = ld.get(bytes, here - 1), early[1] = ly.get(bytes, here - 1), early[2] = lz.get(bytes, here - 1), early[3] = lu.get(bytes, here - 1);
+                Fixed *bc = fixed(in->bc + (p.b * in->length + t) * 2 * ALL + first_n);
 #pragma unroll
                 for (int q = 0; q < SUB; q++) {
                     if (q % 2 == 0) asm volatile("" : "+s"(bc));         // two tokens' B at a time
-                    Fixed *m = bc + (q < here ? q : here - 1) * 2 * NS;
+                    Fixed *m = bc + (q < here ? q : here - 1) * 2 * ALL;
                     d[q] = q < here ? softplus_(up<T>(rd[q]) + bias) : 0.0f;
-                    float x = d[q] * uf[q];
+                    float x = q < here ? d[q] * up<T>(ru[q]) : 0.0f;
                     if (begins >> q & 1)
 #pragma unroll
                         for (int n = 0; n < NS; n++) h[n] = 0;
@@ -485,14 +487,24 @@ template <class T, int NS> __global__ __launch_bounds__(256, NS >= 32 ? 2 : 2) v
                 for (int q = 0; q < SUB; q++) asm volatile("" : "+v"(d[q]));
                 asm volatile("" : "+s"(bc));
                 float *to = sums + (turn * waves + wave) * SUB * M;
+                float *others = meet + (turn * waves + wave) * SUB * 3 * kWave + lane;
                 FixedArgs *out_to = fresh_args();
                 const int64_t row = (p.b * out_to->length + t) * out_to->width;
                 Line<raw> gu((raw *)out_to->du, row, out_to->width), gd((raw *)out_to->ddt, row, out_to->width), gz((raw *)out_to->dz, row, out_to->width);
+                // a token's gradients from its sums over all states
+                auto finish = [&](int q, float out, float zf, float sig, float o, float y, float gB, float gk, float raw_d, float dq, float uq) __attribute__((always_inline)) {
+                    float dd = __builtin_fmaf(uq, gB, gk * kLn2), draw = dd * sigmoid_(raw_d);
+                    dD = __builtin_fmaf(o, uq, dD);
+                    dbias += draw;
+                    gu.put(down<T>(__builtin_fmaf(D, o, dq * gB)), bytes, q);
+                    gd.put(down<T>(draw), bytes, q);
+                    if (gated) gz.put(down<T>(out * __builtin_fmaf(D, uq, y) * sig * (1.0f + zf * (1.0f - sig))), bytes, q);
+                };
 #pragma unroll
                 for (int q = SUB - 1; q >= 0; q--) {
                     Pair<NS> m;
-                    m.read(bc + (q < here ? q : here - 1) * 2 * NS);
-                    float raw_d = up<T>(early[0]) + bias, out = q < here ? up<T>(early[1]) : 0.0f, zf = 0, gate = 1, sig = 0;
+                    m.read(bc + (q < here ? q : here - 1) * 2 * ALL, ALL);
+                    float raw_d = up<T>(early[0]) + bias, out = q < here ? up<T>(early[1]) : 0.0f, uq = q < here ? up<T>(early[3]) : 0.0f, zf = 0, gate = 1, sig = 0;
                     if (gated) {
                         zf = up<T>(early[2]);
                         sig = sigmoid_(zf);
@@ -500,11 +512,13 @@ template <class T, int NS> __global__ __launch_bounds__(256, NS >= 32 ? 2 : 2) v
                     }
                     if (q > 0) {                 // the token before, one token ahead
                         int at = q - 1 < here ? q - 1 : here - 1;
-                        early[0] = ld.get(bytes, at), early[1] = ly.get(bytes, at), early[2] = lz.get(bytes, at);
+                        early[0] = ld.get(bytes, at), early[1] = ly.get(bytes, at), early[2] = lz.get(bytes, at), early[3] = lu.get(bytes, at);
                     }
-                    float o = out * gate, x = d[q] * uf[q], gB = 0, gk = 0, y = D * uf[q], v[NS];
+                    float o = out * gate, x = d[q] * uq, gB = 0, gk = 0, y = 0, v[NS];
 #pragma unroll
                     for (int n = 0; n < NS; n++) {
+                        // four states at a time, their sums added up here and not when they are next asked for: what the compiler
+                        // would keep for later does not fit the registers
                         if (n % 4 == 0)
 #pragma unroll
                             for (int k = n; k < n + 4; k++) asm volatile("" : "+v"(keep[q][k]), "+v"(g[k]));
@@ -524,26 +538,38 @@ template <class T, int NS> __global__ __launch_bounds__(256, NS >= 32 ? 2 : 2) v
                     if (begins >> q & 1)
 #pragma unroll
                         for (int n = 0; n < NS; n++) g[n] = 0;
-                    float dd = __builtin_fmaf(uf[q], gB, gk * kLn2), draw = q < here ? dd * sigmoid_(raw_d) : 0.0f;
-                    dD = __builtin_fmaf(o, uf[q], dD);
-                    dbias += draw;
-                    if (q < here) {
-                        gu.put(down<T>(__builtin_fmaf(D, o, d[q] * gB)), bytes, q);
-                        gd.put(down<T>(draw), bytes, q);
-                        if (gated) gz.put(down<T>(out * y * sig * (1.0f + zf * (1.0f - sig))), bytes, q);
-                    }
+                    if constexpr (H == 1) {
+                        if (q < here) finish(q, out, zf, sig, o, y, gB, gk, raw_d, d[q], uq);
+                    } else others[(q * 3 + 0) * kWave] = y, others[(q * 3 + 1) * kWave] = gB, others[(q * 3 + 2) * kWave] = gk;
                     float total = wave_sums<M>(v);
                     if (lane % (kWave / M) == 0) to[q * M + lane / (kWave / M)] = total;
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                // the other half of `sums` is read by nobody after this barrier, and this half is written again after the next
+                // the other half of `sums` and `meet` is read by nobody after this barrier, and this half is written again after the next
                 __syncthreads();
+                if constexpr (H > 1) {
+                    const float *both = meet + (turn * waves + wave / H * H) * SUB * 3 * kWave + lane;
+                    for (int q = half; q < here; q += H) {
+                        float uq = up<T>(lu.get(bytes, q)), raw_d = up<T>(ld.get(bytes, q)) + bias, out = up<T>(ly.get(bytes, q)), zf = 0, gate = 1, sig = 0, s[3] = {0, 0, 0};
+                        if (gated) {
+                            zf = up<T>(lz.get(bytes, q));
+                            sig = sigmoid_(zf);
+                            gate = zf * sig;
+                        }
+#pragma unroll
+                        for (int k = 0; k < 3; k++)
+#pragma unroll
+                            for (int w = 0; w < H; w++) s[k] += both[((w * SUB + q) * 3 + k) * kWave];
+                        finish(q, out, zf, sig, out * gate, s[0], s[1], s[2], raw_d, softplus_(raw_d), uq);
+                    }
+                }
                 const float *from = sums + turn * waves * SUB * M;
                 FixedArgs *sums_to = fresh_args();
-                float *bc_to = sums_to->part_bc + (((int64_t)part * sums_to->batch + p.b) * sums_to->length + t) * M;
-                for (int k = threadIdx.x; k < here * M; k += blockDim.x) {
+                float *bc_to = sums_to->part_bc + (((int64_t)part * sums_to->batch + p.b) * sums_to->length + t) * 2 * ALL;
+                for (int k = threadIdx.x; k < here * 2 * ALL; k += blockDim.x) {
+                    const int q = k / (2 * ALL), n = k % NS, of = k / NS % H, which = k / ALL % 2;       // [token][B | C][half][state]
                     float v = 0;
-                    for (int w = 0; w < waves; w++) v += from[w * SUB * M + k];
+                    for (int w = of; w < waves; w += H) v += from[(w * SUB + q) * M + which * NS + n];
                     bc_to[k] = v;
                 }
                 turn ^= 1;
@@ -553,58 +579,43 @@ template <class T, int NS> __global__ __launch_bounds__(256, NS >= 32 ? 2 : 2) v
                 for (int64_t c0 = p.t0 + (stop - 1 - p.t0) / kGroup * kGroup; c0 >= p.t0; c0 -= kGroup) {
                     uint32_t begins = group_mask(*fresh_args(), p.b, c0, p.end);
                     int count = (int)(c0 + kGroup < stop ? kGroup : stop - c0);
-                    for (int i = (count - 1) / KEPT * KEPT; i >= 0; i -= KEPT) {
+                    for (int i = (count - 1) / SUB * SUB; i >= 0; i -= SUB) {
                         float h[NS];
                         FixedArgs *states_of = fresh_args();
-                        const int64_t row = p.b * states_of->chunks + (c0 + i) / KEPT;
-                        kept_row<NS>(*states_of, row, p.bytes(4), h);
-                        int subs = kSubs == 1 || count - i <= SUB ? 1 : (count - i < KEPT ? count - i + SUB - 1 : KEPT) / SUB;
-                        if constexpr (kSubs > 1) {
-                            const raw *u = (const raw *)a.u + p.b * a.u_batch, *dt = (const raw *)a.dt + p.b * a.dt_batch;
-                            for (int k = 0; k + 1 < subs; k++) {
-#pragma unroll
-                                for (int q = 0; q < SUB; q++) {
-                                    int64_t t = c0 + i + k * SUB + q;
-                                    float d = softplus_(up<T>((dt + t * a.dt_time)[p.e]) + bias), x = d * up<T>((u + t * a.u_time)[p.e]);
-                                    if (begins >> (i + k * SUB + q) & 1)
-#pragma unroll
-                                        for (int n = 0; n < NS; n++) h[n] = 0;
-                                    Fixed *m = fixed(a.bc + (p.b * a.length + t) * 2 * NS);
-#pragma unroll
-                                    for (int n = 0; n < NS; n++) h[n] = __builtin_fmaf(exp2_(d * A2[n]), h[n], x * m[n]);
-                                }
-#pragma unroll
-                                for (int n = 0; n < NS; n++) states[(k * NS + n) * kWave] = h[n];
-                            }
-                        }
-                        for (int k = subs - 1; k >= 0; k--) {
-                            if constexpr (kSubs > 1) {
-                                if (k > 0)
-#pragma unroll
-                                    for (int n = 0; n < NS; n++) h[n] = states[((k - 1) * NS + n) * kWave];
-                                else if (subs > 1) kept_row<NS>(*fresh_args(), row, p.bytes(4), h);
-                            }
-                            int from = i + k * SUB, here = count - from < SUB ? count - from : SUB;
-                            walk(c0 + from, here, begins >> from, h);
-                        }
+                        kept_row<NS>(*states_of, p.b * states_of->chunks + (c0 + i) / SUB, p.bytes(4), h, ALL, first_n);
+                        walk(c0 + i, count - i < SUB ? count - i : SUB, begins >> i, h);
                     }
                 }
-            if (p.on && p.seg == 0 && a.segments == 1 && a.dstate != nullptr) last_state<NS>(a.dstate, a, p.b, p.e, g);
+            if (p.on && p.seg == 0 && a.segments == 1 && a.dstate != nullptr) last_state<NS>(a.dstate, a, p.b, p.e, g, first_n);
         }
         raw *du = (raw *)a.du + p.b * a.length * a.width, *ddt = (raw *)a.ddt + p.b * a.length * a.width, *dz = a.z != nullptr ? (raw *)a.dz + p.b * a.length * a.width : nullptr;
-        if (p.on)
+        if (p.on && half == 0)
             for (int64_t t = p.t0 > p.end ? p.t0 : p.end; t < p.t1; t++) {
                 (du + t * a.width)[p.e] = (ddt + t * a.width)[p.e] = down<T>(0.0f);
                 if (dz != nullptr) (dz + t * a.width)[p.e] = down<T>(0.0f);
             }
     }
-    int at = part * (int)blockDim.x + (int)threadIdx.x;
-    if (at < a.width) {
-        float *to = a.part + (int64_t)group * (NS + 2) * a.width + at;
+    // dD and ddt_bias: each half has its tokens' part
+    float other[2] = {0, 0};
+    if constexpr (H > 1) {
+        __syncthreads();
+        sums[(wave * 2 + 0) * kWave + lane] = dD, sums[(wave * 2 + 1) * kWave + lane] = dbias;
+        __syncthreads();
 #pragma unroll
-        for (int n = 0; n < NS; n++) to[(int64_t)n * a.width] = dA[n];
-        to[(int64_t)NS * a.width] = dD;
-        to[(int64_t)(NS + 1) * a.width] = dbias;
+        for (int w = 1; w < H; w++)
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+                if (half == 0) other[k] += sums[((wave + w) * 2 + k) * kWave + lane];
+    }
+    int at = part * lanes + mine;
+    if (at < a.width) {
+        float *to = a.part + (int64_t)group * (ALL + 2) * a.width + at;
+#pragma unroll
+        for (int n = 0; n < NS; n++) to[(int64_t)(first_n + n) * a.width] = dA[n];
+        if (half == 0) {
+            to[(int64_t)ALL * a.width] = dD + other[0];
+            to[(int64_t)(ALL + 1) * a.width] = dbias + other[1];
+        }
     }
 }
 
@@ -696,7 +707,13 @@ template <class T, int Q> __global__ __launch_bounds__(256) void scan_step(ScanA
 }
 
 // ---- host ----
-static int scan_ns(const mws_scan_args *a) { return a->states <= 4 ? 4 : a->states <= 8 ? 8 : a->states <= 16 ? 16 : 32; }
+// The states that a lane walks with.  Powers of two where a backward pass follows, whose sums over a wave halve them step by step;
+// steps of four and eight where none does (3 x 5000 x 777 x 12 fp16 112 us, padded to 16 states 134 us).
+static int scan_ns(const mws_scan_args *a, bool backward) {
+    int n = a->states;
+    if (!backward && a->kept == nullptr && n > 8) return n <= 12 ? 12 : n <= 16 ? 16 : n <= 24 ? 24 : 32;
+    return n <= 4 ? 4 : n <= 8 ? 8 : n <= 16 ? 16 : 32;
+}
 
 struct ScanPlan {
     int ns, lanes, across, segments, span, groups;
@@ -735,16 +752,16 @@ static int64_t best_span(int64_t waves, int64_t groups, bool backward) {
 
 static ScanPlan scan_plan(const mws_scan_args *a, bool backward) {
     ScanPlan p = {};
-    p.ns = scan_ns(a);
+    p.ns = scan_ns(a, backward);
     int waves = (int)ceil_div(a->width, kWave), of_block = block_waves(waves, lanes_of(p.ns) / kWave);
     p.lanes = of_block * kWave;
     p.across = (int)ceil_div(a->width, p.lanes);
-    p.chunks = ceil_div(a->length, kept_of(p.ns));
-    int64_t groups = ceil_div(a->length > 0 ? a->length : 1, kGroup), each = best_span(a->batch * p.across * of_block, groups, backward);
+    p.chunks = ceil_div(a->length, kKept);
+    int64_t groups = ceil_div(a->length > 0 ? a->length : 1, kGroup), halves = backward && p.ns > 16 ? 2 : 1, each = best_span(a->batch * p.across * of_block * halves, groups, backward);
     p.segments = (int)ceil_div(groups, each);
     p.span = (int)(each * kGroup);
     // blocks over the items, four rounds of the places at most: each leaves partial sums of dA, dD and ddt_bias
-    int64_t items = a->batch * p.segments, most = 8 * kSimds / ((int64_t)of_block * p.across) > 0 ? 8 * kSimds / ((int64_t)of_block * p.across) : 1;
+    int64_t items = a->batch * p.segments, most = 8 * kSimds / (of_block * halves * p.across) > 0 ? 8 * kSimds / (of_block * halves * p.across) : 1;
     p.groups = (int)(items < most ? items : most);
     int64_t at = 0, tokens = a->batch * a->length;
     auto take = [&at](int64_t n) {
@@ -814,15 +831,17 @@ template <class T, int NS> static void forward_go(const mws_scan_args *a, const 
     hipLaunchKernelGGL((scan_forward<T, NS>), grid, block, 0, stream, d);
 }
 template <class T, int NS> static void backward_go(const mws_scan_args *a, const ScanPlan &p, const ScanArgs &d, hipStream_t stream) {
-    constexpr int SUB = sub_of(NS);
+    constexpr int H = NS > 16 ? 2 : 1, PER = NS / H;
     dim3 block(p.lanes);
     spread_go<T, NS>(a, d, stream);
     if (p.segments > 1) {
         hipLaunchKernelGGL((scan_segment_back<T, NS>), dim3((unsigned)(d.batch * p.segments * p.across)), block, 0, stream, d);
         join_go(d, NS, true, stream);
     }
-    size_t lds = (size_t)(p.lanes / kWave) * ((kept_of(NS) / SUB - 1) * NS * kWave + 2 * SUB * 2 * NS) * sizeof(float);
-    if (d.batch > 0) hipLaunchKernelGGL((scan_backward<T, NS>), dim3((unsigned)(p.groups * p.across)), block, lds, stream, d);
+    // 25 KB a wave of a half, 8 KB for four waves without: under the 64 KB that a block has without asking for more
+    const int waves = p.lanes / kWave * H;
+    size_t lds = (size_t)2 * waves * kKept * (2 * PER + (H > 1 ? 3 * kWave : 0)) * sizeof(float);
+    if (d.batch > 0) hipLaunchKernelGGL((scan_backward<T, PER, H>), dim3((unsigned)(p.groups * p.across)), dim3(waves * kWave), lds, stream, d);
     int64_t count = d.batch * d.length * 2 * NS;
     if (count > 0)
         hipLaunchKernelGGL((scan_bc_out<T>), dim3((unsigned)ceil_div(count, 256)), dim3(256), 0, stream, d.part_bc, a->lengths, a->dB, a->dC, d.batch, d.length, p.across, a->states, NS);
@@ -833,7 +852,9 @@ template <class T> static void scan_go(const mws_scan_args *a, const ScanPlan &p
 #define MWS_GO(NS) (backward ? backward_go<T, NS>(a, p, d, stream) : forward_go<T, NS>(a, p, d, stream))
     if (p.ns == 4) MWS_GO(4);
     else if (p.ns == 8) MWS_GO(8);
+    else if (p.ns == 12) forward_go<T, 12>(a, p, d, stream);
     else if (p.ns == 16) MWS_GO(16);
+    else if (p.ns == 24) forward_go<T, 24>(a, p, d, stream);
     else MWS_GO(32);
 #undef MWS_GO
 }
@@ -860,7 +881,7 @@ using namespace mws;
 
 extern "C" int64_t mws_scan_kept(const mws_scan_args *a) {
     if (int32_t e = scan_check(a, "mws_scan_kept", false, false, false)) return e;
-    return a->batch * ceil_div(a->length, kept_of(scan_ns(a))) * scan_ns(a) * a->width;
+    return a->batch * ceil_div(a->length, kKept) * scan_ns(a, true) * a->width;
 }
 
 extern "C" int64_t mws_scan_workspace(const mws_scan_args *a, int32_t backward) {
