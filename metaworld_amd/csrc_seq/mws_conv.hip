@@ -397,7 +397,7 @@ static int32_t conv_check(const mws_conv_args *a, const char *what, bool backwar
     if (a->type < MWS_F32 || a->type > MWS_F16) return fail("%s: type %d is none of MWS_F32, MWS_BF16, MWS_F16", what, a->type);
     if (a->param_type != MWS_F32 && a->param_type != a->type) return fail("%s: parameters are float or of the activations' type", what);
     if (a->taps < MWS_CONV_MIN_TAPS || a->taps > MWS_CONV_MAX_TAPS) return fail("%s: %d taps are not within %d .. %d", what, a->taps, MWS_CONV_MIN_TAPS, MWS_CONV_MAX_TAPS);
-    if (a->width < 1 || a->width > (1 << 24)) return fail("%s: width %d", what, a->width);
+    if (a->width < 1 || a->width > (1 << 22)) return fail("%s: width %d", what, a->width);
     if (a->batch < 0 || a->length < 0 || a->batch > (1 << 30) || a->length > (1 << 30) || a->batch * (a->length + 1) > ((int64_t)1 << 33)) return fail("%s: %lld rows of %lld tokens", what, (long long)a->batch, (long long)a->length);
     if (a->weight == nullptr) return fail("%s: weight is NULL", what);
     if (step && a->length != 1) return fail("%s: one token at a time", what);

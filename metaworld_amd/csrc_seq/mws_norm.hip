@@ -98,7 +98,9 @@ template <class T, int V, int PER, int TPR> struct Row {
                 v[k * V + i] = c;
                 q += c * c;
             }
-        return __builtin_amdgcn_rsqf(row_sum<TPR>(q, meet, turn) * share + eps);
+        float v = row_sum<TPR>(q, meet, turn) * share + eps;
+        // (the hardware's 1 / sqrt takes numbers below the smallest normal one as zeros: they are scaled)
+        return v < 0x1p-96f ? __builtin_amdgcn_rsqf(v * 0x1p64f) * 0x1p32f : __builtin_amdgcn_rsqf(v);
     }
 };
 

@@ -353,11 +353,11 @@ __global__ __launch_bounds__(256) void scan_join(ScanArgs a, int ns, bool backwa
     float A2 = real ? a.A[(int64_t)e * a.states + n] * kLog2e : 0.0f;
     const float *from = backward ? a.dlast : a.state;
     float h = from != nullptr && real ? from[(b * a.width + e) * a.states + n] : 0.0f;
-    // eight segments' values under way at a time: the chain through h does not wait for them
-    for (int k0 = 0; k0 <= last; k0 += 8) {
-        float left[8], sum[8];
+    // sixteen segments' values under way at a time: the chain through h does not wait for them
+    for (int k0 = 0; k0 <= last; k0 += 16) {
+        float left[16], sum[16];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
+        for (int j = 0; j < 16; j++) {
             int k = k0 + j, s = backward ? last - k : k;
             bool asked = k < last || (k == last && backward && a.dstate != nullptr);
             int64_t row = b * a.segments + (asked ? s : 0);
@@ -365,11 +365,13 @@ __global__ __launch_bounds__(256) void scan_join(ScanArgs a, int ns, bool backwa
             sum[j] = asked ? a.sum[row * a.width + e] : 0.0f;
         }
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
+        for (int j = 0; j < 16; j++) {
             int k = k0 + j, s = backward ? last - k : k;
-            if (k > last) break;
-            a.seg[((b * a.segments + s) * ns + n) * a.width + e] = h;
-            h = sum[j] < 0.0f || h == 0.0f ? left[j] : __builtin_fmaf(exp2_(sum[j] * A2), h, left[j]);
+            float next = sum[j] < 0.0f || h == 0.0f ? left[j] : __builtin_fmaf(exp2_(sum[j] * A2), h, left[j]);
+            if (k <= last) {
+                a.seg[((b * a.segments + s) * ns + n) * a.width + e] = h;
+                h = next;
+            }
         }
     }
     if (backward && a.dstate != nullptr && real) {
@@ -708,7 +710,7 @@ template <class T, int Q> __global__ __launch_bounds__(256) void scan_step(ScanA
 
 // ---- host ----
 // The states that a lane walks with.  Powers of two where a backward pass follows, whose sums over a wave halve them step by step;
-// steps of four and eight where none does (3 x 5000 x 777 x 12 fp16 112 us, padded to 16 states 134 us).
+// steps of four and eight where none does (3 x 5000 x 777 x 12 fp16 120 us, padded to 16 states 134 us).
 static int scan_ns(const mws_scan_args *a, bool backward) {
     int n = a->states;
     if (!backward && a->kept == nullptr && n > 8) return n <= 12 ? 12 : n <= 16 ? 16 : n <= 24 ? 24 : 32;
@@ -782,7 +784,7 @@ static int32_t scan_check(const mws_scan_args *a, const char *what, bool backwar
     if (a == nullptr) return fail("%s: no arguments", what);
     if (a->type < MWS_F32 || a->type > MWS_F16) return fail("%s: type %d is none of MWS_F32, MWS_BF16, MWS_F16", what, a->type);
     if (a->states < 1 || a->states > MWS_SCAN_MAX_STATES) return fail("%s: %d states are not within 1 .. %d", what, a->states, MWS_SCAN_MAX_STATES);
-    if (a->width < 1 || a->width > (1 << 24)) return fail("%s: width %d", what, a->width);
+    if (a->width < 1 || a->width > (1 << 22)) return fail("%s: width %d", what, a->width);
     if (a->batch < 0 || a->length < 0 || a->batch > (1 << 30) || a->length > (1 << 30) || a->batch * (a->length + 1) > ((int64_t)1 << 33)) return fail("%s: %lld rows of %lld tokens", what, (long long)a->batch, (long long)a->length);
     if (step && a->length != 1) return fail("%s: one token at a time", what);
     for (int64_t stride : {a->u_time, a->dt_time, a->z_time, a->dy_time})
@@ -834,7 +836,7 @@ template <class T, int NS> static void backward_go(const mws_scan_args *a, const
     constexpr int H = NS > 16 ? 2 : 1, PER = NS / H;
     dim3 block(p.lanes);
     spread_go<T, NS>(a, d, stream);
-    if (p.segments > 1) {
+    if (p.segments > 1 && d.batch > 0) {
         hipLaunchKernelGGL((scan_segment_back<T, NS>), dim3((unsigned)(d.batch * p.segments * p.across)), block, 0, stream, d);
         join_go(d, NS, true, stream);
     }
@@ -894,7 +896,8 @@ static int32_t scan_call(const mws_scan_args *a, const char *what, bool backward
     ScanPlan p = scan_plan(a, backward);
     if (a->workspace_bytes < p.bytes || (p.bytes > 0 && a->workspace == nullptr)) return fail("%s: the workspace needs %lld bytes", what, (long long)p.bytes);
     if (!backward && a->batch == 0) return 0;
-    if (a->batch * p.segments * p.across > 0x7fffffff) return fail("%s: too many rows", what);
+    if (a->batch * p.segments * p.across > 0x7fffffff || ceil_div(a->batch * a->length * 2 * p.ns, 256) > 0x7fffffff || ceil_div(a->batch * p.ns * a->width, 256) > 0x7fffffff)
+        return fail("%s: too many rows", what);
     scan_run(a, p, scan_device(a, p), backward, (hipStream_t)stream);
     return launched(what);
 }

@@ -115,6 +115,10 @@ def test_layer_norm_shapes_strides_and_broadcast_inputs():
     # rows that are constant: no variance, y is the bias
     flat = torch.full((3, 90), 2.5, device="cuda")
     assert torch.equal(sequence.layer_norm(flat), torch.zeros_like(flat))
+    # without eps a variance below the smallest normal number (values of 1e-21) still normalises; it has few bits left
+    small = torch.randn(4, 256, device="cuda") * 1e-21
+    y = sequence.layer_norm(small, eps=0.0)
+    assert torch.allclose(y, sequence.layer_norm(small * 1e21, eps=0.0), rtol=0.01, atol=0.01)
 
 
 # ---- tokens of both operators over time ----
@@ -447,6 +451,9 @@ def test_rows_and_tokens_of_none():
     y, last = sequence.selective_scan(u[:0], dt[:0], A, B[:0], C[:0], D, z[:0], bias)
     assert y.shape == (0, 4, 10) and last.shape == (0, 10, 16)
     assert torch.equal(torch.autograd.grad(y.sum(), A)[0], torch.zeros_like(A))
+    none = torch.zeros(0, 700, 10, device="cuda")                          # no row of many tokens
+    y, last = sequence.selective_scan(none, none, A, none[..., :1].expand(0, 700, 16), none[..., :1].expand(0, 700, 16))
+    assert torch.equal(torch.autograd.grad(y.sum() + last.sum(), A)[0], torch.zeros_like(A))
     w, held = torch.randn(10, 4, device="cuda", requires_grad=True), torch.randn(3, 3, 10, device="cuda", requires_grad=True)
     y, last = sequence.causal_conv(empty(u), w, state=held)
     assert y.shape == (3, 0, 10) and torch.equal(last, held)
