@@ -147,6 +147,14 @@ template <int NS> __device__ __forceinline__ void put_row(float *p, int64_t row,
     for (int n = 0; n < NS; n++) (p + (row * NS + n) * a.width)[e] = h[n];
 }
 
+// An episode begins: the states count as zeros.  As a branch, which is hardly ever taken; selections would be there for every token.
+template <int NS> __device__ __forceinline__ void forget(float (&h)[NS]) {
+#pragma unroll
+    for (int n = 0; n < NS; n++) {
+        h[n] = 0;
+        asm volatile("" : "+v"(h[n]));
+    }
+}
 template <int NS, class Args> __device__ __forceinline__ void kept_row(const Args &a, int64_t row, uint32_t bytes, float (&h)[NS], int all, int first) {
 #pragma unroll
     for (int n = 0; n < NS; n++) h[n] = Line<float>(a.kept, (row * all + first + n) * a.width, 0).get(bytes);
@@ -190,9 +198,7 @@ template <class T, int NS> __global__ __launch_bounds__(256) void scan_forward(S
             Pair<NS> m;
             m.read(bc);
             float uf = up<T>(ru), d = softplus_(up<T>(rd) + bias), du = d * uf, o = D * uf, o2 = 0;
-            if (first)
-#pragma unroll
-                for (int n = 0; n < NS; n++) h[n] = 0;
+            if (first) forget<NS>(h);
 #pragma unroll
             for (int n = 0; n < NS; n++) {
                 h[n] = __builtin_fmaf(exp2_(d * A2[n]), h[n], du * m.B[n]);
@@ -265,9 +271,7 @@ template <class T, int NS> __global__ __launch_bounds__(256) void scan_segment(S
             for (int q = 0; q < G; q++) {
                 float d = softplus_(up<T>(rd[q]) + bias), x = d * up<T>(ru[q]);
                 sum += d;
-                if (begins >> q & 1)
-#pragma unroll
-                    for (int n = 0; n < NS; n++) h[n] = 0;
+                if (begins >> q & 1) forget<NS>(h);
 #pragma unroll
                 for (int n = 0; n < NS; n++) h[n] = __builtin_fmaf(exp2_(d * A2[n]), h[n], x * bc[n]);
                 bc += 2 * NS;
@@ -327,9 +331,7 @@ template <class T, int NS> __global__ __launch_bounds__(256) void scan_segment_b
                 Fixed *C = bc + (q * 2 + 1) * NS;
 #pragma unroll
                 for (int n = 0; n < NS; n++) g[n] = exp2_(d * A2[n]) * __builtin_fmaf(o, C[n], g[n]);
-                if (begins >> (i + q) & 1)
-#pragma unroll
-                    for (int n = 0; n < NS; n++) g[n] = 0;
+                if (begins >> (i + q) & 1) forget<NS>(g);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -466,13 +468,11 @@ template <class T, int NS, int H> __global__ __launch_bounds__(256, 2) void scan
                 Fixed *bc = fixed(in->bc + (p.b * in->length + t) * 2 * ALL + first_n);
 #pragma unroll
                 for (int q = 0; q < SUB; q++) {
-                    if (q % 2 == 0) asm volatile("" : "+s"(bc));         // two tokens' B at a time
+                    if (q % 2 == 0) asm volatile("" : "+s"(bc), "+s"(here), "+s"(begins));         // two tokens' B at a time, and no comparison held for later
                     Fixed *m = bc + (q < here ? q : here - 1) * 2 * ALL;
                     d[q] = q < here ? softplus_(up<T>(rd[q]) + bias) : 0.0f;
                     float x = q < here ? d[q] * up<T>(ru[q]) : 0.0f;
-                    if (begins >> q & 1)
-#pragma unroll
-                        for (int n = 0; n < NS; n++) h[n] = 0;
+                    if (begins >> q & 1) forget<NS>(h);
 #pragma unroll
                     for (int n = 0; n < NS; n++) {
                         keep[q][n] = exp2_(d[q] * A2[n]) * h[n];
@@ -504,6 +504,7 @@ template <class T, int NS, int H> __global__ __launch_bounds__(256, 2) void scan
                 };
 #pragma unroll
                 for (int q = SUB - 1; q >= 0; q--) {
+                    asm volatile("" : "+s"(here), "+s"(begins));
                     Pair<NS> m;
                     m.read(bc + (q < here ? q : here - 1) * 2 * ALL, ALL);
                     float raw_d = up<T>(early[0]) + bias, out = q < here ? up<T>(early[1]) : 0.0f, uq = q < here ? up<T>(early[3]) : 0.0f, zf = 0, gate = 1, sig = 0;
@@ -537,9 +538,7 @@ template <class T, int NS, int H> __global__ __launch_bounds__(256, 2) void scan
 #pragma unroll
                             for (int k = n - 3; k <= n; k++) asm volatile("" : "+v"(dA[k]), "+v"(g[k]), "+v"(v[k]));
                     }
-                    if (begins >> q & 1)
-#pragma unroll
-                        for (int n = 0; n < NS; n++) g[n] = 0;
+                    if (begins >> q & 1) forget<NS>(g);
                     if constexpr (H == 1) {
                         if (q < here) finish(q, out, zf, sig, o, y, gB, gk, raw_d, d[q], uq);
                     } else others[(q * 3 + 0) * kWave] = y, others[(q * 3 + 1) * kWave] = gB, others[(q * 3 + 2) * kWave] = gk;
