@@ -5,8 +5,9 @@
 //
 // where x of a token before the row's first comes from the state, and of one before the episode's first is zero.
 //
-// Bound by memory.  A lane keeps V neighbouring channels (one 16-byte access a token), a wave walks over a tile of tokens with the
-// last K of them in registers, so that every value is read once but for K - 1 tokens at a tile's edge.  The episodes' beginnings
+// Bound by memory, 512 x 128 x 1024 bf16 forward in 59 us (4.6 TB/s; a copy reaches 4.8), backward in 99 us (4.1 TB/s, the vector
+// unit at it for most of the time), one token of 4096 x 1024 bf16 in 14 us (4.7 TB/s).  A lane keeps V neighbouring channels (one 16-byte access a token), a wave walks over a tile of tokens with the
+// last K of them in registers, so that every value is read once but for K - 1 tokens at a tile's edge (backward 2 K - 2).  The episodes' beginnings
 // of a tile are one 64-bit mask in scalar registers.
 #include "mws_common.hpp"
 

@@ -10,7 +10,8 @@
 // A lane is a channel with all its states in registers, so that a token's B and C are the same for the whole wave: they come in
 // scalar registers, from a small copy in float, [token][B | C][states], that `spread` makes first (128 bytes a token next to the
 // channels' 8 bytes each).  A wave walks along the time axis; u, dt, z and y are read and written in order of channels.
-// Bound by the vector unit: per value and state one exp and four multiplications or additions forward.
+// Bound by the vector unit: per value and state one exp (two issue slots) and four multiplications or additions forward, some 145
+// slots a token and wave with 16 states.  2048 x 64 x 512 x 16 bf16 forward in 303 us, 85 % of the slots taken; the memory would allow 140.
 //
 // Where batch x channels leave the card empty, the time axis is cut into segments of whole chunks: scan_segment takes each
 // segment's end state from zero and its sum of d (the product of its a is exp(A sum d)), scan_join runs over the segments, and the
@@ -418,9 +419,11 @@ template <int M> __device__ __forceinline__ float wave_sums(float (&v)[M / 2]) {
 // wave's channels token by token (wave_sums), over the block's waves after kKept tokens, over blocks by scan_bc_out.  Tokens past the
 // row's end count with d = u = dy = 0, which leaves g as it is and adds nothing.
 // More than 16 states are two halves (H = 2), each a wave's: what a token's gradients need of both, its output and two sums over the
-// states, meets in shared memory, and each of the two waves finishes every second token (405 x 66 x 874 x 32 bf16 4413 us with all
+// states, meets in shared memory, and each of the two waves finishes every second token (405 x 66 x 874 x 32 bf16 976 us; 4413 us with all
 // states in one wave, most of that for registers that do not fit).
-// Bound by the vector unit: 2048 x 64 x 512 x 16 bf16 take 1.28 ms, 440 instructions a token and wave, at 70 % of its issue slots.
+// Bound by the vector unit: 2048 x 64 x 512 x 16 bf16 take 1.22 ms, 392 instructions a token and wave (98 of them for the way there),
+// at 69 % of its issue slots with the two waves to a SIMD that the registers allow; three waves with half the tokens each, whose
+// registers spill, take 1.96 ms with the forward pass where these take 1.56 ms.
 template <class T, int NS, int H> __global__ __launch_bounds__(256, 2) void scan_backward(ScanArgs a) {
     using raw = typename T::raw;
     constexpr int SUB = kKept, M = 2 * NS, ALL = NS * H;
@@ -648,7 +651,7 @@ struct ScanOut {
 
 // ---- one token ----
 // Q lanes share a channel, four states each: the state goes through registers in 16-byte pieces, in order of memory.  Bound by memory:
-// 8 bytes a state.  Q = 0: a lane takes a channel's states one by one, for numbers of states that four lanes cannot share evenly.
+// 8 bytes a state (4096 x 1024 x 16 bf16 in 110 us, 5.2 TB/s).  Q = 0: a lane takes a channel's states one by one, for numbers of states that four lanes cannot share evenly.
 // A lane keeps its channel's parameters for up to kStepRows rows; a row's state is under way while the one before is worked on.
 constexpr int kStepRows = 4;
 template <class T, int Q> __global__ __launch_bounds__(256) void scan_step(ScanArgs a, const void *B, const void *C, int64_t B_batch, int64_t C_batch, int64_t each) {
@@ -709,7 +712,7 @@ template <class T, int Q> __global__ __launch_bounds__(256) void scan_step(ScanA
 
 // ---- host ----
 // The states that a lane walks with.  Powers of two where a backward pass follows, whose sums over a wave halve them step by step;
-// steps of four and eight where none does (3 x 5000 x 777 x 12 fp16 120 us, padded to 16 states 134 us).
+// steps of four and eight where none does (3 x 5000 x 777 x 12 fp16 116 us; padded to 16 states it was 134 us when this was 120).
 static int scan_ns(const mws_scan_args *a, bool backward) {
     int n = a->states;
     if (!backward && a->kept == nullptr && n > 8) return n <= 12 ? 12 : n <= 16 ? 16 : n <= 24 ? 24 : 32;
