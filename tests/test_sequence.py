@@ -519,6 +519,129 @@ def test_another_stream():
     assert torch.equal(got, want)
 
 
+@gpu
+def test_two_calls_at_once():
+    """on two streams, each with scratch memory of its own: the segments' states, partial sums and copies of one do not reach the other"""
+    gen = seeded(61)
+    sets = [[on(t, torch.float32, True) for t in scan_inputs(gen, 2, 900, 100, 16, torch.float32)] for _ in range(2)]
+    dy = torch.randn(2, 900, 100, device="cuda")
+
+    def once(ins):
+        y, last = sequence.selective_scan(*ins[:8], state=ins[8])
+        return [t.detach() for t in (y, last, *torch.autograd.grad((y, last), ins, (dy, torch.ones_like(last))))]
+
+    want = [once(ins) for ins in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for k in range(5):
+        for which in range(2):
+            with torch.cuda.stream(streams[which]):
+                got[which].append(once(sets[which]))
+    torch.cuda.synchronize()
+    for which in range(2):
+        for run in got[which]:
+            assert all(torch.equal(a, b) for a, b in zip(run, want[which]))
+
+
+@gpu
+def test_steps_in_a_graph():
+    """the state of a captured step goes on from replay to replay, with eager steps of the same state between"""
+    gen = seeded(62)
+    u, dt, A, B, C, D, z, bias, state = (on(t, torch.float32) for t in scan_inputs(gen, 30, 8, 70, 16, torch.float32))
+    w, line = torch.randn(70, 4, device="cuda"), torch.randn(30, 3, 70, device="cuda")
+    reset = torch.rand(30, 8, device="cuda") < 0.2
+    one = [t[:, 0].clone() for t in (u, dt, B, C, z, reset)]
+    h, l = state.clone(), line.clone()
+
+    def step(h, l):
+        v = sequence.causal_conv_step(one[0], w, state=l, reset=one[5])
+        return sequence.selective_scan_step(v, one[1], A, one[2], one[3], D, one[4], bias, state=h, reset=one[5])
+
+    with torch.no_grad():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(h.clone(), l.clone())
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(h, l)
+        h.copy_(state), l.copy_(line)
+        want_h, want_l = state.clone(), line.clone()
+        for t in range(8):
+            for k, x in enumerate((u, dt, B, C, z, reset)):
+                one[k].copy_(x[:, t])
+            want = step(want_h, want_l)
+            if t % 3 == 2:
+                got = step(h, l)
+            else:
+                graph.replay()
+                got = out
+            torch.cuda.synchronize()
+            assert torch.equal(got, want) and torch.equal(h, want_h) and torch.equal(l, want_l)
+
+
+@gpu
+def test_views_at_odd_addresses():
+    """every tensor one value behind an aligned address"""
+    gen = seeded(63)
+
+    def moved(t):
+        return torch.cat([t.new_zeros(1), t.reshape(-1)])[1:].view(t.shape)
+
+    for kind in TYPES:
+        ins = [on(t, kind if k in (0, 1, 3, 4, 6) else torch.float32) for k, t in enumerate(scan_inputs(gen, 3, 40, 72, 16, kind))]
+        off = [moved(t) for t in ins]
+        assert all(torch.equal(a, b) for a, b in zip(sequence.selective_scan(*ins[:8], state=ins[8]), sequence.selective_scan(*off[:8], state=off[8])))
+        w, b, line = torch.randn(72, 4, device="cuda"), torch.randn(72, device="cuda"), torch.randn(3, 3, 72, device="cuda").to(kind)
+        assert all(torch.equal(a, c) for a, c in zip(sequence.causal_conv(ins[0], w, b, state=line), sequence.causal_conv(off[0], moved(w), moved(b), state=moved(line))))
+        assert torch.equal(sequence.layer_norm(ins[0], b, b), sequence.layer_norm(off[0], moved(b), moved(b)))
+        with torch.no_grad():
+            h, g, l, m = ins[8].clone(), moved(ins[8]), line.clone(), moved(line)
+            one, two = ([t[k][:, 3] for k in (0, 1)] + [t[2]] + [t[k][:, 3] for k in (3, 4)] + [t[5], t[6][:, 3], t[7]] for t in (ins, off))
+            assert torch.equal(sequence.selective_scan_step(*one, state=h), sequence.selective_scan_step(*two, state=g)) and torch.equal(h, g)
+            assert torch.equal(sequence.causal_conv_step(ins[0][:, 3], w, b, state=l), sequence.causal_conv_step(off[0][:, 3], moved(w), moved(b), state=m)) and torch.equal(l, m)
+
+
+@gpu
+def test_tokens_far_apart():
+    """a time stride past what the scan's addresses hold is copied; below it, it is not"""
+    gen = seeded(64)
+    u, dt, A, B, C, D, z, bias, state = (on(t, torch.float32) for t in scan_inputs(gen, 1, 3, 8, 4, torch.float32))
+    want = sequence.selective_scan(u, dt, A, B, C, D, z, bias)
+    for stride in (1 << 26, (1 << 26) + 8):
+        room = torch.empty(2 * stride + 8, device="cuda")
+        far = room.as_strided((1, 3, 8), (0, stride, 1))
+        for k, tensors in enumerate(((far, dt, z), (u, far, z), (u, dt, far))):
+            far.copy_((u, dt, z)[k])
+            got = sequence.selective_scan(tensors[0], tensors[1], A, B, C, D, tensors[2], bias)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@gpu
+def test_more_values_than_32_bits_count():
+    """the last rows of tensors of more than 2^31 values, forward and backward, are those of the same rows at the front"""
+    batch, time, width = 2200, 1000, 1024
+    assert batch * time * width > 1 << 31
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    row = torch.randn(1, time, width, generator=gen, device="cuda").bfloat16()
+    x = torch.empty(batch, time, width, dtype=torch.bfloat16, device="cuda").copy_(row.expand(batch, time, width))
+    x[1] *= 0.5
+    x[-2:] = x[:2]
+    x.requires_grad_()
+    w = torch.randn(width, 4, generator=gen, device="cuda")
+    A, bias = -torch.rand(width, 4, generator=gen, device="cuda") - 0.1, torch.full((width,), -2.0, device="cuda")
+    pair = torch.randn(batch, time, 8, generator=gen, device="cuda").bfloat16()
+    pair[-2:] = pair[:2]
+    for f in (lambda: sequence.layer_norm(x), lambda: sequence.causal_conv(x, w)[0], lambda: sequence.selective_scan(x, x, A, pair[..., :4], pair[..., 4:], dt_bias=bias)[0]):
+        y = f()
+        dx, = torch.autograd.grad(y, x, x.detach())
+        for t in (y, dx):
+            assert torch.equal(t[-2:], t[:2]) and torch.isfinite(t[-2:]).all() and t[-1].abs().sum() > 0 and not torch.equal(t[-1], t[-2])
+        del y, dx, t
+    torch.cuda.empty_cache()
+
+
 def layer(p, x, reset, conv_state, scan_state):
     """one layer of a policy with memory, as recurrent_policy has it"""
     n = sequence.layer_norm(x, p["w"], p["b"])
