@@ -20,13 +20,15 @@ container); nothing here travels to the GPU box except the fixtures it produced.
 from __future__ import annotations
 
 import enum
+import os
 import sys
 import time
 import types
 
 import numpy as np
 
-REFERENCE_ROOT = "/root/reference"
+# a checkout without the package (an empty folder) is none: then this names the missing package, which no caller takes for a folder
+REFERENCE_ROOT = "/root/reference" if os.path.isdir("/root/reference/metaworld") else "/root/reference/metaworld"
 
 
 # =============================================================================
@@ -669,7 +671,6 @@ def install(reference_root=REFERENCE_ROOT):
     global _installed
     if _installed:
         return
-    import os
     if not os.path.isdir(os.path.join(reference_root, "metaworld")):
         raise RuntimeError(f"reference sources not found under {reference_root}")
     mj = _make_mujoco()
