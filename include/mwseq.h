@@ -15,6 +15,8 @@
  * Tokens are [batch, length].  `reset` (uint8 [batch, length] by strides, may be NULL): non-zero where an episode begins, so that
  * neither the state nor any earlier token of the row is seen from there on.  `lengths` (int32 [batch], may be NULL): how many
  * tokens of a row count, taken into [0, length]; outputs and gradients of the others are zero, their inputs are not used.
+ *
+ * Sizes of which one launch would need 2^32 threads or more (2^26 rows of one token, 2^27 tokens of 16 states backward) are refused.
  */
 #ifndef MWSEQ_H
 #define MWSEQ_H

@@ -161,5 +161,7 @@ inline int32_t launched(const char *what) {
     return MWS_LAUNCH;
 }
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+// a launch counts its threads along an axis in 32 bits, its blocks in 31
+inline bool fits(int64_t blocks, int threads) { return blocks <= 0x7fffffff && blocks * threads <= 0xffffffffLL; }
 
 }  // namespace mws

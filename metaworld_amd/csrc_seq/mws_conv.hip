@@ -410,6 +410,15 @@ static int32_t conv_check(const mws_conv_args *a, const char *what, bool backwar
     return 0;
 }
 
+// whether the launches can count their threads
+static int32_t conv_fits(const mws_conv_args *a, const char *what, bool backward, bool step) {
+    const int v = step && a->width % conv_v(a) != 0 ? 1 : conv_v(a);
+    bool all = step       ? fits(ceil_div(step_lanes(a->batch, ceil_div(a->width, v), kStepRows) * ceil_div(a->width, v), 256), 256)
+               : backward ? fits(ceil_div((int64_t)(a->taps + 1) * a->width, 32), 1024)
+                          : fits(ceil_div(a->batch * conv_tiles(a), 4), 256);
+    return all ? 0 : fail("%s: %lld rows of %lld tokens and %d channels are more than one launch can count", what, (long long)a->batch, (long long)a->length, a->width);
+}
+
 static ConvArgs conv_device(const mws_conv_args *a) {
     ConvArgs d = {};
     d.x = a->x, d.weight = a->weight, d.bias = a->bias, d.state = a->state, d.dy = a->dy, d.dlast = a->dlast;
@@ -461,6 +470,7 @@ using namespace mws;
 extern "C" int32_t mws_conv_forward(const mws_conv_args *a, void *stream) {
     if (int32_t e = conv_check(a, "mws_conv_forward", false, false)) return e;
     if (a->batch == 0) return 0;
+    if (int32_t e = conv_fits(a, "mws_conv_forward", false, false)) return e;
     conv_run(a, conv_device(a), kForward, (hipStream_t)stream);
     return launched("mws_conv_forward");
 }
@@ -474,6 +484,7 @@ extern "C" int32_t mws_conv_backward(const mws_conv_args *a, void *stream) {
     if (int32_t e = conv_check(a, "mws_conv_backward", true, false)) return e;
     int64_t need = mws_conv_workspace(a);
     if (a->workspace_bytes < need || (need > 0 && a->workspace == nullptr)) return fail("mws_conv_backward: the workspace needs %lld bytes", (long long)need);
+    if (int32_t e = conv_fits(a, "mws_conv_backward", true, false)) return e;
     ConvArgs d = conv_device(a);
     bool params = a->dweight != nullptr || a->dbias != nullptr;
     d.part = params ? (float *)a->workspace : nullptr;
@@ -489,6 +500,7 @@ extern "C" int32_t mws_conv_backward(const mws_conv_args *a, void *stream) {
 extern "C" int32_t mws_conv_step(const mws_conv_args *a, void *stream) {
     if (int32_t e = conv_check(a, "mws_conv_step", false, true)) return e;
     if (a->batch == 0) return 0;
+    if (int32_t e = conv_fits(a, "mws_conv_step", false, true)) return e;
     conv_run(a, conv_device(a), kStep, (hipStream_t)stream);
     return launched("mws_conv_step");
 }

@@ -867,9 +867,19 @@ static void scan_run(const mws_scan_args *a, const ScanPlan &p, const ScanArgs &
     else if (a->type == MWS_BF16) scan_go<BF16>(a, p, d, backward, stream);
     else scan_go<F16>(a, p, d, backward, stream);
 }
+static int step_lanes_of(const mws_scan_args *a) { return a->states == 4 ? 1 : a->states == 8 ? 2 : a->states == 16 ? 4 : a->states == 32 ? 8 : 0; }
+static int64_t step_rows(const mws_scan_args *a, int64_t &lanes) {
+    int q = step_lanes_of(a);
+    lanes = (int64_t)a->width * (q > 0 ? q : 1);
+    return step_lanes(a->batch, lanes, kStepRows);
+}
+static int64_t step_blocks(const mws_scan_args *a) {
+    int64_t lanes, each = step_rows(a, lanes);
+    return ceil_div(each * lanes, 256);
+}
 template <class T> static void step_go(const mws_scan_args *a, const ScanArgs &d, hipStream_t stream) {
-    int q = a->states == 4 ? 1 : a->states == 8 ? 2 : a->states == 16 ? 4 : a->states == 32 ? 8 : 0;
-    int64_t lanes = (int64_t)d.width * (q > 0 ? q : 1), each = step_lanes(d.batch, lanes, kStepRows);
+    int q = step_lanes_of(a);
+    int64_t lanes, each = step_rows(a, lanes);
     dim3 grid((unsigned)ceil_div(each * lanes, 256));
 #define MWS_GO(Q) hipLaunchKernelGGL((scan_step<T, Q>), grid, dim3(256), 0, stream, d, a->B, a->C, a->B_batch, a->C_batch, each)
     if (q == 1) MWS_GO(1);
@@ -898,8 +908,10 @@ static int32_t scan_call(const mws_scan_args *a, const char *what, bool backward
     ScanPlan p = scan_plan(a, backward);
     if (a->workspace_bytes < p.bytes || (p.bytes > 0 && a->workspace == nullptr)) return fail("%s: the workspace needs %lld bytes", what, (long long)p.bytes);
     if (!backward && a->batch == 0) return 0;
-    if (a->batch * p.segments * p.across > 0x7fffffff || ceil_div(a->batch * a->length * 2 * p.ns, 256) > 0x7fffffff || ceil_div(a->batch * p.ns * a->width, 256) > 0x7fffffff)
-        return fail("%s: too many rows", what);
+    const int64_t tokens = a->batch * a->length;
+    if (!fits(a->batch * p.segments * p.across, p.lanes) || (backward && !fits(ceil_div(tokens * 2 * p.ns, 256), 256)) || !fits(ceil_div(a->length * 2 * p.ns / 4, 256), 256) ||
+        (p.segments > 1 && !fits(ceil_div(a->batch * p.ns * a->width, 256), 256)) || !fits(ceil_div((int64_t)(p.ns + 2) * a->width, 32), 1024))
+        return fail("%s: %lld rows of %lld tokens, %d channels and %d states are more than one launch can count", what, (long long)a->batch, (long long)a->length, a->width, a->states);
     scan_run(a, p, scan_device(a, p), backward, (hipStream_t)stream);
     return launched(what);
 }
@@ -909,6 +921,7 @@ extern "C" int32_t mws_scan_backward(const mws_scan_args *a, void *stream) { ret
 extern "C" int32_t mws_scan_step(const mws_scan_args *a, void *stream) {
     if (int32_t e = scan_check(a, "mws_scan_step", false, true, true)) return e;
     if (a->batch == 0) return 0;
+    if (!fits(step_blocks(a), 256)) return fail("mws_scan_step: %lld rows of %d channels are more than one launch can count", (long long)a->batch, a->width);
     ScanPlan none = {};
     ScanArgs d = scan_device(a, none);
     if (a->type == MWS_F32) step_go<F32>(a, d, (hipStream_t)stream);

@@ -41,7 +41,7 @@ void want(const char *what, const Tensor &t, at::IntArrayRef shape, at::ScalarTy
 void want_gpu(const char *what, const Tensor &t) { TORCH_CHECK_VALUE(t.is_cuda(), what, " is on ", t.device(), ": the kernels run on a GPU and there is no CPU fallback"); }
 void want_state(const char *what, const Tensor &t) {
     TORCH_CHECK_TYPE(t.defined(), what, ": state has to be a tensor");
-    TORCH_CHECK_VALUE(t.is_contiguous(), "state has to be contiguous: it is updated in place");
+    TORCH_CHECK_VALUE(t.is_contiguous() && !t.is_neg(), "state has to be contiguous: it is updated in place");
 }
 void want_tokens(const Tensor &x, bool time, const Tensor &reset, const Tensor &lengths) {
     if (reset.defined()) {
@@ -54,8 +54,9 @@ void want_tokens(const Tensor &x, bool time, const Tensor &reset, const Tensor &
 }
 
 // ---- launches ----
-Tensor rows(const Tensor &t) { return !t.defined() || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
-Tensor dense(const Tensor &t) { return t.defined() ? t.contiguous() : t; }
+// (a lazily negated view's memory holds the values without their sign)
+Tensor rows(const Tensor &t) { return !t.defined() || ((t.stride(-1) == 1 || t.size(-1) == 1) && !t.is_neg()) ? t : t.resolve_neg().contiguous(); }
+Tensor dense(const Tensor &t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
 Tensor near(const Tensor &t) { return !t.defined() || (t.dim() == 3 && t.stride(1) > MWS_SCAN_MAX_STRIDE) ? dense(t) : rows(t); }
 Tensor like(const Tensor &t) { return t.defined() ? at::empty(t.sizes(), t.options()) : t; }
 void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -73,10 +74,11 @@ template <class F, class A> void launch(F f, const A &a, const Tensor &x) {
 }
 Tensor scratch(int64_t bytes, const Tensor &x) { return at::empty({bytes}, x.options().dtype(at::kByte)); }
 
+// whether derivatives are asked for: backward ones, or forward ones, which the autograd functions refuse
 bool records(std::initializer_list<Tensor> all) {
-    if (!at::GradMode::is_enabled()) return false;
+    const bool grads = at::GradMode::is_enabled();
     for (const Tensor &t : all)
-        if (t.defined() && t.requires_grad()) return true;
+        if (t.defined() && ((grads && t.requires_grad()) || t._fw_grad(0).defined())) return true;
     return false;
 }
 void want_acting(const char *what, std::initializer_list<Tensor> all) {
@@ -207,7 +209,7 @@ variable_list causal_conv(Tensor x, Tensor weight, const Maybe &bias_, const May
     conv_check(x, weight, bias, state, 3);
     want_tokens(x, true, reset, lengths);
     want_gpu("x", x);
-    x = rows(x), weight = weight.contiguous(), bias = rows(bias), state = dense(state), lengths = dense(lengths);
+    x = rows(x), weight = dense(weight), bias = rows(bias), state = dense(state), lengths = dense(lengths);
     return records({x, weight, bias, state}) ? CausalConv::apply(x, weight, maybe(bias), maybe(state), maybe(reset), maybe(lengths), needs({x, weight, bias, state})) : conv_forward(x, weight, bias, state, reset, lengths);
 }
 Tensor causal_conv_step(Tensor x, Tensor weight, const Maybe &bias_, const Maybe &state_, const Maybe &reset_) {
@@ -217,7 +219,7 @@ Tensor causal_conv_step(Tensor x, Tensor weight, const Maybe &bias_, const Maybe
     want_state("causal_conv_step", state);
     want_gpu("x", x);
     want_acting("causal_conv_step", {x, weight, bias, state});
-    x = rows(x), weight = weight.contiguous(), bias = rows(bias);
+    x = rows(x), weight = dense(weight), bias = rows(bias);
     Tensor y = at::empty(x.sizes(), x.options());
     mws_conv_args a = conv_args(x, weight, bias, state, reset, Tensor());
     a.y = ptr(y), a.last = ptr(state);
@@ -304,7 +306,7 @@ ScanIn scan_check(const Tensor &u, const Tensor &dt, const Tensor &A, const Tens
     return t;
 }
 void scan_rows(ScanIn &t) {
-    t.u = near(t.u), t.dt = near(t.dt), t.B = rows(t.B), t.C = rows(t.C), t.D = rows(t.D), t.z = near(t.z), t.dt_bias = rows(t.dt_bias), t.A = t.A.contiguous();
+    t.u = near(t.u), t.dt = near(t.dt), t.B = rows(t.B), t.C = rows(t.C), t.D = rows(t.D), t.z = near(t.z), t.dt_bias = rows(t.dt_bias), t.A = dense(t.A);
 }
 variable_list selective_scan(const Tensor &u, const Tensor &dt, const Tensor &A, const Tensor &B, const Tensor &C, const Maybe &D, const Maybe &z, const Maybe &dt_bias, const Maybe &state,
                              const Maybe &reset, const Maybe &lengths) {

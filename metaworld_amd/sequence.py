@@ -13,7 +13,8 @@ include/mwseq.h), their torch side in _sequence.so; without them, or on CPU tens
 Tokens are [batch, time].  `reset` (bool or uint8, [batch, time]) is true at an episode's first token, from which on neither the
 state nor earlier tokens are seen.  `lengths` (int32 [batch]) says how many tokens of a padded row count, taken into 0 .. time: the
 others' inputs are not looked at, their outputs and gradients are zero, and the returned state is that after the last token that
-counts.  Gradients are deterministic (no atomic additions) and not differentiable again (create_graph is refused).
+counts.  Gradients are deterministic (no atomic additions) and not differentiable again (create_graph is refused, as are forward
+derivatives).
 """
 from __future__ import annotations
 

@@ -739,6 +739,44 @@ def test_what_autograd_refuses():
 
 
 @gpu
+def test_lazily_negated_views_keep_their_sign():
+    """views (as the imaginary part of a conjugate is one) whose memory holds the values with the other sign"""
+    gen = seeded(71)
+    plain = on(rand(gen, 3, 9, 20), torch.float32)
+    x = torch._neg_view(-plain)
+    w, A, s = on(rand(gen, 20, 4), torch.float32), -on(rand(gen, 20, 4).abs(), torch.float32), on(rand(gen, 3, 9, 4), torch.float32)
+    assert x.is_neg() and x.is_contiguous() and torch.equal(x, plain)
+    with torch.no_grad():
+        for t in (x, plain):
+            got = sequence.layer_norm(t), *sequence.causal_conv(t, w), *sequence.selective_scan(t, t, A, s, s, None, t)
+            want = got if t is x else want
+            if t is plain:
+                assert all(torch.equal(g, v) for g, v in zip(got, want))
+        state = torch._neg_view(torch.zeros(3, 3, 20, device="cuda"))
+        with pytest.raises(ValueError, match="contiguous"):
+            sequence.causal_conv_step(plain[:, 0], w, state=state)
+    # as an incoming gradient
+    leaf = plain.clone().requires_grad_()
+    grads = [torch.autograd.grad((sequence.layer_norm(leaf), sequence.causal_conv(leaf, w)[0], sequence.selective_scan(leaf, leaf, A, s, s)[0]), leaf, (t, t, t))[0] for t in (x, plain)]
+    assert torch.equal(*grads)
+
+
+@gpu
+def test_forward_derivatives_are_refused():
+    """they would be dropped without a word where nothing asks for backward ones"""
+    gen = seeded(73)
+    x, w, A, s = (on(rand(gen, *shape), torch.float32) for shape in ((2, 3, 8), (8, 4), (8, 4), (2, 3, 4)))
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: sequence.layer_norm(d), lambda: sequence.causal_conv(d, w), lambda: sequence.selective_scan(d, x, A, s, s),
+                     lambda: sequence.causal_conv_step(d[:, 0], w, state=torch.zeros(2, 3, 8, device="cuda")),
+                     lambda: sequence.selective_scan_step(d[:, 0], x[:, 0], A, s[:, 0], s[:, 0], state=torch.zeros(2, 8, 4, device="cuda"))):
+            with pytest.raises(RuntimeError):
+                call()
+
+
+@gpu
 def test_results_do_not_vary():
     gen = seeded(12)
     ins = [on(t, torch.float32, True) for t in scan_inputs(gen, 9, 100, 200, 16, torch.float32)]
@@ -854,6 +892,21 @@ def test_the_library_refuses_what_a_binding_may_get_wrong():
     assert lib.mws_scan_step(scan(length=3), None) == -1 and "one token" in lib.mws_last_error().decode()
     assert lib.mws_scan_workspace(scan(batch=2, length=7), 0) >= 2 * 7 * 32 * 4 and lib.mws_scan_kept(scan(batch=2, length=33)) == 2 * -(-33 // 8) * 16 * 4          # before every 8th token
     assert lib.mws_sizeof(0) == NORM.size and lib.mws_sizeof(3) == -1
+
+
+def test_more_threads_than_a_launch_counts_are_refused():
+    """2^32 threads along an axis: the library says so before it launches anything (here there is nothing to launch on)"""
+    lib = sequence.library()
+
+    def conv(batch, length, width):
+        return CONV.pack(*[64] * 6, 0, 0, *[64] * 7, batch, length, *[0] * 6, 1 << 60, width, 4, 1, 0)
+
+    def scan(batch, length, width, states):
+        return SCAN.pack(*[64] * 11, 0, 0, *[64] * 13, batch, length, *[0] * 14, 1 << 60, width, states, 1, 0)
+    # a wave for each row's tokens; rows x channels; the gradients of B and C by the token, of A by channel and state
+    for f, args in ((lib.mws_conv_forward, conv(1 << 26, 1, 8)), (lib.mws_conv_step, conv(1 << 27, 1, 2048)), (lib.mws_scan_forward, scan(1 << 26, 1, 8, 16)), (lib.mws_scan_step, scan(1 << 23, 1, 2048, 3)),
+                    (lib.mws_scan_backward, scan(1 << 17, 1 << 10, 8, 16)), (lib.mws_scan_backward, scan(1, 1, (1 << 22) - 64, 32))):
+        assert f(args, None) == -1 and "count" in lib.mws_last_error().decode()
 
 
 def test_without_the_library_it_says_how_to_build_it(monkeypatch, tmp_path):
