@@ -117,13 +117,28 @@ template <class T, int NS> __global__ __launch_bounds__(256) void spread(const v
 // space says, so that they are scalar loads
 using Fixed = const __attribute__((address_space(4))) float;
 __device__ __forceinline__ Fixed *fixed(const float *p) { return (Fixed *)(uintptr_t)p; }
-template <int NS> struct Pair {
-    float B[NS], C[NS];
-    __device__ __forceinline__ void read(Fixed *p, int all = NS) {
+//
+// They are asked for one step ahead: a step's values are in `hold`'s registers when the next step's loads go out, which then have that
+// step's time to arrive (scalar loads may overtake each other, so that a wait is for all of them).  A step is some of a token's states
+// of B and C (half of 16), or a whole token's of one of them, since the scalar registers hold no more.  (2048 x 64 x 512 x 16 bf16 with the
+// backward pass 1448 us, 1564 us with a token's values asked for where they are needed; 3 x 5000 x 777 x 12 fp16 109 us, not 117.)
+template <int S> struct Pair {
+    float B[S], C[S];
+    __device__ __forceinline__ void read(Fixed *p, int all) {
 #pragma unroll
-        for (int n = 0; n < NS; n++) B[n] = p[n], C[n] = p[all + n];
+        for (int n = 0; n < S; n++) B[n] = p[n], C[n] = p[all + n];
     }
+    __device__ __forceinline__ void hold() const { asm volatile("" ::"s"(B[0]), "s"(C[0])); }
 };
+template <int S> struct One {
+    float v[S];
+    __device__ __forceinline__ void read(Fixed *p) {
+#pragma unroll
+        for (int n = 0; n < S; n++) v[n] = p[n];
+    }
+    __device__ __forceinline__ void hold() const { asm volatile("" ::"s"(v[0])); }
+};
+__device__ __forceinline__ void here_only() { __builtin_amdgcn_sched_barrier(0); }      // nothing moves past this
 
 // a lane's states: NS of them from `first` on, of `all` in a row (padded with zeros)
 template <int NS> __device__ __forceinline__ void rates(const ScanArgs &a, uint32_t e, float (&A2)[NS], int first = 0) {       // A / ln 2, for exp2
@@ -177,7 +192,8 @@ struct Place {          // what a block of the grid works on
     }
 };
 
-template <class T, int NS> __global__ __launch_bounds__(256) void scan_forward(ScanArgs a) {
+constexpr int forward_waves(int ns) { return ns <= 8 ? 8 : ns <= 12 ? 7 : ns <= 16 ? 6 : ns <= 24 ? 4 : 3; }         // of a SIMD: the compiler takes more registers than it needs
+template <class T, int NS> __global__ __launch_bounds__(256, forward_waves(NS)) void scan_forward(ScanArgs a) {
     using raw = typename T::raw;
     constexpr int G = 4;
     Place p(a, blockIdx.x / a.across, blockIdx.x % a.across);
@@ -195,16 +211,29 @@ template <class T, int NS> __global__ __launch_bounds__(256) void scan_forward(S
         const raw *z = a.z != nullptr ? (const raw *)a.z + p.b * a.z_batch + p.t0 * a.z_time : nullptr;
         Fixed *bc = fixed(a.bc + (p.b * a.length + p.t0) * 2 * NS);
         float *kept = a.kept != nullptr ? a.kept + (p.b * a.chunks + p.t0 / kKept) * NS * a.width : nullptr;
+        constexpr int P = NS > 16 ? 4 : 2, S = NS / P;
+        Pair<S> m[2];
+        m[0].read(bc, NS);                           // (behind the last token: the next row's, or the workspace's padding)
         auto token = [&](raw ru, raw rd, raw rz, bool first, const Line<raw> &out, int q) __attribute__((always_inline)) {
-            Pair<NS> m;
-            m.read(bc);
-            float uf = up<T>(ru), d = softplus_(up<T>(rd) + bias), du = d * uf, o = D * uf, o2 = 0;
-            if (first) forget<NS>(h);
+            float uf = 0, d = 0, du = 0, o = 0, o2 = 0;
 #pragma unroll
-            for (int n = 0; n < NS; n++) {
-                h[n] = __builtin_fmaf(exp2_(d * A2[n]), h[n], du * m.B[n]);
-                if (n & 1) o2 = __builtin_fmaf(m.C[n], h[n], o2);
-                else o = __builtin_fmaf(m.C[n], h[n], o);
+            for (int k = 0; k < P; k++) {
+                m[k & 1].hold();
+                if (k + 1 == P) bc += 2 * NS;
+                m[~k & 1].read(bc + (k + 1) % P * S, NS);
+                here_only();
+                if (k == 0) {
+                    uf = up<T>(ru), d = softplus_(up<T>(rd) + bias), du = d * uf, o = D * uf;
+                    if (first) forget<NS>(h);
+                }
+#pragma unroll
+                for (int i = 0; i < S; i++) {
+                    const int n = k * S + i;
+                    h[n] = __builtin_fmaf(exp2_(d * A2[n]), h[n], du * m[k & 1].B[i]);
+                    if (n & 1) o2 = __builtin_fmaf(m[k & 1].C[i], h[n], o2);
+                    else o = __builtin_fmaf(m[k & 1].C[i], h[n], o);
+                }
+                here_only();
             }
             o += o2;
             if (z != nullptr) {
@@ -212,8 +241,7 @@ template <class T, int NS> __global__ __launch_bounds__(256) void scan_forward(S
                 o *= zf * sigmoid_(zf);
             }
             out.put(down<T>(o), bytes, q);
-            bc += 2 * NS;
-            __builtin_amdgcn_sched_barrier(0);       // the next token's scalar loads do not fit beside this one's
+            here_only();
         };
         for (int64_t c0 = p.t0; c0 < stop; c0 += kGroup) {
             uint32_t begins = group_mask(a, p.b, c0, p.end);
@@ -260,6 +288,8 @@ template <class T, int NS> __global__ __launch_bounds__(256) void scan_segment(S
     float bias = a.dt_bias != nullptr ? a.dt_bias[p.e] : 0.0f;
     const raw *u = (const raw *)a.u + p.b * a.u_batch + p.t0 * a.u_time, *dt = (const raw *)a.dt + p.b * a.dt_batch + p.t0 * a.dt_time;
     Fixed *bc = fixed(a.bc + (p.b * a.length + p.t0) * 2 * NS);
+    One<NS> B[2];
+    B[0].read(bc);
     for (int64_t c0 = p.t0; c0 < p.t1; c0 += kGroup) {        // whole groups: the row goes on behind the segment
         uint32_t begins = group_mask(a, p.b, c0, p.end);
         cut = cut || begins != 0;
@@ -270,13 +300,16 @@ template <class T, int NS> __global__ __launch_bounds__(256) void scan_segment(S
             for (int q = 0; q < G; q++) ru[q] = lu.get(bytes, q), rd[q] = ld.get(bytes, q);
 #pragma unroll
             for (int q = 0; q < G; q++) {
+                B[q & 1].hold();
+                bc += 2 * NS;
+                B[~q & 1].read(bc);
+                here_only();
                 float d = softplus_(up<T>(rd[q]) + bias), x = d * up<T>(ru[q]);
                 sum += d;
                 if (begins >> q & 1) forget<NS>(h);
 #pragma unroll
-                for (int n = 0; n < NS; n++) h[n] = __builtin_fmaf(exp2_(d * A2[n]), h[n], x * bc[n]);
-                bc += 2 * NS;
-                __builtin_amdgcn_sched_barrier(0);
+                for (int n = 0; n < NS; n++) h[n] = __builtin_fmaf(exp2_(d * A2[n]), h[n], x * B[q & 1].v[n]);
+                here_only();
             }
             begins >>= G;
             u += G * a.u_time, dt += G * a.dt_time;
@@ -314,6 +347,8 @@ template <class T, int NS> __global__ __launch_bounds__(256) void scan_segment_b
                 lz((const raw *)a.z, p.b * a.z_batch + t * a.z_time, a.z_time);
             Fixed *bc = fixed(a.bc + (p.b * a.length + t) * 2 * NS);
             raw rd[G], ry[G], rz[G];
+            One<NS> C[2];
+            C[(G - 1) & 1].read(bc + (G * 2 - 1) * NS);
             const int here = count - i < G ? count - i : G;
 #pragma unroll
             for (int q = 0; q < G; q++) {
@@ -322,6 +357,9 @@ template <class T, int NS> __global__ __launch_bounds__(256) void scan_segment_b
             }
 #pragma unroll
             for (int q = G - 1; q >= 0; q--) {
+                C[q & 1].hold();
+                if (q > 0) C[~q & 1].read(bc + (q * 2 - 1) * NS);
+                here_only();
                 if (q >= here) continue;
                 float d = softplus_(up<T>(rd[q]) + bias), o = up<T>(ry[q]);
                 if (gated) {
@@ -329,11 +367,10 @@ template <class T, int NS> __global__ __launch_bounds__(256) void scan_segment_b
                     o *= zf * sigmoid_(zf);
                 }
                 sum += d;
-                Fixed *C = bc + (q * 2 + 1) * NS;
 #pragma unroll
-                for (int n = 0; n < NS; n++) g[n] = exp2_(d * A2[n]) * __builtin_fmaf(o, C[n], g[n]);
+                for (int n = 0; n < NS; n++) g[n] = exp2_(d * A2[n]) * __builtin_fmaf(o, C[q & 1].v[n], g[n]);
                 if (begins >> (i + q) & 1) forget<NS>(g);
-                __builtin_amdgcn_sched_barrier(0);
+                here_only();
             }
         }
     }
@@ -419,11 +456,11 @@ template <int M> __device__ __forceinline__ float wave_sums(float (&v)[M / 2]) {
 // wave's channels token by token (wave_sums), over the block's waves after kKept tokens, over blocks by scan_bc_out.  Tokens past the
 // row's end count with d = u = dy = 0, which leaves g as it is and adds nothing.
 // More than 16 states are two halves (H = 2), each a wave's: what a token's gradients need of both, its output and two sums over the
-// states, meets in shared memory, and each of the two waves finishes every second token (405 x 66 x 874 x 32 bf16 976 us; 4413 us with all
+// states, meets in shared memory, and each of the two waves finishes every second token (405 x 66 x 874 x 32 bf16 900 us; four times that with all
 // states in one wave, most of that for registers that do not fit).
-// Bound by the vector unit: 2048 x 64 x 512 x 16 bf16 take 1.22 ms, 392 instructions a token and wave (98 of them for the way there),
-// at 69 % of its issue slots with the two waves to a SIMD that the registers allow; three waves with half the tokens each, whose
-// registers spill, take 1.96 ms with the forward pass where these take 1.56 ms.
+// Bound by the vector unit: 2048 x 64 x 512 x 16 bf16 take 1.08 ms, 402 instructions a token and wave (98 of them for the way there),
+// at 80 % of its issue slots with the two waves to a SIMD that the registers allow; three waves with half the tokens each, whose
+// registers spill, took a quarter longer.
 template <class T, int NS, int H> __global__ __launch_bounds__(256, 2) void scan_backward(ScanArgs a) {
     using raw = typename T::raw;
     constexpr int SUB = kKept, M = 2 * NS, ALL = NS * H;
@@ -469,47 +506,58 @@ template <class T, int NS, int H> __global__ __launch_bounds__(256, 2) void scan
                 }
                 early[0] = ld.get(bytes, here - 1), early[1] = ly.get(bytes, here - 1), early[2] = lz.get(bytes, here - 1), early[3] = lu.get(bytes, here - 1);
                 Fixed *bc = fixed(in->bc + (p.b * in->length + t) * 2 * ALL + first_n);
+                constexpr int S = NS / 2;
+                One<NS> B[2];
+                Pair<S> m, m2;
+                auto token = [&](int q) __attribute__((always_inline)) { return bc + (q < here ? q : here - 1) * 2 * ALL; };
+                B[0].read(token(0));
 #pragma unroll
                 for (int q = 0; q < SUB; q++) {
-                    if (q % 2 == 0) asm volatile("" : "+s"(bc), "+s"(here), "+s"(begins));         // two tokens' B at a time, and no comparison held for later
-                    Fixed *m = bc + (q < here ? q : here - 1) * 2 * ALL;
+                    B[q & 1].hold();
+                    asm volatile("" : "+s"(bc), "+s"(here), "+s"(begins));         // no comparison held for later, no B kept for the way back
+                    if (q + 1 < SUB) B[~q & 1].read(token(q + 1));
+                    else m.read(token(q), ALL);
+                    here_only();
                     d[q] = q < here ? softplus_(up<T>(rd[q]) + bias) : 0.0f;
                     float x = q < here ? d[q] * up<T>(ru[q]) : 0.0f;
                     if (begins >> q & 1) forget<NS>(h);
 #pragma unroll
                     for (int n = 0; n < NS; n++) {
                         keep[q][n] = exp2_(d[q] * A2[n]) * h[n];
-                        h[n] = __builtin_fmaf(x, m[n], keep[q][n]);
+                        h[n] = __builtin_fmaf(x, B[q & 1].v[n], keep[q][n]);
                         if (n % 4 == 3)
 #pragma unroll
                             for (int k = n - 3; k <= n; k++) asm volatile("" : "+v"(keep[q][k]), "+v"(h[k]));
                     }
-                    __builtin_amdgcn_sched_barrier(0);
+                    here_only();
                 }
-                // from here on the compiler does not know d and bc: it would rather keep every exp, state and B of the walk before
-                // (2 x SUB x NS vector and SUB x NS scalar registers more) than take them again
+                // from here on the compiler does not know d: it would rather keep every exp and state of the walk before (2 x SUB x NS
+                // registers more) than take them again
 #pragma unroll
                 for (int q = 0; q < SUB; q++) asm volatile("" : "+v"(d[q]));
-                asm volatile("" : "+s"(bc));
                 float *to = sums + (turn * waves + wave) * SUB * M;
                 float *others = meet + (turn * waves + wave) * SUB * 3 * kWave + lane;
                 FixedArgs *out_to = fresh_args();
                 const int64_t row = (p.b * out_to->length + t) * out_to->width;
                 Line<raw> gu((raw *)out_to->du, row, out_to->width), gd((raw *)out_to->ddt, row, out_to->width), gz((raw *)out_to->dz, row, out_to->width);
-                // a token's gradients from its sums over all states
+                // a token's gradients from its sums over all states.  Without branches: where one path stores and the other does not, the
+                // wait for the next token's inputs would be one for the stores as well (without z the last store goes nowhere; 1427 us
+                // with the forward pass, 1450 us with a branch).
                 auto finish = [&](int q, float out, float zf, float sig, float o, float y, float gB, float gk, float raw_d, float dq, float uq) __attribute__((always_inline)) {
-                    float dd = __builtin_fmaf(uq, gB, gk * kLn2), draw = dd * sigmoid_(raw_d);
+                    float dd = __builtin_fmaf(uq, gB, gk * kLn2), draw = q < here ? dd * sigmoid_(raw_d) : 0.0f;
+                    const uint32_t where = q < here ? bytes : kOutside;
                     dD = __builtin_fmaf(o, uq, dD);
                     dbias += draw;
-                    gu.put(down<T>(__builtin_fmaf(D, o, dq * gB)), bytes, q);
-                    gd.put(down<T>(draw), bytes, q);
-                    if (gated) gz.put(down<T>(out * __builtin_fmaf(D, uq, y) * sig * (1.0f + zf * (1.0f - sig))), bytes, q);
+                    gu.put(down<T>(__builtin_fmaf(D, o, dq * gB)), where, q);
+                    gd.put(down<T>(draw), where, q);
+                    gz.put(down<T>(out * __builtin_fmaf(D, uq, y) * sig * (1.0f + zf * (1.0f - sig))), where, q);
                 };
 #pragma unroll
                 for (int q = SUB - 1; q >= 0; q--) {
                     asm volatile("" : "+s"(here), "+s"(begins));
-                    Pair<NS> m;
-                    m.read(bc + (q < here ? q : here - 1) * 2 * ALL, ALL);
+                    m.hold();
+                    m2.read(token(q) + S, ALL);
+                    here_only();
                     float raw_d = up<T>(early[0]) + bias, out = q < here ? up<T>(early[1]) : 0.0f, uq = q < here ? up<T>(early[3]) : 0.0f, zf = 0, gate = 1, sig = 0;
                     if (gated) {
                         zf = up<T>(early[2]);
@@ -523,16 +571,23 @@ template <class T, int NS, int H> __global__ __launch_bounds__(256, 2) void scan
                     float o = out * gate, x = d[q] * uq, gB = 0, gk = 0, y = 0, v[NS];
 #pragma unroll
                     for (int n = 0; n < NS; n++) {
+                        if (n == S) {
+                            here_only();
+                            m2.hold();
+                            if (q > 0) m.read(token(q - 1), ALL);
+                            here_only();
+                        }
+                        const float Bn = n < S ? m.B[n % S] : m2.B[n % S], Cn = n < S ? m.C[n % S] : m2.C[n % S];
                         // four states at a time, their sums added up here and not when they are next asked for: what the compiler
                         // would keep for later does not fit the registers
                         if (n % 4 == 0)
 #pragma unroll
                             for (int k = n; k < n + 4; k++) asm volatile("" : "+v"(keep[q][k]), "+v"(g[k]));
-                        float hn = __builtin_fmaf(x, m.B[n], keep[q][n]);
-                        y = __builtin_fmaf(m.C[n], hn, y);
-                        g[n] = __builtin_fmaf(o, m.C[n], g[n]);
+                        float hn = __builtin_fmaf(x, Bn, keep[q][n]);
+                        y = __builtin_fmaf(Cn, hn, y);
+                        g[n] = __builtin_fmaf(o, Cn, g[n]);
                         v[n] = first_sum(g[n] * x, o * hn);
-                        gB = __builtin_fmaf(g[n], m.B[n], gB);
+                        gB = __builtin_fmaf(g[n], Bn, gB);
                         float gh = g[n] * keep[q][n];
                         gk = __builtin_fmaf(gh, A2[n], gk);
                         dA[n] = __builtin_fmaf(gh, d[q], dA[n]);
@@ -543,11 +598,11 @@ template <class T, int NS, int H> __global__ __launch_bounds__(256, 2) void scan
                     }
                     if (begins >> q & 1) forget<NS>(g);
                     if constexpr (H == 1) {
-                        if (q < here) finish(q, out, zf, sig, o, y, gB, gk, raw_d, d[q], uq);
+                        finish(q, out, zf, sig, o, y, gB, gk, raw_d, d[q], uq);
                     } else others[(q * 3 + 0) * kWave] = y, others[(q * 3 + 1) * kWave] = gB, others[(q * 3 + 2) * kWave] = gk;
                     float total = wave_sums<M>(v);
                     if (lane % (kWave / M) == 0) to[q * M + lane / (kWave / M)] = total;
-                    __builtin_amdgcn_sched_barrier(0);
+                    here_only();
                 }
                 // the other half of `sums` and `meet` is read by nobody after this barrier, and this half is written again after the next
                 __syncthreads();
@@ -773,7 +828,7 @@ static ScanPlan scan_plan(const mws_scan_args *a, bool backward) {
         at += (n + 63) / 64 * 64;
         return from;
     };
-    p.bc = take(tokens * 2 * p.ns);
+    p.bc = take((tokens + 1) * 2 * p.ns);            // and what is asked for behind the last token
     p.seg = take(p.segments > 1 ? a->batch * p.segments * p.ns * a->width : 0);
     p.sum = take(p.segments > 1 ? a->batch * p.segments * a->width : 0);
     p.part_bc = take(backward ? p.across * tokens * 2 * p.ns : 0);
