@@ -53,15 +53,6 @@ template <class T, int V> __device__ __forceinline__ void store_some(typename T:
         if (i < n) p[i] = r.v[i];
 }
 
-// parameters: float, or of the activations' type
-template <class T> __device__ __forceinline__ float param(const void *p, int64_t i, bool wide) {
-    return wide ? ((const float *)p)[i] : up<T>(((const typename T::raw *)p)[i]);
-}
-template <class T> __device__ __forceinline__ void set_param(void *p, int64_t i, float v, bool wide) {
-    if (wide) ((float *)p)[i] = v;
-    else ((typename T::raw *)p)[i] = down<T>(v);
-}
-
 // ---- functions: hardware exp2 / log2 / reciprocal (each within one unit in the last place) ----
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }

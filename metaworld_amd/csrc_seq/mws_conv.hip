@@ -70,8 +70,12 @@ template <class T, int V, int K> __device__ __forceinline__ void taps(const Conv
 #pragma unroll
         for (int i = 0; i < V * K; i++) w[i % K].v[i / K] = up<T>(r.v[i]);
     }
+    if (a.bias == nullptr) b.zero();
+    else if (a.wide) {
+        Vec<F32, V> r = load<F32, V>((const float *)a.bias + e);
 #pragma unroll
-    for (int i = 0; i < V; i++) b.v[i] = a.bias != nullptr ? param<T>(a.bias, e + i, a.wide) : 0.0f;
+        for (int i = 0; i < V; i++) b.v[i] = r.v[i];
+    } else b.set(load<T, V>((const typename T::raw *)a.bias + e));
 }
 
 // the input at token p of row b (p >= -(K - 1); below zero: the state)

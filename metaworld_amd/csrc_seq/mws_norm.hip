@@ -3,7 +3,7 @@
 //   m = mean x, v = mean (x - m)^2, r = (v + eps)^-1/2, n = (x - m) r, y = n w + b
 //   g = dy w, dx = r (g - mean g - n mean(g n)), dw = sum over rows of dy n, db = sum over rows of dy
 //
-// Bound by memory, 262144 x 512 bf16 forward in 127 us (4.2 TB/s; a copy of 4 GiB reaches 4.8), backward in 173 us (4.7 TB/s): one
+// Bound by memory, 262144 x 512 bf16 forward in 121 us (4.4 TB/s; a copy of 4 GiB reaches 4.8), backward in 170 us (4.7 TB/s): one
 // pass over the data.  A row stays in the registers of TPR threads (V values to a 16-byte load, PER loads to
 // a thread), the variance is taken from the centred values (two sums over the lanes, no difference of large squares), and the
 // parameters stay in registers while a block walks over its rows.  The backward pass takes mean and r anew from the row it reads
@@ -71,14 +71,25 @@ template <class T, int V, int PER, int TPR> struct Row {
             if (col < width) store_some<T, V>(p + col, r, width - col);
         }
     }
+    // whole vectors: a condition for each value is a branch with a wait of its own, and every block begins with them (8000 x 512 bf16
+    // forward 5.7 us, 11.4 us value by value)
     __device__ __forceinline__ void read_param(const void *p, int lane, int width, bool wide, float otherwise) {
 #pragma unroll
-        for (int k = 0; k < PER; k++)
+        for (int k = 0; k < PER; k++) {
+            int col = (k * TPR + lane) * V, from = col < width ? col : 0, n = width - col;
+            if (p == nullptr) {
 #pragma unroll
-            for (int i = 0; i < V; i++) {
-                int col = (k * TPR + lane) * V + i;
-                v[k * V + i] = p != nullptr && col < width ? param<T>(p, col, wide) : otherwise;
+                for (int i = 0; i < V; i++) v[k * V + i] = otherwise;
+            } else if (wide) {
+                Vec<F32, V> r = load_some<F32, V>((const float *)p + from, n);
+#pragma unroll
+                for (int i = 0; i < V; i++) v[k * V + i] = r.v[i];
+            } else {
+                Vec<T, V> r = load_some<T, V>((const typename T::raw *)p + from, n);
+#pragma unroll
+                for (int i = 0; i < V; i++) v[k * V + i] = up<T>(r.v[i]);
             }
+        }
     }
     // centres the row and returns r; columns past the width stay zero
     __device__ __forceinline__ float centre(int lane, int width, float share, float eps, float (*meet)[16], int &turn) {
@@ -198,7 +209,7 @@ struct NormOut {
 };
 
 // Threads of a row: eight values each from 1025 columns on (16384 x 4096 bf16 forward 65 us, backward 116 us; with sixteen 71 and
-// 160 us).  Blocks walk over the rows, 4096 waves in all (262144 x 512 bf16 forward 129 us, backward 174 us; with twice as many 133
+// 160 us).  Blocks walk over the rows, 4096 waves in all (262144 x 512 bf16 forward 123 us, backward 170 us; with twice as many 128
 // and 195 us); twice that forward in blocks of 1024 threads, two of which fit a compute unit (4000 x 16384 fp32 116 us, not 182).
 static int norm_rows(int tpr) { return tpr <= kWave ? 256 / tpr : 1; }
 static int norm_tpr(const mws_norm_args *a) {
