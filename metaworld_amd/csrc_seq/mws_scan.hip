@@ -11,7 +11,7 @@
 // scalar registers, from a small copy in float, [token][B | C][states], that `spread` makes first (128 bytes a token next to the
 // channels' 8 bytes each).  A wave walks along the time axis; u, dt, z and y are read and written in order of channels.
 // Bound by the vector unit: per value and state one exp (two issue slots) and four multiplications or additions forward, some 145
-// slots a token and wave with 16 states.  2048 x 64 x 512 x 16 bf16 forward in 303 us, 85 % of the slots taken; the memory would allow 140.
+// slots a token and wave with 16 states.  2048 x 64 x 512 x 16 bf16 forward in 262 us; the memory would allow 140.
 //
 // Where batch x channels leave the card empty, the time axis is cut into segments of whole chunks: scan_segment takes each
 // segment's end state from zero and its sum of d (the product of its a is exp(A sum d)), scan_join runs over the segments, and the
@@ -140,19 +140,44 @@ template <int S> struct One {
 };
 __device__ __forceinline__ void here_only() { __builtin_amdgcn_sched_barrier(0); }      // nothing moves past this
 
-// a lane's states: NS of them from `first` on, of `all` in a row (padded with zeros)
-template <int NS> __device__ __forceinline__ void rates(const ScanArgs &a, uint32_t e, float (&A2)[NS], int first = 0) {       // A / ln 2, for exp2
+// a lane's states: NS of them from `first` on, of a row of `states` (padded with zeros).  All loads go out before the first is waited
+// for: a condition for each of them would be a branch with a wait of its own, and every wave begins with them (2048 x 64 x 512 x 16
+// bf16 forward 271 us, 314 us so; 405 x 66 x 874 x 32 211 us, not 278).
+template <int NS> __device__ __forceinline__ void get_states(const float *row, int states, int first, float (&h)[NS]) {
+    if (states % 4 == 0) {
+        Vec<F32, 4> r[NS / 4];
 #pragma unroll
-    for (int n = 0; n < NS; n++) A2[n] = first + n < a.states ? a.A[(int64_t)e * a.states + first + n] * kLog2e : 0.0f;
+        for (int k = 0; k < NS / 4; k++) r[k] = load<F32, 4>(row + (first + k * 4 < states ? first + k * 4 : 0));
+#pragma unroll
+        for (int n = 0; n < NS; n++) h[n] = first + n < states ? r[n / 4].v[n % 4] : 0.0f;
+    } else {
+#pragma unroll
+        for (int n = 0; n < NS; n++) h[n] = row[first + n < states ? first + n : 0];
+#pragma unroll
+        for (int n = 0; n < NS; n++) h[n] = first + n < states ? h[n] : 0.0f;
+    }
+}
+template <int NS> __device__ __forceinline__ void rates(const ScanArgs &a, uint32_t e, float (&A2)[NS], int first = 0) {       // A / ln 2, for exp2
+    get_states<NS>(a.A + (int64_t)e * a.states, a.states, first, A2);
+#pragma unroll
+    for (int n = 0; n < NS; n++) A2[n] *= kLog2e;
 }
 template <int NS> __device__ __forceinline__ void first_state(const float *state, const ScanArgs &a, int64_t b, uint32_t e, float (&h)[NS], int first = 0) {
+    if (state != nullptr) get_states<NS>(state + (b * a.width + e) * a.states, a.states, first, h);
+    else
 #pragma unroll
-    for (int n = 0; n < NS; n++) h[n] = state != nullptr && first + n < a.states ? state[(b * a.width + e) * a.states + first + n] : 0.0f;
+        for (int n = 0; n < NS; n++) h[n] = 0;
 }
 template <int NS> __device__ __forceinline__ void last_state(float *to, const ScanArgs &a, int64_t b, uint32_t e, const float (&h)[NS], int first = 0) {
+    float *row = to + (b * a.width + e) * a.states + first;
+    if (a.states % 4 == 0) {
 #pragma unroll
-    for (int n = 0; n < NS; n++)
-        if (first + n < a.states) to[(b * a.width + e) * a.states + first + n] = h[n];
+        for (int k = 0; k < NS / 4; k++)
+            if (first + k * 4 < a.states) store<F32, 4>(row + k * 4, {h[k * 4], h[k * 4 + 1], h[k * 4 + 2], h[k * 4 + 3]});
+    } else
+#pragma unroll
+        for (int n = 0; n < NS; n++)
+            if (first + n < a.states) row[n] = h[n];
 }
 template <int NS> __device__ __forceinline__ void get_row(const float *p, int64_t row, const ScanArgs &a, uint32_t e, float (&h)[NS], int all = NS, int first = 0) {
 #pragma unroll
@@ -394,24 +419,26 @@ __global__ __launch_bounds__(256) void scan_join(ScanArgs a, int ns, bool backwa
     const float *from = backward ? a.dlast : a.state;
     float h = from != nullptr && real ? from[(b * a.width + e) * a.states + n] : 0.0f;
     // sixteen segments' values under way at a time: the chain through h does not wait for them
+    const int64_t step = (backward ? -1 : 1) * (int64_t)a.width, row = b * a.segments + (backward ? last : 0);
+    float *seg = a.seg + (row * ns + n) * a.width + e;
+    const float *sums = a.sum + row * a.width + e;
+    const int asked = backward && a.dstate != nullptr ? last + 1 : last;
     for (int k0 = 0; k0 <= last; k0 += 16) {
-        float left[16], sum[16];
+        float left[16], sum[16], *from_seg = seg;
 #pragma unroll
         for (int j = 0; j < 16; j++) {
-            int k = k0 + j, s = backward ? last - k : k;
-            bool asked = k < last || (k == last && backward && a.dstate != nullptr);
-            int64_t row = b * a.segments + (asked ? s : 0);
-            left[j] = asked ? a.seg[(row * ns + n) * a.width + e] : 0.0f;
-            sum[j] = asked ? a.sum[row * a.width + e] : 0.0f;
+            left[j] = k0 + j < asked ? *from_seg : 0.0f;
+            sum[j] = k0 + j < asked ? *sums : 0.0f;
+            from_seg += step * ns, sums += step;
         }
 #pragma unroll
         for (int j = 0; j < 16; j++) {
-            int k = k0 + j, s = backward ? last - k : k;
             float next = sum[j] < 0.0f || h == 0.0f ? left[j] : __builtin_fmaf(exp2_(sum[j] * A2), h, left[j]);
-            if (k <= last) {
-                a.seg[((b * a.segments + s) * ns + n) * a.width + e] = h;
+            if (k0 + j <= last) {
+                *seg = h;
                 h = next;
             }
+            seg += step * ns;
         }
     }
     if (backward && a.dstate != nullptr && real) {
@@ -456,8 +483,8 @@ template <int M> __device__ __forceinline__ float wave_sums(float (&v)[M / 2]) {
 // wave's channels token by token (wave_sums), over the block's waves after kKept tokens, over blocks by scan_bc_out.  Tokens past the
 // row's end count with d = u = dy = 0, which leaves g as it is and adds nothing.
 // More than 16 states are two halves (H = 2), each a wave's: what a token's gradients need of both, its output and two sums over the
-// states, meets in shared memory, and each of the two waves finishes every second token (405 x 66 x 874 x 32 bf16 900 us; four times that with all
-// states in one wave, most of that for registers that do not fit).
+// states, meets in shared memory, and each of the two waves finishes every second token (405 x 66 x 874 x 32 bf16 with the forward pass 1230 us; 4413 us without it where all
+// states are one wave's, most of that for registers that do not fit).
 // Bound by the vector unit: 2048 x 64 x 512 x 16 bf16 take 1.08 ms, 402 instructions a token and wave (98 of them for the way there),
 // at 80 % of its issue slots with the two waves to a SIMD that the registers allow; three waves with half the tokens each, whose
 // registers spill, took a quarter longer.
