@@ -817,20 +817,22 @@ static int block_waves(int waves, int most) {
     return best;
 }
 
-// Segments.  `places`: the waves that run at a time to some use, two to a SIMD backward (its registers allow no more), four forward.
-// The time is that of the rounds over the places times the tokens of a segment; cutting costs a second walk (forward 0.8 of the
-// first, backward 0.3) and joining.
-static int64_t best_span(int64_t waves, int64_t groups, bool backward) {
-    const double places = (backward ? 2 : 4) * kSimds, walks = backward ? 1.3 : 1.8;
-    auto rounds = [&](double w) {
-        double r = w / places;
-        return r <= 1 ? 1.0 : backward ? (double)(int64_t)(r + 0.999) : r;
+// Segments: how many groups each.  A group of one wave alone takes a SIMD 12 us forward and 42 us backward, for what its instructions
+// wait for; several waves take their issue slots' time (49 + 6 ns and 110 + 22 ns slots a token, four cycles each) and some of that
+// once.  Cutting costs a second walk (0.8 of the first, backward 0.25), two launches and a step of scan_join for each segment.  With
+// this 3 x 5000 x 777 x 12 fp16 is walked in segments of one group, forward 94 us (of 2: 103, of 4: 135, of 8: 210 us), the backward pass as
+// well (forward and backward 345 us; backward in segments of 2: 377, of 4: 460 us).
+static int64_t best_span(int64_t waves, int64_t groups, int ns, bool backward) {
+    const double alone = backward ? 42 : 12, slots = backward ? 110 + 22 * ns : 49 + 6 * ns, busy = slots * kGroup * 4 / 2400, walks = backward ? 1.25 : 1.8;
+    auto group = [&](int64_t w) {
+        double t = ((double)ceil_div(w, kSimds) + 0.7) * busy;
+        return t > alone ? t : alone;
     };
     int64_t best = groups;
-    double least = rounds((double)waves) * (double)groups;
-    for (int64_t s = 2; s <= groups && s <= 256; s++) {
+    double least = group(waves) * (double)groups;
+    for (int64_t s = 2; s <= groups && s <= 1024; s++) {
         int64_t each = ceil_div(groups, s), count = ceil_div(groups, each);
-        double cost = rounds((double)waves * (double)count) * (double)each * walks + 0.5 + 0.02 * (double)count;
+        double cost = group(waves * count) * (double)each * walks + 5 + 0.08 * (double)count;
         if (cost < least) best = each, least = cost;
     }
     return best;
@@ -843,7 +845,7 @@ static ScanPlan scan_plan(const mws_scan_args *a, bool backward) {
     p.lanes = of_block * kWave;
     p.across = (int)ceil_div(a->width, p.lanes);
     p.chunks = ceil_div(a->length, kKept);
-    int64_t groups = ceil_div(a->length > 0 ? a->length : 1, kGroup), halves = backward && p.ns > 16 ? 2 : 1, each = best_span(a->batch * p.across * of_block * halves, groups, backward);
+    int64_t groups = ceil_div(a->length > 0 ? a->length : 1, kGroup), halves = backward && p.ns > 16 ? 2 : 1, each = best_span(a->batch * p.across * of_block * halves, groups, halves == 2 ? 16 : p.ns, backward);
     p.segments = (int)ceil_div(groups, each);
     p.span = (int)(each * kGroup);
     // blocks over the items, four rounds of the places at most: each leaves partial sums of dA, dD and ddt_bias
