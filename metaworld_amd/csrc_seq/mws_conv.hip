@@ -5,7 +5,7 @@
 //
 // where x of a token before the row's first comes from the state, and of one before the episode's first is zero.
 //
-// Bound by memory, 512 x 128 x 1024 bf16 forward in 59 us (4.6 TB/s; a copy reaches 4.8), backward in 99 us (4.1 TB/s, the vector
+// Bound by memory, 512 x 128 x 1024 bf16 forward in 55 us (4.9 TB/s; a copy of 4 GiB reaches 4.8), backward in 92 us (4.4 TB/s, the vector
 // unit at it for most of the time), one token of 4096 x 1024 bf16 in 14 us (4.7 TB/s).  A lane keeps V neighbouring channels (one 16-byte access a token), a wave walks over a tile of tokens with the
 // last K of them in registers, so that every value is read once but for K - 1 tokens at a tile's edge (backward 2 K - 2).  The episodes' beginnings
 // of a tile are one 64-bit mask in scalar registers.
@@ -181,8 +181,9 @@ template <class T, int V, int K> __global__ __launch_bounds__(256) void conv_for
 }
 
 // A wave walks from its tile's first token to K - 1 tokens past it: it takes dw and db of its own tokens, and dx of them, whose last
-// terms come from the tokens past the tile.  The state's K - 1 inputs count as tokens before the first.
-template <class T, int V, int K> __global__ __launch_bounds__(256) void conv_backward(ConvArgs a) {
+// terms come from the tokens past the tile.  The state's K - 1 inputs count as tokens before the first.  Four waves to a SIMD: with the
+// next four tokens under way they do not fit (12 x 1000 x 640 fp32 with the forward pass 41 us, 79 us so; with three waves 51 us).
+template <class T, int V, int K> __global__ __launch_bounds__(256, 4) void conv_backward(ConvArgs a) {
     using raw = typename T::raw;
     int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), waves = blockDim.x / kWave;
     const Mine<V> m(blockIdx.y * kWave + lane, a.width);
@@ -300,20 +301,19 @@ template <class T, int V, int K> __global__ __launch_bounds__(256) void conv_bac
             for (int64_t t = t0 > end ? t0 : end; t < t1; t++) store<T, V>(dx + (t - t0) * a.width, none.rounded());
     }
     if (a.part == nullptr) return;
-    __shared__ float meet[4][kWave];
+    // the block's sums: its waves' meet in shared memory, behind one barrier for all of them
+    __shared__ float meet[4][(K + 1) * V][kWave];
     float *part = a.part + (int64_t)blockIdx.x * (K + 1) * a.width;
 #pragma unroll
     for (int j = 0; j <= K; j++)
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-            __syncthreads();
-            meet[wave][lane] = j < K ? dw[j < K ? j : 0].v[i] : db.v[i];
-            __syncthreads();
-            if (wave == 0 && m.on) {
-                float s = 0;
-                for (int k = 0; k < waves; k++) s += meet[k][lane];
-                part[(int64_t)j * a.width + m.e + i] = s;
-            }
+        for (int i = 0; i < V; i++) meet[wave][j * V + i][lane] = j < K ? dw[j < K ? j : 0].v[i] : db.v[i];
+    __syncthreads();
+    if (m.on)
+        for (int r = wave; r < (K + 1) * V; r += waves) {
+            float s = 0;
+            for (int k = 0; k < waves; k++) s += meet[k][r][lane];
+            part[(int64_t)(r / V) * a.width + m.e + r % V] = s;
         }
 }
 
@@ -381,7 +381,7 @@ static int conv_v(const mws_conv_args *a) {
     return a->width >= v ? v : 1;
 }
 // backward four of any type: with eight the weights, inputs, sums and gradients of the taps leave two waves to a SIMD (512 x 128 x 1024
-// bf16 102 us, with eight 118 us)
+// bf16 102 us when with eight it was 118 us)
 static int conv_back_v(const mws_conv_args *a) { return a->width >= 4 ? 4 : 1; }
 static int conv_tile(const mws_conv_args *a) {
     int64_t across = a->batch * ceil_div(a->width, kWave * conv_v(a));

@@ -171,27 +171,26 @@ template <class T, int V, int PER, int TPR> __global__ __launch_bounds__(TPR > k
         }
     }
     if (a.part == nullptr) return;
-    // the block's sums: the rows that it took side by side meet in shared memory, V x PER x TPR columns at a time
-    __shared__ float pool[kRows > 1 ? 256 : 1];
     float *part = a.part + (int64_t)blockIdx.x * 2 * a.width;
+    if constexpr (kRows > 1) {
+        // the block's sums: the rows that it took side by side meet in shared memory, behind one barrier for all columns
+        __shared__ float pool[2 * PER * V][256];
 #pragma unroll
-    for (int k = 0; k < PER * V; k++) {
-        int col = ((k / V) * TPR + lane) * V + k % V;
+        for (int k = 0; k < PER * V; k++) pool[k][threadIdx.x] = dw[k], pool[PER * V + k][threadIdx.x] = db[k];
+        __syncthreads();
+        for (int r = sub; r < 2 * PER * V; r += kRows) {
+            float v = 0;
 #pragma unroll
-        for (int which = 0; which < 2; which++) {
-            float v = which ? db[k] : dw[k];
-            if constexpr (kRows > 1) {
-                __syncthreads();
-                pool[threadIdx.x] = v;
-                __syncthreads();
-                v = 0;
-                if (sub == 0)
-#pragma unroll
-                    for (int j = 0; j < kRows; j++) v += pool[j * TPR + lane];
-            }
-            if (sub == 0 && col < a.width) part[which * a.width + col] = v;
+            for (int j = 0; j < kRows; j++) v += pool[r][j * TPR + lane];
+            int k = r % (PER * V), col = ((k / V) * TPR + lane) * V + k % V;
+            if (col < a.width) part[r / (PER * V) * a.width + col] = v;
         }
-    }
+    } else
+#pragma unroll
+        for (int k = 0; k < PER * V; k++) {
+            int col = ((k / V) * TPR + lane) * V + k % V;
+            if (col < a.width) part[col] = dw[k], part[a.width + col] = db[k];
+        }
 }
 
 struct NormOut {
