@@ -13,16 +13,16 @@
 // Bound by the vector unit: per value and state one exp (two issue slots) and four multiplications or additions forward, some 145
 // slots a token and wave with 16 states.  2048 x 64 x 512 x 16 bf16 forward in 262 us; the memory would allow 140.
 //
-// Where batch x channels leave the card empty, the time axis is cut into segments of whole chunks: scan_segment takes each
+// Where batch x channels leave the card empty, the time axis is cut into segments: scan_segment takes each
 // segment's end state from zero and its sum of d (the product of its a is exp(A sum d)), scan_join runs over the segments, and the
 // scan itself starts every segment from its joined state.  The same holds for g, from the end.
 #include "mws_common.hpp"
 
 namespace mws {
 
-// Tokens are walked in groups of kGroup, whose episodes' beginnings are one mask; segments are whole groups.  Every kKept-th token's
-// state is kept for the backward pass, which holds what lies between two of them in registers (states x tokens = 128).  lanes_of: a
-// block's channels at most.
+// Tokens are walked in groups of kGroup, whose episodes' beginnings are one mask.  Every kKept-th token's state is kept for the
+// backward pass, which holds what lies between two of them in registers (states x tokens = 128); segments begin at these tokens.
+// lanes_of: a block's channels at most.
 constexpr int kGroup = 32, kKept = 8;
 constexpr int lanes_of(int ns) { return ns >= 32 ? 128 : 256; }
 
@@ -315,10 +315,11 @@ template <class T, int NS> __global__ __launch_bounds__(256) void scan_segment(S
     Fixed *bc = fixed(a.bc + (p.b * a.length + p.t0) * 2 * NS);
     One<NS> B[2];
     B[0].read(bc);
-    for (int64_t c0 = p.t0; c0 < p.t1; c0 += kGroup) {        // whole groups: the row goes on behind the segment
-        uint32_t begins = group_mask(a, p.b, c0, p.end);
+    for (int64_t c0 = p.t0; c0 < p.t1; c0 += kGroup) {        // (a whole segment: the row goes on behind it)
+        uint32_t begins = group_mask(a, p.b, c0, p.t1);
         cut = cut || begins != 0;
-        for (int i = 0; i < kGroup; i += G) {
+        const int count = (int)(c0 + kGroup < p.t1 ? kGroup : p.t1 - c0);
+        for (int i = 0; i < count; i += G) {
             Line<raw> lu(u, 0, a.u_time), ld(dt, 0, a.dt_time);
             raw ru[G], rd[G];
 #pragma unroll
@@ -363,7 +364,7 @@ template <class T, int NS> __global__ __launch_bounds__(256) void scan_segment_b
     const bool gated = a.z != nullptr;
     float bias = a.dt_bias != nullptr ? a.dt_bias[p.e] : 0.0f;
     for (int64_t c0 = p.t0 + (stop - 1 - p.t0) / kGroup * kGroup; c0 >= p.t0; c0 -= kGroup) {
-        uint32_t begins = group_mask(a, p.b, c0, p.end);
+        uint32_t begins = group_mask(a, p.b, c0, stop);
         cut = cut || begins != 0;
         int count = (int)(c0 + kGroup < stop ? kGroup : stop - c0);
         for (int i = (count - 1) / G * G; i >= 0; i -= G) {
@@ -817,22 +818,24 @@ static int block_waves(int waves, int most) {
     return best;
 }
 
-// Segments: how many groups each.  A group of one wave alone takes a SIMD 12 us forward and 42 us backward, for what its instructions
-// wait for; several waves take their issue slots' time (49 + 6 ns and 110 + 22 ns slots a token, four cycles each) and some of that
-// once.  Cutting costs a second walk (0.8 of the first, backward 0.25), two launches and a step of scan_join for each segment.  With
-// this 3 x 5000 x 777 x 12 fp16 is walked in segments of one group, forward 94 us (of 2: 103, of 4: 135, of 8: 210 us), the backward pass as
-// well (forward and backward 345 us; backward in segments of 2: 377, of 4: 460 us).
-static int64_t best_span(int64_t waves, int64_t groups, int ns, bool backward) {
-    const double alone = backward ? 42 : 12, slots = backward ? 110 + 22 * ns : 49 + 6 * ns, busy = slots * kGroup * 4 / 2400, walks = backward ? 1.25 : 1.8;
-    auto group = [&](int64_t w) {
-        double t = ((double)ceil_div(w, kSimds) + 0.7) * busy;
-        return t > alone ? t : alone;
+// Segments: how many times kKept tokens each.  kKept tokens of one wave alone take a SIMD 3 us forward and 10.5 us backward, for what
+// its instructions wait for; several waves take their issue slots' time (49 + 6 ns and 110 + 22 ns slots a token, four cycles each)
+// and some of that once.  Each wave begins with its rates and state.  Cutting costs a second walk (0.8 of the first, backward 0.25),
+// two launches and a step of scan_join for each segment.  (3 x 5000 x 777 x 12 fp16 forward in segments of 8 tokens 127 us, of 24: 86,
+// of 40: 82, of 48, which this takes: 90, of 64: 104, of 128: 136 us; 1 x 300 x 512 x 16 bf16 of 8, which this takes: 25, of 32: 36, of
+// 64: 62 us.)
+static int64_t best_span(int64_t waves, int64_t parts, int ns, bool backward) {
+    const double alone = backward ? 10.5 : 3, slots = backward ? 110 + 22 * ns : 49 + 6 * ns, busy = slots * kKept * 4 / 2400, walks = backward ? 1.25 : 1.8;
+    auto time = [&](int64_t w, int64_t each) {
+        double one = alone * (double)each + 1.5, all = ((double)ceil_div(w, kSimds) + 0.7) * (busy * (double)each + (backward ? 0.08 : 0.04) * ns);
+        return one > all ? one : all;
     };
-    int64_t best = groups;
-    double least = group(waves) * (double)groups;
-    for (int64_t s = 2; s <= groups && s <= 1024; s++) {
-        int64_t each = ceil_div(groups, s), count = ceil_div(groups, each);
-        double cost = group(waves * count) * (double)each * walks + 5 + 0.08 * (double)count;
+    int64_t best = parts;
+    double least = time(waves, parts);
+    for (int64_t each = 1; each < parts; each = each < 16 ? each + 1 : each + each / 8) {
+        int64_t count = ceil_div(parts, each);
+        if (count > 1024) continue;
+        double cost = time(waves * count, each) * walks + 5 + 0.08 * (double)count;
         if (cost < least) best = each, least = cost;
     }
     return best;
@@ -845,9 +848,9 @@ static ScanPlan scan_plan(const mws_scan_args *a, bool backward) {
     p.lanes = of_block * kWave;
     p.across = (int)ceil_div(a->width, p.lanes);
     p.chunks = ceil_div(a->length, kKept);
-    int64_t groups = ceil_div(a->length > 0 ? a->length : 1, kGroup), halves = backward && p.ns > 16 ? 2 : 1, each = best_span(a->batch * p.across * of_block * halves, groups, halves == 2 ? 16 : p.ns, backward);
-    p.segments = (int)ceil_div(groups, each);
-    p.span = (int)(each * kGroup);
+    int64_t parts = ceil_div(a->length > 0 ? a->length : 1, kKept), halves = backward && p.ns > 16 ? 2 : 1, each = best_span(a->batch * p.across * of_block * halves, parts, halves == 2 ? 16 : p.ns, backward);
+    p.segments = (int)ceil_div(parts, each);
+    p.span = (int)(each * kKept);
     // blocks over the items, four rounds of the places at most: each leaves partial sums of dA, dD and ddt_bias
     int64_t items = a->batch * p.segments, most = 8 * kSimds / (of_block * halves * p.across) > 0 ? 8 * kSimds / (of_block * halves * p.across) : 1;
     p.groups = (int)(items < most ? items : most);
