@@ -377,6 +377,28 @@ def test_scan_of_long_rows_in_segments(batch, time, width, states):
 
 
 @gpu
+@pytest.mark.parametrize("batch", [5, 40, 80])
+def test_segments_of_few_and_of_many_rows(batch):
+    """the more rows there are, the fewer threads share the chain over a row's segments: rows at the batch's ends against the plain scan"""
+    time, width, states = 150, 70, 16
+    gen = seeded(batch, time, width, states)
+    ins = scan_inputs(gen, batch, time, width, states, torch.float32)
+    dy, dlast = rand(gen, batch, time, width, kind=torch.float32), rand(gen, batch, width, states, kind=torch.float32)
+    reset = torch.rand((batch, time), generator=gen) < 0.02
+    lengths = torch.randint(0, time + 1, (batch,), generator=gen, dtype=torch.int32)
+    rows = [0, 1, batch - 1]
+    lengths[0], lengths[1] = time, 9
+    leaves = [on(t, torch.float32, True) for t in ins]
+    y, last = sequence.selective_scan(*leaves[:8], state=leaves[8], reset=on(reset), lengths=on(lengths))
+    grads = torch.autograd.grad((y, last), leaves, (on(dy, torch.float32), on(dlast, torch.float32)))
+    some = [t if k in (2, 5, 7) else t[rows] for k, t in enumerate(ins)]            # A, D and dt_bias are everyone's
+    want, mag = (plain_scan(*some, reset[rows], lengths[rows], dy[rows], dlast[rows], m) for m in (False, True))
+    for what, got, v, m in zip(SCAN_NAMES, (y, last, *grads), want, mag):
+        if what not in ("dA", "dD", "dbias"):
+            check(what, got[rows], v, m, scan_operations(ins, time, 0))
+
+
+@gpu
 @pytest.mark.parametrize("which", ["norm", "conv", "scan"])
 def test_gradients_against_differences(which):
     """central differences of the plain 64-bit values along a random direction: off by h^2 of third derivatives (h = 1e-4), and the kernels' gradient by
