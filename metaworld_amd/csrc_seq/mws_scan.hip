@@ -107,8 +107,13 @@ template <class T, int NS> __global__ __launch_bounds__(256) void spread(const v
     for (int64_t b = blockIdx.y; b < batch; b += gridDim.y) {
         const typename T::raw *from = (const typename T::raw *)(second ? C : B) + (second ? b * C_batch + t * C_time : b * B_batch + t * B_time) + n;
         Vec<F32, 4> v;
+        if (states % 4 == 0) {
+            Vec<T, 4> r = load<T, 4>(n < states ? from : from - n);
 #pragma unroll
-        for (int k = 0; k < 4; k++) v.v[k] = n + k < states ? up<T>(from[k]) : 0.0f;
+            for (int k = 0; k < 4; k++) v.v[k] = n < states ? up<T>(r.v[k]) : 0.0f;
+        } else
+#pragma unroll
+            for (int k = 0; k < 4; k++) v.v[k] = n + k < states ? up<T>(from[k]) : 0.0f;
         store<F32, 4>(bc + ((b * length + t) * 2 * NS + at), v);
     }
 }
@@ -728,17 +733,26 @@ template <class T, int NS, int H> __global__ __launch_bounds__(256, 2) void scan
     }
 }
 
+// four values to a thread
 template <class T> __global__ __launch_bounds__(256) void scan_bc_out(const float *part, const int32_t *lengths, void *dB, void *dC, int64_t batch, int64_t length, int parts, int states,
                                                                        int ns) {
-    int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, all = batch * length * 2 * ns;
+    using raw = typename T::raw;
+    int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, all = batch * length * 2 * ns;
     if (at >= all) return;
     int n = (int)(at % ns);
     if (n >= states) return;
     int64_t rest = at / ns, token = rest >> 1;
-    float v = 0;
+    Vec<F32, 4> v = {};
     if (lengths == nullptr || token % length < row_length(lengths, token / length, length))
-        for (int k = 0; k < parts; k++) v += part[k * all + at];
-    ((typename T::raw *)(rest & 1 ? dC : dB))[token * states + n] = down<T>(v);
+        for (int k = 0; k < parts; k++) {
+            Vec<F32, 4> p = load<F32, 4>(part + k * all + at);
+#pragma unroll
+            for (int i = 0; i < 4; i++) v.v[i] += p.v[i];
+        }
+    Vec<T, 4> r;
+#pragma unroll
+    for (int i = 0; i < 4; i++) r.v[i] = down<T>(v.v[i]);
+    store_some<T, 4>((raw *)(rest & 1 ? dC : dB) + token * states + n, r, states - n);
 }
 
 struct ScanOut {
@@ -962,7 +976,7 @@ template <class T, int NS> static void backward_go(const mws_scan_args *a, const
     if (d.batch > 0) hipLaunchKernelGGL((scan_backward<T, PER, H>), dim3((unsigned)(p.groups * p.across)), dim3(waves * kWave), lds, stream, d);
     int64_t count = d.batch * d.length * 2 * NS;
     if (count > 0)
-        hipLaunchKernelGGL((scan_bc_out<T>), dim3((unsigned)ceil_div(count, 256)), dim3(256), 0, stream, d.part_bc, a->lengths, a->dB, a->dC, d.batch, d.length, p.across, a->states, NS);
+        hipLaunchKernelGGL((scan_bc_out<T>), dim3((unsigned)ceil_div(count / 4, 256)), dim3(256), 0, stream, d.part_bc, a->lengths, a->dB, a->dC, d.batch, d.length, p.across, a->states, NS);
     ScanOut out = {a->dA, a->dD, a->ddt_bias, a->width, a->states, NS};
     launch_sum_parts(d.part, p.groups, (int64_t)(NS + 2) * a->width, out, stream);
 }
