@@ -10,8 +10,8 @@
 // A lane is a channel with all its states in registers, so that a token's B and C are the same for the whole wave: they come in
 // scalar registers, from a small copy in float, [token][B | C][states], that `spread` makes first (128 bytes a token next to the
 // channels' 8 bytes each).  A wave walks along the time axis; u, dt, z and y are read and written in order of channels.
-// Bound by the vector unit: per value and state one exp (two issue slots) and four multiplications or additions forward, some 145
-// slots a token and wave with 16 states.  2048 x 64 x 512 x 16 bf16 forward in 262 us; the memory would allow 140.
+// Bound by the vector unit: per value and state one exp (two issue slots) and four multiplications or additions forward, 147
+// slots a token and wave with 16 states.  2048 x 64 x 512 x 16 bf16 forward in 259 us, every slot taken; the memory would allow 140.
 //
 // Where batch x channels leave the card empty, the time axis is cut into segments: scan_segment takes each
 // segment's end state from zero and its sum of d (the product of its a is exp(A sum d)), scan_join runs over the segments, and the
@@ -511,10 +511,10 @@ template <int M> __device__ __forceinline__ float wave_sums(float (&v)[M / 2]) {
 // wave's channels token by token (wave_sums), over the block's waves after kKept tokens, over blocks by scan_bc_out.  Tokens past the
 // row's end count with d = u = dy = 0, which leaves g as it is and adds nothing.
 // More than 16 states are two halves (H = 2), each a wave's: what a token's gradients need of both, its output and two sums over the
-// states, meets in shared memory, and each of the two waves finishes every second token (405 x 66 x 874 x 32 bf16 with the forward pass 1230 us; 4413 us without it where all
-// states are one wave's, most of that for registers that do not fit).
-// Bound by the vector unit: 2048 x 64 x 512 x 16 bf16 take 1.08 ms, 402 instructions a token and wave (98 of them for the way there),
-// at 80 % of its issue slots with the two waves to a SIMD that the registers allow; three waves with half the tokens each, whose
+// states, meets in shared memory, and each of the two waves finishes every second token (405 x 66 x 874 x 32 bf16 with the forward
+// pass 1120 us; 4413 us without it where all states are one wave's, most of that for registers that do not fit).
+// Bound by the vector unit: 2048 x 64 x 512 x 16 bf16 take some 1.0 ms, 403 instructions a token and wave (98 of them for the way there),
+// at 84 % of its issue slots with the two waves to a SIMD that the registers allow; three waves with half the tokens each, whose
 // registers spill, took a quarter longer.
 template <class T, int NS, int H> __global__ __launch_bounds__(256, 2) void scan_backward(ScanArgs a) {
     using raw = typename T::raw;
