@@ -884,7 +884,8 @@ static ScanPlan scan_plan(const mws_scan_args *a, bool backward) {
     p.lanes = of_block * kWave;
     p.across = (int)ceil_div(a->width, p.lanes);
     p.chunks = ceil_div(a->length, kKept);
-    int64_t parts = ceil_div(a->length > 0 ? a->length : 1, kKept), halves = backward && p.ns > 16 ? 2 : 1, each = best_span(a->batch * p.across * of_block * halves, parts, halves == 2 ? 16 : p.ns, backward);
+    // (a forward pass is cut alike whether a backward pass follows or not: the same values to the last bit)
+    int64_t parts = ceil_div(a->length > 0 ? a->length : 1, kKept), halves = backward && p.ns > 16 ? 2 : 1, each = best_span(a->batch * p.across * of_block * halves, parts, halves == 2 ? 16 : scan_ns(a, true), backward);
     p.segments = (int)ceil_div(parts, each);
     p.span = (int)(each * kKept);
     // blocks over the items, four rounds of the places at most: each leaves partial sums of dA, dD and ddt_bias

@@ -14,7 +14,7 @@ Tokens are [batch, time].  `reset` (bool or uint8, [batch, time]) is true at an 
 state nor earlier tokens are seen.  `lengths` (int32 [batch]) says how many tokens of a padded row count, taken into 0 .. time: the
 others' inputs are not looked at, their outputs and gradients are zero, and the returned state is that after the last token that
 counts.  Gradients are deterministic (no atomic additions) and not differentiable again (create_graph is refused, as are forward
-derivatives).
+derivatives).  A call gives the same values to the last bit whether it is recorded for them or not.
 """
 from __future__ import annotations
 

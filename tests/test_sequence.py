@@ -377,6 +377,25 @@ def test_scan_of_long_rows_in_segments(batch, time, width, states):
 
 
 @gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("batch,time,width,states", [(2, 70, 50, 20), (1, 300, 33, 24), (2, 150, 40, 9), (3, 100, 20, 31), (1, 900, 30, 12), (1, 400, 140, 28)])
+def test_recording_changes_nothing(kind, batch, time, width, states):
+    """numbers of states that are padded less where no backward pass follows: the plain values, and those of the recorded pass to the last bit"""
+    gen = seeded(batch, time, width, states)
+    reset, lengths = flags(gen, batch, time, "padded")
+    ins = scan_inputs(gen, batch, time, width, states, kind)
+    leaves = [on(t, kind if k in (0, 1, 3, 4, 6) else torch.float32, True) for k, t in enumerate(ins)]
+    with torch.no_grad():
+        y, last = sequence.selective_scan(*leaves[:8], state=leaves[8], reset=on(reset), lengths=on(lengths))
+    zero = torch.zeros(batch, time, width, dtype=torch.float64), torch.zeros(batch, width, states, dtype=torch.float64)
+    want, mag = (plain_scan(*ins, reset, lengths, *zero, m) for m in (False, True))
+    for what, got, v, m in zip(SCAN_NAMES, (y, last), want, mag):
+        check(what, got, v, m, scan_operations(ins, time, 0))
+    again = sequence.selective_scan(*leaves[:8], state=leaves[8], reset=on(reset), lengths=on(lengths))
+    assert torch.equal(again[0], y) and torch.equal(again[1], last)
+
+
+@gpu
 @pytest.mark.parametrize("batch", [5, 40, 80])
 def test_segments_of_few_and_of_many_rows(batch):
     """the more rows there are, the fewer threads share the chain over a row's segments: rows at the batch's ends against the plain scan"""
