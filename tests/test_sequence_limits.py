@@ -1,0 +1,164 @@
+"""The selective scan where its forms could part from the recurrence: rows cut into segments, numbers of states that are padded,
+infinities, growing states.  Against the recurrence in 64 bits, with an error bound that decays with the states.
+
+The bound.  `recurrence` carries along with every value its magnitude (the same formulas with every term's absolute value) and a bound
+on its error in float32.  U = 2^-24 is half a step; exp2, log2 and reciprocals of the hardware are off by 2 U.  raw = dt + dt_bias is off
+by |raw| U, e^raw by another (2 |raw| + 2) U, the logarithm and its correction by 14 U at most: d by (3 |raw| + 16) U.  The exponent d A
+has a constant and a product more (4 U), its exp2 3 U; where a row is cut, d is first summed over a segment and a stretch of segments (at
+most SUMMED additions, U each).  A state is what is kept of the one before, with that one's error, and its own terms; a cut row adds it up
+twice.  So an error lives as long as the state it is in, and the bound does not grow with the row.
+"""
+import numpy as np
+import pytest
+import torch
+
+from metaworld_amd import sequence
+
+gpu = pytest.mark.gpu
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+U, SUMMED = 2.0 ** -24, 300
+NAMES = ("y", "last", "du", "ddt", "dA", "dB", "dC", "dD", "dz", "dbias", "dstate")
+
+
+def recurrence(u, dt, A, B, C, D, z, bias, state, reset, lengths, dy, dlast, keep_state=lambda t, h: h):
+    """{name: (value, bound on its error in float32)}, token by token, all rows at once"""
+    batch, time, width = u.shape
+    states = A.shape[1]
+    ends = lengths.long() if lengths is not None else torch.full((batch,), time)
+    reset = reset if reset is not None else torch.zeros(batch, time, dtype=torch.bool)
+    raw = dt + bias
+    d = torch.logaddexp(raw, torch.zeros_like(raw))
+    rel_d = (3 * raw.abs() + 16) * U
+    sig = torch.sigmoid(z)
+    gate = z * sig
+    gate_rel = (2 * z.abs() + 9) * U
+    slope, slope_err = sig * (1 + z * (1 - sig)), sig * (1 + z.abs()) * (4 * z.abs() + 16) * U
+    zero = torch.zeros((), dtype=torch.float64)
+    h, hm, he = state.clone(), state.abs(), torch.zeros_like(state)
+    out = {n: (torch.zeros_like(t), torch.zeros_like(t)) for n, t in zip(NAMES, (u, state, u, dt, A, B, C, D, z, bias, state))}
+    tape = []
+    for t in range(time):
+        on = (t < ends)[:, None]
+        a = torch.exp(d[:, t, :, None] * A)
+        rel_a = d[:, t, :, None] * A.abs() * (rel_d[:, t, :, None] + (SUMMED + 4) * U) + 3 * U
+        fresh = reset[:, t, None, None]
+        keep, km, ke = (torch.where(fresh, zero, v) for v in (a * h, a * hm, a * he + a * hm * rel_a))
+        x = (d[:, t] * u[:, t])[..., None] * B[:, t, None]
+        new, nm = keep + x, km + x.abs()
+        ne = ke + x.abs() * (rel_d[:, t, :, None] + 3 * U) + 3 * U * nm
+        o, om = (new * C[:, t, None]).sum(-1) + D * u[:, t], (nm * C[:, t, None].abs()).sum(-1) + (D * u[:, t]).abs()
+        oe = (ne * C[:, t, None].abs()).sum(-1) + (states + 4) * U * om
+        out["y"][0][:, t] = torch.where(on, o * gate[:, t], zero)
+        out["y"][1][:, t] = torch.where(on, (oe + om * gate_rel[:, t]) * gate[:, t].abs(), zero)
+        h, hm, he = (torch.where(on[..., None], n, v) for n, v in ((keep_state(t, new), h), (nm, hm), (ne, he)))
+        tape.append((on, a, rel_a, fresh, keep, km, ke, new, nm, ne, o, om, oe))
+    out["last"] = h, he
+    if dy is None:
+        return out
+    g, gm, ge = dlast.clone(), dlast.abs(), torch.zeros_like(dlast)
+    adds = {n: torch.zeros_like(out[n][0]) for n in ("dA", "dD", "dbias")}           # magnitudes: a sum over all tokens adds as many roundings
+    for t in range(time - 1, -1, -1):
+        on, a, rel_a, fresh, keep, km, ke, new, nm, ne, o, om, oe = tape[t]
+        on3, dt_, rd, Bt, Ct, ut = on[..., None], d[:, t], rel_d[:, t], B[:, t, None], C[:, t, None], u[:, t]
+        dyt = torch.where(on, dy[:, t], zero)
+        do = dyt * gate[:, t]
+        dom, doe = do.abs(), do.abs() * gate_rel[:, t]
+        G, Gm = g + do[..., None] * Ct, gm + dom[..., None] * Ct.abs()
+        Ge = ge + doe[..., None] * Ct.abs() + 3 * U * Gm
+        live = [torch.where(on3, v, zero) for v in (G, Gm, Ge)]
+        both = lambda v, m, e, over: ((v).sum(over), (e + 40 * U * m).sum(over))         # a sum over channels or states, by lanes, waves and blocks
+        du_ = dt_ * ut
+
+        def put(name, value, error):
+            out[name][0][:, t], out[name][1][:, t] = torch.where(on.view(batch, *[1] * (value.dim() - 1)), value, zero), torch.where(on.view(batch, *[1] * (value.dim() - 1)), error, zero)
+        put("dz", dyt * o * slope[:, t], dyt.abs() * (oe * slope[:, t].abs() + om * (slope_err[:, t] + 4 * U)))
+        put("dC", *both(do[..., None] * new, dom[..., None] * nm, dom[..., None] * ne + doe[..., None] * nm, 1))
+        put("dB", *both(live[0] * du_[..., None], live[1] * du_.abs()[..., None], live[2] * du_.abs()[..., None] + live[1] * (du_.abs() * (rd + U))[..., None], 1))
+        gB, gBm, gBe = ((x * y).sum(-1) for x, y in zip(live, (Bt, Bt.abs(), Bt.abs())))
+        put("du", D * do + dt_ * gB, D.abs() * doe + dt_ * (gBe + gBm * (rd + (states + 4) * U)) + 4 * U * (D.abs() * dom + dt_ * gBm))
+        gk, gkm, gke = live[0] * keep, live[1] * km, live[2] * km + live[1] * ke
+        dd, ddm = ut * gB + (gk * A).sum(-1), ut.abs() * gBm + (gkm * A.abs()).sum(-1)
+        dde = ut.abs() * gBe + (gke * A.abs()).sum(-1) + (states + 10) * U * ddm
+        s = torch.sigmoid(raw[:, t])
+        draw, drawm, drawe = dd * s, ddm * s, dde * s + ddm * s * (3 * raw[:, t].abs() + 8) * U
+        draw, drawm, drawe = (torch.where(on, v, zero) for v in (draw, drawm, drawe))
+        put("ddt", draw, drawe)
+        for name, v, m, e in (("dbias", draw, drawm, drawe), ("dD", do * ut, dom * ut.abs(), doe * ut.abs()),
+                              ("dA", gk * dt_[..., None], gkm * dt_[..., None], gke * dt_[..., None] + gkm * (dt_ * (rd + 4 * U))[..., None])):
+            v, m, e = (torch.where(on.view(batch, *[1] * (v.dim() - 1)), x, zero).sum(0) for x in (v, m, e))
+            out[name] = out[name][0] + v, out[name][1] + e
+            adds[name] = adds[name] + m
+        cg, cm, ce = (torch.where(fresh, zero, v) for v in (a * G, a * Gm, a * Ge + a * Gm * rel_a))
+        g, gm, ge = (torch.where(on3, n, v) for n, v in ((cg, g), (cm, gm), (ce, ge)))
+    out["dstate"] = g, ge
+    for name, m in adds.items():
+        out[name] = out[name][0], out[name][1] + (batch * time + 40) * U * m
+    return out
+
+
+def beyond(got, want, error):
+    """how far off, in tolerances: the bound, with a twentieth for terms of second order, and the rounding of the output's type.  What passes through
+    numbers below float32's smallest normal one, 2^-126, is off by 2^-150 an operation there: together, with the factors that follow, under 2^-126 as
+    long as operations times factors stay under 2^24 (at most 500 tokens x 32 states, factors under 100, that decay from there)"""
+    kind, g = got.dtype, got.detach().double().cpu()
+    error = 1.05 * error + 2.0 ** -126
+    tol = error + torch.finfo(kind).eps / 2 * (want.abs() + error) + torch.finfo(kind).tiny * torch.finfo(kind).eps
+    return (g - want).abs() / tol
+
+
+def rand(gen, *shape, scale=1.0, kind=torch.float64):
+    return (torch.randn(shape, generator=gen, dtype=torch.float64) * scale).to(kind).double()
+
+
+def inputs(seed, batch, time, width, states, kind, slow=2e-3):
+    """rates from `slow` to 4 and steps around 0.1: memories of a few to some thousand tokens"""
+    gen = torch.Generator().manual_seed(seed)
+    u, dt, z, B, C = (rand(gen, batch, time, n, kind=kind) for n in (width, width, width, states, states))
+    A = -torch.exp(torch.rand((width, states), generator=gen, dtype=torch.float64) * (np.log(4) - np.log(slow)) + np.log(slow)).float().double()
+    D, bias, state = rand(gen, width, kind=torch.float32), (rand(gen, width, scale=0.5) - 2.2).float().double(), rand(gen, batch, width, states, kind=torch.float32)
+    dy, dlast = rand(gen, batch, time, width, kind=kind), rand(gen, batch, width, states, kind=torch.float32)
+    return (u, dt * 0.5, A, B, C, D, z, bias, state), dy, dlast, gen
+
+
+def on_gpu(ins, kind, grad=False):
+    return [t.to("cuda", kind if k in (0, 1, 3, 4, 6) else torch.float32).requires_grad_(grad) for k, t in enumerate(ins)]
+
+
+def gpu_or_none(*all_):
+    return [t.cuda() if t is not None else None for t in all_]
+
+
+# ---- values and gradients within the bound ----
+@gpu
+@pytest.mark.parametrize("batch,time,width,states", [(1, 700, 70, 16), (2, 1500, 33, 4), (1, 500, 130, 32), (2, 90, 256, 16), (3, 50, 192, 7), (2, 60, 128, 32), (2, 70, 250, 20)])
+def test_scan_within_the_decaying_bound(batch, time, width, states):
+    """rows cut into segments, blocks of one to four waves, more than 16 states in two pairs of waves"""
+    ins, dy, dlast, gen = inputs(time + width, batch, time, width, states, torch.float32)
+    few = torch.rand((batch, time), generator=gen) < 2.0 / time
+    ends = torch.randint(time // 2, time, (batch,), generator=gen, dtype=torch.int32)
+    for reset, lengths in ((None, None), (few, ends)):
+        want = recurrence(*ins, reset, lengths, dy, dlast)
+        leaves = on_gpu(ins, torch.float32, True)
+        r, n = gpu_or_none(reset, lengths)
+        y, last = sequence.selective_scan(*leaves[:8], state=leaves[8], reset=r, lengths=n)
+        grads = torch.autograd.grad((y, last), leaves, (dy.float().cuda(), dlast.float().cuda()))
+        for name, got in zip(NAMES, (y, last, *grads)):
+            off = beyond(got, *want[name])
+            assert off.max() <= 1, f"{name}: {int((off > 1).sum())} of {off.numel()} values off, by up to {float(off.max()):.3g} of the tolerance"
+
+
+@pytest.mark.parametrize("batch,time,width,states", [(1, 700, 70, 16), (2, 1500, 33, 4)])
+def test_the_bound_tells_a_state_of_fewer_bits(batch, time, width, states):
+    """the mistakes are planted in the recurrence itself: its states, or every 48th of them (what a segment begins with), or what a segment begins with
+    left out by a thousandth; float32 states pass"""
+    ins, *_ = inputs(time + width, batch, time, width, states, torch.float32)
+    want = recurrence(*ins, None, None, None, None)
+
+    def off(keep):
+        got = recurrence(*ins, None, None, None, None, keep_state=keep)
+        return [float(beyond(got[n][0].float(), *want[n]).max()) for n in ("y", "last")]
+    at_borders = lambda f: lambda t, h: f(h) if t % 48 == 47 else h
+    assert max(off(lambda t, h: h.float().double())) <= 1
+    assert off(lambda t, h: h.bfloat16().double())[0] > 1
+    assert off(at_borders(lambda h: h.bfloat16().double()))[0] > 1
+    assert off(at_borders(lambda h: h * 0.999))[0] > 1
