@@ -416,7 +416,8 @@ template <class T, int NS> __global__ __launch_bounds__(256) void scan_segment_b
 // its last (from the segment that the row ends in; those behind it are not read).  J threads share a row's chain: each runs over its
 // stretch of the segments from zero, then from what the stretches before it make of the row's own state.  (1 x 4096 x 1024 x 16, a
 // chain of 512 segments: forward 57 us with eight threads, 67 us with one; where the chains fill the card by themselves one is better,
-// 12 x 1000 x 640 x 16: 9 us, with eight 18 us.)
+// 12 x 1000 x 640 x 16: 9 us, with eight 18 us.)  Chains are counted without the padding of their states, which may differ between a
+// pass that is recorded and one that is not: both add in the same order.
 static int joiners(int64_t chains, int segments) {
     return segments <= 16 ? 1 : chains * 8 <= 4 * kSimds * kWave ? 8 : chains * 4 <= 4 * kSimds * kWave ? 4 : 1;
 }
@@ -946,9 +947,8 @@ template <class T, int NS> static void spread_go(const mws_scan_args *a, const S
                            const_cast<float *>(d.bc), a->batch, a->length, a->B_batch, a->B_time, a->C_batch, a->C_time, a->states);
 }
 static void join_go(const ScanArgs &d, int ns, bool backward, hipStream_t stream) {
-    const int64_t chains = d.batch * ns * d.width;
-    const int j = joiners(chains, d.segments);
-    dim3 grid((unsigned)ceil_div(chains, 256 / j));
+    const int j = joiners(d.batch * d.states * d.width, d.segments);
+    dim3 grid((unsigned)ceil_div(d.batch * ns * d.width, 256 / j));
     if (j == 8) hipLaunchKernelGGL(scan_join<8>, grid, dim3(256), 0, stream, d, ns, backward);
     else if (j == 4) hipLaunchKernelGGL(scan_join<4>, grid, dim3(256), 0, stream, d, ns, backward);
     else hipLaunchKernelGGL(scan_join<1>, grid, dim3(256), 0, stream, d, ns, backward);

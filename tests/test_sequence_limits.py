@@ -162,3 +162,19 @@ def test_the_bound_tells_a_state_of_fewer_bits(batch, time, width, states):
     assert off(lambda t, h: h.bfloat16().double())[0] > 1
     assert off(at_borders(lambda h: h.bfloat16().double()))[0] > 1
     assert off(at_borders(lambda h: h * 0.999))[0] > 1
+
+
+# ---- recorded or not ----
+@gpu
+@pytest.mark.parametrize("kind", [torch.float32, torch.float16])
+@pytest.mark.parametrize("batch,time,width,states", [(4, 1000, 600, 12), (6, 1000, 768, 12), (2, 1000, 600, 20), (3, 700, 340, 9)])
+def test_recording_changes_no_bit_of_cut_rows(kind, batch, time, width, states):
+    """numbers of states whose padding differs with recording, at sizes where the number of chains over the segments, so padded, would lie on both sides of a limit"""
+    gen = torch.Generator(device="cuda").manual_seed(time + width + states)
+    r = lambda *s, k=kind: torch.randn(s, generator=gen, device="cuda").to(k)
+    args = [r(batch, time, width), r(batch, time, width) - 2, -torch.rand(width, states, generator=gen, device="cuda"), r(batch, time, states), r(batch, time, states)]
+    state = r(batch, width, states, k=torch.float32)
+    with torch.no_grad():
+        y, last = sequence.selective_scan(*args, state=state)
+    again, last2 = sequence.selective_scan(*[t.requires_grad_() for t in args], state=state)
+    assert torch.equal(y, again) and torch.equal(last, last2)
