@@ -447,7 +447,16 @@ template <int J> __global__ __launch_bounds__(256) void scan_join(ScanArgs a, in
             sum[j] = there ? a.sum[place(k) * a.width + e] : 0.0f;
         }
     };
-    auto next = [&](float h, float s, float l) __attribute__((always_inline)) { return s < 0.0f || h == 0.0f ? l : __builtin_fmaf(exp2_(s * A2), h, l); };
+    // A factor above 2^126 (a rate above zero) as three: it may pass the range of a number where its product with a small state does not.
+    auto next = [&](float h, float s, float l) __attribute__((always_inline)) {
+        if (s < 0.0f || h == 0.0f) return l;
+        const float p = s * A2;
+        if (p > 126.0f) {
+            const float third = exp2_(p * (1.0f / 3));
+            return __builtin_fmaf(third, h * third * third, l);
+        }
+        return __builtin_fmaf(exp2_(p), h, l);
+    };
     float h = first;
     if constexpr (J > 1) {
         float total = 0;

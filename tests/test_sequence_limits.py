@@ -178,3 +178,35 @@ def test_recording_changes_no_bit_of_cut_rows(kind, batch, time, width, states):
         y, last = sequence.selective_scan(*args, state=state)
     again, last2 = sequence.selective_scan(*[t.requires_grad_() for t in args], state=state)
     assert torch.equal(y, again) and torch.equal(last, last2)
+
+
+# ---- growing states ----
+@gpu
+@pytest.mark.parametrize("at,count,step,start", [(40, 8, 12.0, 1e-20), (40, 8, 17.0, 1e-38), (200, 8, 12.0, 1e-20), (33, 60, 1.5, 1e-20), (40, 8, 17.0, 1e-20)])
+@pytest.mark.parametrize("width,states", [(20, 4), (70, 9)])
+def test_states_that_grow_in_a_cut_row(width, states, at, count, step, start):
+    """rates above zero, no steps but `count` large ones: a segment's factor of up to 2^138 or 2^196 on a state of 1e-20 or 1e-38 is a number, and what
+    passes the range (the last case) is an infinity, as token by token"""
+    time = 400
+    dt = torch.full((1, time, width), -20.0, dtype=torch.float64)
+    dt[:, at:at + count] = step
+    u, C = torch.zeros(1, time, width, dtype=torch.float64), torch.ones(1, time, states, dtype=torch.float64)
+    A = torch.linspace(-1, 1, width * states, dtype=torch.float64).view(width, states).float().double()
+    small = torch.full((1, width, states), start, dtype=torch.float64).float().double()
+    ins = (u, dt, A, C, C, torch.zeros(width, dtype=torch.float64), torch.full_like(u, 1.0), torch.zeros(width, dtype=torch.float64), small)
+    dy, dlast = torch.zeros_like(u), small * 0.5
+    want = recurrence(*ins, None, None, dy, dlast)
+    leaves = on_gpu(ins, torch.float32, True)
+    y, last = sequence.selective_scan(*leaves[:8], state=leaves[8])
+    outputs = [y, last]
+    most = torch.finfo(torch.float32).max
+    passes = want["last"][0].max() > 2 * most
+    if not passes:                   # (where a state passes the range, so do factors of gradients that do not)
+        outputs += torch.autograd.grad((y, last), leaves, (dy.float().cuda(), dlast.float().cuda()))
+    for name, got in zip(NAMES, outputs):
+        value, error = want[name]
+        inside = (value.abs() + 2 * error) < most / 2
+        assert inside.any() and torch.isfinite(got.cpu()[inside]).all(), name
+        assert (beyond(got, value, error)[inside] <= 1).all(), name
+        assert torch.isposinf(got.cpu()[value - 2 * error > 2 * most]).all(), name
+    assert passes == (step == 17.0 and start == 1e-20) and want["last"][0].max() > 1e18
