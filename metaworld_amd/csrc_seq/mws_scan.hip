@@ -451,6 +451,7 @@ template <int J> __global__ __launch_bounds__(256) void scan_join(ScanArgs a, in
     auto next = [&](float h, float s, float l) __attribute__((always_inline)) {
         if (s < 0.0f || h == 0.0f) return l;
         const float p = s * A2;
+        if (__builtin_isinf(h)) return h + l;            // token by token it stays infinite, though the whole factor may be too small for a number
         if (p > 126.0f) {
             const float third = exp2_(p * (1.0f / 3));
             return __builtin_fmaf(third, h * third * third, l);

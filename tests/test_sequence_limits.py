@@ -210,3 +210,24 @@ def test_states_that_grow_in_a_cut_row(width, states, at, count, step, start):
         assert (beyond(got, value, error)[inside] <= 1).all(), name
         assert torch.isposinf(got.cpu()[value - 2 * error > 2 * most]).all(), name
     assert passes == (step == 17.0 and start == 1e-20) and want["last"][0].max() > 1e18
+
+
+# ---- infinities ----
+def classes(t):
+    t = t.detach().double().cpu()
+    return torch.where(t.isnan(), 3.0, torch.where(t.isinf(), t.sign(), 0.0))
+
+
+@gpu
+def test_an_infinite_state_stays_one_over_segments():
+    """a state that is infinite decays to an infinity, also where a segment's factor as a whole is too small for a number"""
+    batch, time, width, states = 1, 500, 30, 8
+    ins, *_ = inputs(3, batch, time, width, states, torch.float32, slow=1.0)
+    u, dt, A, B, C, D, z, bias, state = ins
+    dt = torch.full_like(dt, 3.0)
+    state[0, ::2] = float("inf")
+    ins = (u, dt, A, B, C, D, z, bias, state)
+    want = recurrence(*ins, None, None, None, None)
+    leaves = on_gpu(ins, torch.float32)
+    y, last = sequence.selective_scan(*leaves[:8], state=leaves[8])
+    assert torch.equal(classes(last), classes(want["last"][0])) and (classes(last) == 1).any() and torch.equal(classes(y), classes(want["y"][0]))
