@@ -573,16 +573,17 @@ template <class T, int NS, int H> __global__ __launch_bounds__(256, 2) void scan
                 Pair<S> m, m2;
                 auto token = [&](int q) __attribute__((always_inline)) { return bc + (q < here ? q : here - 1) * 2 * ALL; };
                 B[0].read(token(0));
+                uint32_t unseen = begins | ~0u << here;          // where no state is seen from: nothing behind the row sees its last one, which may be infinite
 #pragma unroll
                 for (int q = 0; q < SUB; q++) {
                     B[q & 1].hold();
-                    asm volatile("" : "+s"(bc), "+s"(here), "+s"(begins));         // no comparison held for later, no B kept for the way back
+                    asm volatile("" : "+s"(bc), "+s"(here), "+s"(unseen));         // no comparison held for later, no B kept for the way back
                     if (q + 1 < SUB) B[~q & 1].read(token(q + 1));
                     else m.read(token(q), ALL);
                     here_only();
                     d[q] = q < here ? softplus_(up<T>(rd[q]) + bias) : 0.0f;
                     float x = q < here ? d[q] * up<T>(ru[q]) : 0.0f;
-                    if (begins >> q & 1) forget<NS>(h);
+                    if (unseen >> q & 1) forget<NS>(h);
 #pragma unroll
                     for (int n = 0; n < NS; n++) {
                         keep[q][n] = exp2_(d[q] * A2[n]) * h[n];

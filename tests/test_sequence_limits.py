@@ -231,3 +231,18 @@ def test_an_infinite_state_stays_one_over_segments():
     leaves = on_gpu(ins, torch.float32)
     y, last = sequence.selective_scan(*leaves[:8], state=leaves[8])
     assert torch.equal(classes(last), classes(want["last"][0])) and (classes(last) == 1).any() and torch.equal(classes(y), classes(want["y"][0]))
+
+
+@gpu
+@pytest.mark.parametrize("time,end", [(13, 13), (24, 19)])
+def test_an_infinity_in_a_rows_last_token_reaches_no_rate(time, end):
+    """what comes behind a row's last token counts for nothing: dA has no term of the last state"""
+    ins, dy, dlast, _ = inputs(5, 1, time, 9, 8, torch.float32)
+    ins[0][0, end - 1, 4] = float("inf")
+    dy[0, end - 1] = 0
+    lengths = torch.tensor([end], dtype=torch.int32)
+    want = recurrence(*ins, None, lengths, dy, dlast)["dA"]
+    leaves = on_gpu(ins, torch.float32, True)
+    out = sequence.selective_scan(*leaves[:8], state=leaves[8], lengths=lengths.cuda())
+    dA, = torch.autograd.grad(out, leaves[2:3], (dy.float().cuda(), dlast.float().cuda()))
+    assert torch.isfinite(want[0]).all() and (beyond(dA, *want) <= 1).all()
