@@ -219,6 +219,42 @@ def classes(t):
 
 
 @gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("states", [1, 3, 5, 6, 9, 12, 13, 18, 20, 24, 29, 31, 32])
+@pytest.mark.parametrize("where", ["u", "dt"])
+def test_infinite_inputs_give_infinities(kind, states, where):
+    """an infinite input or step makes states infinite, until an episode begins: not the padding of a number of states, which counts for nothing, NaN"""
+    batch, time, width = 2, 60, 40
+    ins, dy, dlast, gen = inputs(states, batch, time, width, states, kind)
+    u, dt, A, B, C, D, z, bias, state = ins
+    B, C, z, u, D = B.abs() + 0.25, C.abs() + 0.25, z.abs() + 0.25, u.abs() + 0.25, D.abs()
+    (u if where == "u" else dt)[0, 17, ::3] = float("inf")
+    (u if where == "u" else dt)[1, 59, 1] = float("inf")
+    reset = torch.zeros(batch, time, dtype=torch.bool)
+    reset[0, 33] = True
+    u, B, C, z, D = (t.to(kind).double() for t in (u, B, C, z, D))          # the numbers that the kernels get
+    ins = (u, dt, A, B, C, D, z, bias, state)
+    want = recurrence(*ins, reset, None, None, None)
+    leaves = on_gpu(ins, kind)
+    y, last = sequence.selective_scan(*leaves[:8], state=leaves[8], reset=reset.cuda())
+    for name, got in (("y", y), ("last", last)):
+        value, error = want[name]
+        assert torch.equal(classes(got), classes(value)) and (classes(value) == 1).any(), name
+        assert (beyond(got, value, error)[classes(value) == 0] <= 1).all(), name
+    for t in leaves:
+        t.requires_grad_()
+    again = sequence.selective_scan(*leaves[:8], state=leaves[8], reset=reset.cuda())
+    assert torch.equal(torch.nan_to_num(again[0]), torch.nan_to_num(y)) and torch.equal(torch.nan_to_num(again[1]), torch.nan_to_num(last))
+    # where the formula has a number, padding makes it no NaN: gradients of the tokens before an infinite step, which wipes the states, and of those of the other episode
+    grads = torch.autograd.grad(again, leaves, (dy.to("cuda", kind), dlast.float().cuda()))
+    want = recurrence(*ins, reset, None, dy, dlast)
+    for name, got in zip(NAMES[2:], grads):
+        value, error = want[name]
+        inside = torch.isfinite(value) & torch.isfinite(error)
+        assert torch.isfinite(got.cpu()[inside]).all() and (beyond(got, value, error)[inside] <= 1).all(), name
+
+
+@gpu
 def test_an_infinite_state_stays_one_over_segments():
     """a state that is infinite decays to an infinity, also where a segment's factor as a whole is too small for a number"""
     batch, time, width, states = 1, 500, 30, 8
