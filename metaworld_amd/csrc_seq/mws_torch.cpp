@@ -3,6 +3,8 @@
 // action of 50 environments) are bound by the host: a call costs 4 us here and 14 us through ctypes, a recorded forward and backward
 // pass 36 us and 143 us (layer norm of 50 x 256).
 #include <torch/extension.h>
+#include <ATen/TracerMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include "../../include/mwseq.h"
 
@@ -25,6 +27,12 @@ std::string shape_of(at::IntArrayRef s) {
 }
 int type_of(at::ScalarType t) { return t == at::kFloat ? MWS_F32 : t == at::kBFloat16 ? MWS_BF16 : t == at::kHalf ? MWS_F16 : -1; }
 
+// a recording of torch's own operations has the memory of the outputs and not the kernels that fill it
+void want_untraced() {
+    using Modes = c10::impl::TorchDispatchModeTLS;
+    const bool traced = at::tracer::impl::is_dispatch_enabled() || (Modes::any_modes_set() && Modes::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value());
+    TORCH_CHECK(!traced, "the sequence operators cannot be traced (torch.jit.trace, torch.fx): a trace would hold their outputs' memory without the kernels that fill it");
+}
 void want_activations(const char *what, const Tensor &t, int64_t dims = -1) {
     TORCH_CHECK_TYPE(t.defined(), what, " has to be a tensor");
     TORCH_CHECK_TYPE(type_of(t.scalar_type()) >= 0, what, " is ", t.scalar_type(), ": float32, bfloat16 and float16 are supported");
@@ -140,6 +148,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     }
 };
 Tensor layer_norm(const Tensor &x, const Maybe &weight_, const Maybe &bias_, double eps) {
+    want_untraced();
     Tensor weight = given(weight_), bias = given(bias_);
     want_activations("x", x);
     int64_t width = x.size(-1);
@@ -205,6 +214,7 @@ void conv_check(const Tensor &x, const Tensor &weight, const Tensor &bias, const
     want("state", state, {x.size(0), weight.size(1) - 1, width}, x.scalar_type(), x);
 }
 variable_list causal_conv(Tensor x, Tensor weight, const Maybe &bias_, const Maybe &state_, const Maybe &reset_, const Maybe &lengths_) {
+    want_untraced();
     Tensor bias = given(bias_), state = given(state_), reset = given(reset_), lengths = given(lengths_);
     conv_check(x, weight, bias, state, 3);
     want_tokens(x, true, reset, lengths);
@@ -213,6 +223,7 @@ variable_list causal_conv(Tensor x, Tensor weight, const Maybe &bias_, const May
     return records({x, weight, bias, state}) ? CausalConv::apply(x, weight, maybe(bias), maybe(state), maybe(reset), maybe(lengths), needs({x, weight, bias, state})) : conv_forward(x, weight, bias, state, reset, lengths);
 }
 Tensor causal_conv_step(Tensor x, Tensor weight, const Maybe &bias_, const Maybe &state_, const Maybe &reset_) {
+    want_untraced();
     Tensor bias = given(bias_), state = given(state_), reset = given(reset_);
     conv_check(x, weight, bias, state, 2);
     want_tokens(x, false, reset, Tensor());
@@ -287,6 +298,7 @@ struct SelectiveScan : torch::autograd::Function<SelectiveScan> {
 };
 ScanIn scan_check(const Tensor &u, const Tensor &dt, const Tensor &A, const Tensor &B, const Tensor &C, const Maybe &D, const Maybe &z, const Maybe &dt_bias, const Maybe &state, const Maybe &reset,
                   const Maybe &lengths, int64_t dims) {
+    want_untraced();
     ScanIn t = {u, dt, A, B, C, given(D), given(z), given(dt_bias), given(state), given(reset), given(lengths)};
     want_activations("u", u, dims);
     int64_t width = u.size(-1);

@@ -15,6 +15,9 @@ state nor earlier tokens are seen.  `lengths` (int32 [batch]) says how many toke
 others' inputs are not looked at, their outputs and gradients are zero, and the returned state is that after the last token that
 counts.  Gradients are deterministic (no atomic additions) and not differentiable again (create_graph is refused, as are forward
 derivatives).  A call gives the same values to the last bit whether it is recorded for them or not.
+
+Calls are no operations that torch knows: they run inside torch.compile's programs between its graphs, and raise where torch records
+its operations (torch.jit.trace, torch.fx), which would hold their outputs' memory and not the kernels that fill it.
 """
 from __future__ import annotations
 

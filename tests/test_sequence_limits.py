@@ -12,6 +12,8 @@ import numpy as np
 import pytest
 import torch
 
+from torch.fx.experimental.proxy_tensor import make_fx
+
 from metaworld_amd import sequence
 
 gpu = pytest.mark.gpu
@@ -282,3 +284,16 @@ def test_an_infinity_in_a_rows_last_token_reaches_no_rate(time, end):
     out = sequence.selective_scan(*leaves[:8], state=leaves[8], lengths=lengths.cuda())
     dA, = torch.autograd.grad(out, leaves[2:3], (dy.float().cuda(), dlast.float().cuda()))
     assert torch.isfinite(want[0]).all() and (beyond(dA, *want) <= 1).all()
+
+
+# ---- what the calls refuse ----
+def test_tracing_is_refused():
+    """a traced function would hold the outputs' memory and not the kernels that fill it"""
+    w, A = torch.zeros(6, 4), -torch.ones(6, 3)
+    x, s = torch.zeros(2, 5, 6), torch.zeros(2, 5, 3)
+    held, h = torch.zeros(2, 3, 6), torch.zeros(2, 6, 3)
+    for call in (lambda x: sequence.layer_norm(x), lambda x: sequence.causal_conv(x, w), lambda x: sequence.causal_conv_step(x[:, 0], w, state=held),
+                 lambda x: sequence.selective_scan(x, x, A, s, s), lambda x: sequence.selective_scan_step(x[:, 0], x[:, 0], A, s[:, 0], s[:, 0], state=h)):
+        for trace in (lambda: torch.jit.trace(call, (x,)), lambda: make_fx(call)(x)):
+            with pytest.raises(RuntimeError, match="cannot be traced"):
+                trace()
