@@ -16,7 +16,8 @@
  * neither the state nor any earlier token of the row is seen from there on.  `lengths` (int32 [batch], may be NULL): how many
  * tokens of a row count, taken into [0, length]; outputs and gradients of the others are zero, their inputs are not used.
  *
- * Sizes of which one launch would need 2^32 threads or more (2^26 rows of one token, 2^27 tokens of 16 states backward) are refused.
+ * Sizes of which one launch would need 2^32 threads or more (2^26 rows of one token) are refused, and scans with 2^32 values of dB and
+ * dC together (2^27 tokens of 16 states), both backward and forward with `kept`.
  */
 #ifndef MWSEQ_H
 #define MWSEQ_H

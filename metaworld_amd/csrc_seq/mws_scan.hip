@@ -1069,14 +1069,19 @@ extern "C" int64_t mws_scan_workspace(const mws_scan_args *a, int32_t backward) 
     return scan_plan(a, backward != 0).bytes;
 }
 
+// whether the launches can count their threads.  dB's and dC's kernel counts its values, four times its threads.
+static bool scan_fits(const mws_scan_args *a, const ScanPlan &p, bool backward) {
+    return fits(a->batch * p.segments * p.across, p.lanes) && (!backward || fits(ceil_div(a->batch * a->length * 2 * p.ns, 256), 256)) && fits(ceil_div(a->length * 2 * p.ns / 4, 256), 256) &&
+           (p.segments <= 1 || fits(ceil_div(a->batch * p.ns * a->width, 256), 256)) && fits(ceil_div((int64_t)(p.ns + 2) * a->width, 32), 1024);
+}
+
 static int32_t scan_call(const mws_scan_args *a, const char *what, bool backward, void *stream) {
     if (int32_t e = scan_check(a, what, backward, false, true)) return e;
     ScanPlan p = scan_plan(a, backward);
     if (a->workspace_bytes < p.bytes || (p.bytes > 0 && a->workspace == nullptr)) return fail("%s: the workspace needs %lld bytes", what, (long long)p.bytes);
     if (!backward && a->batch == 0) return 0;
-    const int64_t tokens = a->batch * a->length;
-    if (!fits(a->batch * p.segments * p.across, p.lanes) || (backward && !fits(ceil_div(tokens * 2 * p.ns, 256), 256)) || !fits(ceil_div(a->length * 2 * p.ns / 4, 256), 256) ||
-        (p.segments > 1 && !fits(ceil_div(a->batch * p.ns * a->width, 256), 256)) || !fits(ceil_div((int64_t)(p.ns + 2) * a->width, 32), 1024))
+    // (a pass that is recorded, before its backward pass would be refused)
+    if (!scan_fits(a, p, backward) || (!backward && a->kept != nullptr && !scan_fits(a, scan_plan(a, true), true)))
         return fail("%s: %lld rows of %lld tokens, %d channels and %d states are more than one launch can count", what, (long long)a->batch, (long long)a->length, a->width, a->states);
     scan_run(a, p, scan_device(a, p), backward, (hipStream_t)stream);
     return launched(what);

@@ -8,6 +8,8 @@ has a constant and a product more (4 U), its exp2 3 U; where a row is cut, d is 
 most SUMMED additions, U each).  A state is what is kept of the one before, with that one's error, and its own terms; a cut row adds it up
 twice.  So an error lives as long as the state it is in, and the bound does not grow with the row.
 """
+import struct
+
 import numpy as np
 import pytest
 import torch
@@ -297,3 +299,11 @@ def test_tracing_is_refused():
         for trace in (lambda: torch.jit.trace(call, (x,)), lambda: make_fx(call)(x)):
             with pytest.raises(RuntimeError, match="cannot be traced"):
                 trace()
+
+
+def test_a_recorded_scan_is_refused_where_its_backward_pass_would_be():
+    """more of dB and dC than is counted: said by the forward pass that keeps states, before it launches anything"""
+    lib = sequence.library()
+    args = struct.pack("@26Q17q4i", *[64] * 11, 0, 0, *[64] * 13, 1 << 17, 1 << 10, *[0] * 14, 1 << 60, 8, 16, 1, 0)
+    for f in (lib.mws_scan_backward, lib.mws_scan_forward):
+        assert f(args, None) == -1 and "count" in lib.mws_last_error().decode()
