@@ -7,7 +7,7 @@
  * thread).  All pointers but the argument struct are device pointers owned by the caller.  The library holds no state and no
  * device memory: scratch memory is the caller's `workspace`, of at least the bytes that the _workspace function returns for the
  * same struct (pointers in it are looked at for being NULL or not, nothing else); two calls that may run at the same time need
- * workspaces of their own.
+ * workspaces of their own.  Pointers are aligned as their elements are, workspaces as float.
  *
  * Activations are MWS_F32, MWS_BF16 or MWS_F16 (`type`); their last dimension is contiguous, the strides of the others are given
  * in elements.  Parameters are float or of the activations' type (`param_type`).  Sums, statistics and scan states are float.

@@ -5,8 +5,8 @@
 //
 // where x of a token before the row's first comes from the state, and of one before the episode's first is zero.
 //
-// Bound by memory, 512 x 128 x 1024 bf16 forward in 55 us (4.9 TB/s; a copy of 4 GiB reaches 4.8), backward in 92 us (4.4 TB/s, the vector
-// unit at it for most of the time), one token of 4096 x 1024 bf16 in 14 us (4.7 TB/s).  A lane keeps V neighbouring channels (one 16-byte access a token), a wave walks over a tile of tokens with the
+// Bound by memory, 512 x 128 x 1024 bf16 forward in 55 us (4.9 TB/s; a copy of 4 GiB reaches 4.8), backward in 93 us (4.3 TB/s, the vector
+// unit at it for most of the time), one token of 4096 x 1024 bf16 in 13 us (5.1 TB/s; of 4096 x 1023, one value to a lane, 14 us).  A lane keeps V neighbouring channels (one 16-byte access a token), a wave walks over a tile of tokens with the
 // last K of them in registers, so that every value is read once but for K - 1 tokens at a tile's edge (backward 2 K - 2).  The episodes' beginnings
 // of a tile are one 64-bit mask in scalar registers.
 #include "mws_common.hpp"
@@ -182,7 +182,7 @@ template <class T, int V, int K> __global__ __launch_bounds__(256) void conv_for
 
 // A wave walks from its tile's first token to K - 1 tokens past it: it takes dw and db of its own tokens, and dx of them, whose last
 // terms come from the tokens past the tile.  The state's K - 1 inputs count as tokens before the first.  Four waves to a SIMD: with the
-// next four tokens under way they do not fit (12 x 1000 x 640 fp32 with the forward pass 41 us, 79 us so; with three waves 51 us).
+// next four tokens under way they do not fit (12 x 1000 x 640 fp32 with the forward pass 41 us when it was built, 79 us so; with three waves 51 us).
 template <class T, int V, int K> __global__ __launch_bounds__(256, 4) void conv_backward(ConvArgs a) {
     using raw = typename T::raw;
     int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), waves = blockDim.x / kWave;
@@ -381,7 +381,7 @@ static int conv_v(const mws_conv_args *a) {
     return a->width >= v ? v : 1;
 }
 // backward four of any type: with eight the weights, inputs, sums and gradients of the taps leave two waves to a SIMD (512 x 128 x 1024
-// bf16 102 us when with eight it was 118 us)
+// bf16 with eight 118 us when with four it was 102 us)
 static int conv_back_v(const mws_conv_args *a) { return a->width >= 4 ? 4 : 1; }
 static int conv_tile(const mws_conv_args *a) {
     int64_t across = a->batch * ceil_div(a->width, kWave * conv_v(a));

@@ -72,7 +72,7 @@ template <class T, int V, int PER, int TPR> struct Row {
         }
     }
     // whole vectors: a condition for each value is a branch with a wait of its own, and every block begins with them (8000 x 512 bf16
-    // forward 5.7 us, 11.4 us value by value)
+    // forward 6 us, 11 us value by value)
     __device__ __forceinline__ void read_param(const void *p, int lane, int width, bool wide, float otherwise) {
 #pragma unroll
         for (int k = 0; k < PER; k++) {
@@ -207,9 +207,10 @@ struct NormOut {
     }
 };
 
-// Threads of a row: eight values each from 1025 columns on (16384 x 4096 bf16 forward 65 us, backward 116 us; with sixteen 71 and
-// 160 us).  Blocks walk over the rows, 4096 waves in all (262144 x 512 bf16 forward 123 us, backward 170 us; with twice as many 128
-// and 195 us); twice that forward in blocks of 1024 threads, two of which fit a compute unit (4000 x 16384 fp32 116 us, not 182).
+// Threads of a row: eight values each from 1025 columns on (16384 x 4096 bf16 forward 53 us, backward 115 us; with sixteen 71 and
+// 160 us when with eight it was 65 and 116).  Blocks walk over the rows, 4096 waves in all (262144 x 512 bf16 forward 123 us, backward 170 us; with twice as many 128
+// and 195 us); twice that forward in blocks of 1024 threads, two of which fit a compute unit (4000 x 16384 fp32 113 us, not 182).  Beyond 8192 columns a thread has sixteen again, and backward some registers
+// do not fit (bf16 28, fp16 16 spilled; 4000 x 16384 bf16 backward 140 us, 2.8 TB/s; fp32 183 us, 4.3 TB/s).
 static int norm_rows(int tpr) { return tpr <= kWave ? 256 / tpr : 1; }
 static int norm_tpr(const mws_norm_args *a) {
     int v = a->type == MWS_F32 ? 4 : 8, w = a->width;

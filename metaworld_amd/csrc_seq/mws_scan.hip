@@ -11,7 +11,8 @@
 // scalar registers, from a small copy in float, [token][B | C][states], that `spread` makes first (128 bytes a token next to the
 // channels' 8 bytes each).  A wave walks along the time axis; u, dt, z and y are read and written in order of channels.
 // Bound by the vector unit: per value and state one exp (two issue slots) and four multiplications or additions forward, 147
-// slots a token and wave with 16 states.  2048 x 64 x 512 x 16 bf16 forward in 259 us, every slot taken; the memory would allow 140.
+// slots a token and wave with 16 states.  2048 x 64 x 512 x 16 bf16 forward in 267 us with the copy of B and C (7 us), 251 us of them slots; the
+// memory would allow 140.
 //
 // Where batch x channels leave the card empty, the time axis is cut into segments: scan_segment takes each
 // segment's end state from zero and its sum of d (the product of its a is exp(A sum d)), scan_join runs over the segments, and the
@@ -126,7 +127,7 @@ __device__ __forceinline__ Fixed *fixed(const float *p) { return (Fixed *)(uintp
 // They are asked for one step ahead: a step's values are in `hold`'s registers when the next step's loads go out, which then have that
 // step's time to arrive (scalar loads may overtake each other, so that a wait is for all of them).  A step is some of a token's states
 // of B and C (half of 16), or a whole token's of one of them, since the scalar registers hold no more.  (2048 x 64 x 512 x 16 bf16 with the
-// backward pass 1448 us, 1564 us with a token's values asked for where they are needed; 3 x 5000 x 777 x 12 fp16 109 us, not 117.)
+// backward pass 1448 us when it was built, 1564 us with a token's values asked for where they are needed; 3 x 5000 x 777 x 12 fp16 109 us, not 117.)
 template <int S> struct Pair {
     float B[S], C[S];
     __device__ __forceinline__ void read(Fixed *p, int all) {
@@ -147,7 +148,7 @@ __device__ __forceinline__ void here_only() { __builtin_amdgcn_sched_barrier(0);
 
 // a lane's states: NS of them from `first` on, of a row of `states` (padded with zeros).  All loads go out before the first is waited
 // for: a condition for each of them would be a branch with a wait of its own, and every wave begins with them (2048 x 64 x 512 x 16
-// bf16 forward 271 us, 314 us so; 405 x 66 x 874 x 32 211 us, not 278).
+// bf16 forward 271 us when it was built, 314 us so; 405 x 66 x 874 x 32 211 us, not 278).
 template <int NS> __device__ __forceinline__ void get_states(const float *row, int states, int first, float (&h)[NS]) {
     if (states % 4 == 0) {
         Vec<F32, 4> r[NS / 4];
@@ -425,9 +426,9 @@ template <class T, int NS> __global__ __launch_bounds__(256) void scan_segment_b
 // Every segment's incoming state, in the place of what it left from zero: forward the state before its first token, backward g after
 // its last (from the segment that the row ends in; those behind it are not read).  J threads share a row's chain: each runs over its
 // stretch of the segments from zero, then from what the stretches before it make of the row's own state.  (1 x 4096 x 1024 x 16, a
-// chain of 512 segments: forward 57 us with eight threads, 67 us with one; where the chains fill the card by themselves one is better,
-// 12 x 1000 x 640 x 16: 9 us, with eight 18 us.)  Chains are counted without the padding of their states, which may differ between a
-// pass that is recorded and one that is not: both add in the same order.
+// chain of over a hundred segments: bf16 forward 56 us with eight threads, 71 us with one; where the chains fill the card by themselves one
+// is better, 12 x 1000 x 640 x 16 fp32: 88 us, with eight 96 us.)  Chains are counted without the padding of their states, which may differ
+// between a pass that is recorded and one that is not: both add in the same order.
 static int joiners(int64_t chains, int segments) {
     return segments <= 16 ? 1 : chains * 8 <= 4 * kSimds * kWave ? 8 : chains * 4 <= 4 * kSimds * kWave ? 4 : 1;
 }
@@ -529,10 +530,9 @@ template <int M> __device__ __forceinline__ float wave_sums(float (&v)[M / 2]) {
 // row's end count with d = u = dy = 0, which leaves g as it is and adds nothing.
 // More than 16 states are two halves (H = 2), each a wave's: what a token's gradients need of both, its output and two sums over the
 // states, meets in shared memory, and each of the two waves finishes every second token (405 x 66 x 874 x 32 bf16 with the forward
-// pass 1120 us; 4413 us without it where all states are one wave's, most of that for registers that do not fit).
-// Bound by the vector unit: 2048 x 64 x 512 x 16 bf16 take some 1.0 ms, 403 instructions a token and wave (98 of them for the way there),
-// at 84 % of its issue slots with the two waves to a SIMD that the registers allow; three waves with half the tokens each, whose
-// registers spill, took a quarter longer.
+// pass 1120 us when it was built; 4413 us without it where all states are one wave's, most of that for registers that do not fit).
+// Bound by the vector unit: 2048 x 64 x 512 x 16 bf16 take some 1.0 ms, 403 instructions (466 issue slots) a token and wave, 98 of them for
+// the way there, at 84 % of the slots with the two waves to a SIMD that the registers allow: all 256, and 8 more in 28 bytes of scratch.  Three waves with half the tokens each, whose registers spill within them, took a quarter longer.
 template <class T, int NS, int H, bool PAD> __global__ __launch_bounds__(256, 2) void scan_backward(ScanArgs a) {
     using raw = typename T::raw;
     constexpr int SUB = kKept, M = 2 * NS, ALL = NS * H;
@@ -804,7 +804,8 @@ struct ScanOut {
 
 // ---- one token ----
 // Q lanes share a channel, four states each: the state goes through registers in 16-byte pieces, in order of memory.  Bound by memory:
-// 8 bytes a state (4096 x 1024 x 16 bf16 in 110 us, 5.2 TB/s).  Q = 0: a lane takes a channel's states one by one, for numbers of states that four lanes cannot share evenly.
+// 8 bytes a state (4096 x 1024 x 16 bf16 in 114 us, 5.0 TB/s).  Q = 0, for all numbers of states but 4, 8, 16 and 32: a lane takes a channel's
+// states one by one, bound by their round trips and scattered accesses (4096 x 1024 bf16 with 7 states 92 us, 12: 255 us, 24: 1380 us).
 // A lane keeps its channel's parameters for up to kStepRows rows; a row's state is under way while the one before is worked on.
 constexpr int kStepRows = 4;
 template <class T, int Q> __global__ __launch_bounds__(256) void scan_step(ScanArgs a, const void *B, const void *C, int64_t B_batch, int64_t C_batch, int64_t each) {
@@ -865,7 +866,7 @@ template <class T, int Q> __global__ __launch_bounds__(256) void scan_step(ScanA
 
 // ---- host ----
 // The states that a lane walks with.  Powers of two where a backward pass follows, whose sums over a wave halve them step by step;
-// steps of four and eight where none does (3 x 5000 x 777 x 12 fp16 116 us; padded to 16 states it was 134 us when this was 120).
+// 12 and 24 too where none does (3 x 5000 x 777 x 12 fp16 110 us, padded to 16 states 125 us).
 static int scan_ns(const mws_scan_args *a, bool backward) {
     int n = a->states;
     if (!backward && a->kept == nullptr && n > 8) return n <= 12 ? 12 : n <= 16 ? 16 : n <= 24 ? 24 : 32;
@@ -878,22 +879,20 @@ struct ScanPlan {
     int64_t bc, seg, sum, part_bc, part, bytes;      // offsets into the workspace, in floats
 };
 
-// Waves of a block: as many as leave the fewest of them without channels.
+// Waves of a block: as many as leave none of them without channels.
 static int block_waves(int waves, int most) {
-    int best = 1, least = waves;
-    for (int w = 2; w <= most; w++) {
-        int used = (waves + w - 1) / w * w;
-        if (used <= least || w == 1) best = w, least = used;
-    }
+    int best = 1;
+    for (int w = 2; w <= most; w++)
+        if (waves % w == 0) best = w;
     return best;
 }
 
 // Segments: how many times kKept tokens each.  kKept tokens of one wave alone take a SIMD 3 us forward and 10.5 us backward, for what
 // its instructions wait for; several waves take their issue slots' time (49 + 6 ns and 110 + 22 ns slots a token, four cycles each)
 // and some of that once.  Each wave begins with its rates and state.  Cutting costs a second walk (0.8 of the first, backward 0.25),
-// two launches and a step of scan_join for each segment.  (3 x 5000 x 777 x 12 fp16 forward in segments of 8 tokens 127 us, of 24: 86,
-// of 40: 82, of 48, which this takes: 90, of 64: 104, of 128: 136 us; 1 x 300 x 512 x 16 bf16 of 8, which this takes: 25, of 32: 36, of
-// 64: 62 us.)
+// two launches and a step of scan_join for each segment.  (3 x 5000 x 777 x 12 fp16 forward, full rows, in segments of 8 tokens 171 us, of
+// 24: 122, of 40: 112, of 48, which this takes: 109, of 64: 107, of 128: 137 us; 1 x 300 x 512 x 16 bf16 of 8, which this takes: 22, of
+// 32: 39, of 64: 59 us.)
 static int64_t best_span(int64_t waves, int64_t parts, int ns, bool backward) {
     const double alone = backward ? 10.5 : 3, slots = backward ? 110 + 22 * ns : 49 + 6 * ns, busy = slots * kKept * 4 / 2400, walks = backward ? 1.25 : 1.8;
     auto time = [&](int64_t w, int64_t each) {
@@ -1004,7 +1003,8 @@ template <class T, int NS, bool PAD> static void backward_go(const mws_scan_args
         hipLaunchKernelGGL((scan_segment_back<T, NS>), dim3((unsigned)(d.batch * p.segments * p.across)), block, 0, stream, d);
         join_go(d, NS, true, stream);
     }
-    // 25 KB a wave of a half, 8 KB for four waves without: under the 64 KB that a block has without asking for more
+    // 14 KB a wave of a half, 56 KB for the four of a block; 8 KB for four waves without halves: under the 64 KB that a block has without
+    // asking for more
     const int waves = p.lanes / kWave * H;
     size_t lds = (size_t)2 * waves * kKept * (2 * PER + (H > 1 ? 3 * kWave : 0)) * sizeof(float);
     if (d.batch > 0) hipLaunchKernelGGL((scan_backward<T, PER, H, PAD>), dim3((unsigned)(p.groups * p.across)), dim3(waves * kWave), lds, stream, d);

@@ -7,7 +7,9 @@ time, and a training pass reads whole segments of a rollout at once.  A layer is
 
     x + out(scan(conv(v), gate z)),    v, z = in(norm(x))
 
-with B, C and the step width d of the scan read off conv(v) (sequence.py has the operators)."""
+with B, C and the step width d of the scan read off conv(v) (sequence.py has the operators).  The layer and its initialisation (decay
+rates 1 .. states, step widths spread log-uniformly over 0.001 .. 0.1 through the inverse of softplus, step widths of a rank of a
+sixteenth of the width) are those published by A. Gu and T. Dao, "Linear-Time Sequence Modeling with Selective State Spaces", 2023."""
 from __future__ import annotations
 
 import math

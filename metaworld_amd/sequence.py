@@ -16,6 +16,10 @@ others' inputs are not looked at, their outputs and gradients are zero, and the 
 counts.  Gradients are deterministic (no atomic additions) and not differentiable again (create_graph is refused, as are forward
 derivatives).  A call gives the same values to the last bit whether it is recorded for them or not.
 
+Infinities and NaN in inputs that count give what the formulas give token by token; no padding of a width, of a number of states or of a
+row adds a NaN to an output.  Of the gradients that holds for those that are numbers by the formulas; another may be NaN where the
+formula has an infinity.  Rates A above zero let states grow: they pass the range of a number where they do token by token.
+
 Calls are no operations that torch knows: they run inside torch.compile's programs between its graphs, and raise where torch records
 its operations (torch.jit.trace, torch.fx), which would hold their outputs' memory and not the kernels that fill it.
 """
